@@ -1,0 +1,1038 @@
+// Kernels over the whole vocabulary for MI355X (gfx950, CDNA4):
+//
+//   * softmax cross entropy of N rows h against a table w of V rows, without
+//     the scores [N, V] in memory, and its gradient
+//       s_nv = <h_n, w_v>          lse_n  = log sum_v exp s_nv
+//       loss_n = lse_n - s_n,y(n)  c_nv   = g_n (exp(s_nv - lse_n) - [v=y(n)])
+//       dh = c w                   dw     = c^T h
+//   * rows in 8-bit floats (e4m3) with a power-of-two scale for each block of
+//     128 columns, and the product of such rows.
+//
+// All of them are matrix products whose one side is the table, so they share
+// one tile: 128 table rows x 128 sample rows per workgroup of four waves,
+// 64 x 64 per wave in 16x16 MFMA blocks, with the table's rows as the
+// instruction's M side.  A lane then holds four neighbouring table rows of
+// ONE sample, so the softmax's running maximum and sum stay in the lane until
+// the workgroup's last tile, and scores are stored 4 to an instruction.
+
+#include <hip/hip_runtime.h>
+#include <pybind11/pybind11.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+
+namespace py = pybind11;
+
+#define HIP_CLEAR_ERROR() (void)hipGetLastError()
+#define HIP_CHECK(expr)                                                     \
+  do {                                                                      \
+    hipError_t _e = (expr);                                                 \
+    if (_e != hipSuccess)                                                   \
+      throw std::runtime_error(std::string("HIP error: ") +                 \
+                               hipGetErrorString(_e) + " at " __FILE__ ":" + \
+                               std::to_string(__LINE__));                   \
+  } while (0)
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// exp(s - m) is taken as 2^(s log2e - m log2e) with one rounding of m log2e,
+// which costs at most |m| 2^-25 in the exponent.  Past this |m| the exponent
+// is (s - m) log2e instead: one instruction more, but it cannot overflow.
+constexpr float kFar = 1e6f;
+constexpr int kTile = 128;       // rows of either side per workgroup
+constexpr int kSlab = 128;       // bytes of every row per step of the k loop
+constexpr int kTileBytes = kTile * kSlab;
+
+enum Type { kF32 = 0, kBF16 = 1, kFP8 = 2 };
+
+// Storage of one element, and of one element as the matrix instruction takes
+// it: 8-bit rows are brought to bf16, which holds e4m3 times a power of two
+// exactly.
+template <int T> struct Elem;
+template <> struct Elem<kF32> { using S = float; static constexpr int size = 4; };
+template <> struct Elem<kBF16> { using S = uint16_t; static constexpr int size = 2; };
+template <> struct Elem<kFP8> { using S = uint8_t; static constexpr int size = 1; };
+
+// Rows of a matrix in global memory.  `vec`: every row starts at a multiple
+// of 16 bytes.
+struct Rows {
+  const char* p;
+  int64_t ld;      // bytes from row to row
+  int64_t rows;
+  int kb;          // bytes of a row
+  int vec;
+  const uint8_t* scales;   // 8-bit rows: exponents + 127, one per 128 columns
+  int64_t lds;             // scales from row to row
+};
+
+__device__ __forceinline__ float bf16_to_f32(uint16_t h) {
+  return __uint_as_float((uint32_t)h << 16);
+}
+__device__ __forceinline__ float exp_of(float x) {
+  return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+// Joins two (maximum, sum of exp(s - maximum)).
+__device__ __forceinline__ void join(float& top, float& sum, float t, float s) {
+  const float next = fmaxf(top, t);
+  const float ref = next == -INFINITY ? 0.f : next;
+  sum = sum * exp_of(top - ref) + s * exp_of(t - ref);
+  top = next;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  bf16x2 v;
+  v[0] = (__bf16)a;
+  v[1] = (__bf16)b;
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// 16 bytes of a row from byte `o` on; zeros outside of the matrix.
+template <int ES>
+__device__ __forceinline__ u32x4 load16(const Rows& m, int64_t row, int o) {
+  u32x4 r = {0, 0, 0, 0};
+  if (row >= m.rows || o >= m.kb) return r;
+  const char* q = m.p + row * m.ld + o;
+  if (m.vec && o + 16 <= m.kb) return *reinterpret_cast<const u32x4*>(q);
+  const int have = (m.kb - o) / ES;
+  if (ES == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < have) r[i] = reinterpret_cast<const uint32_t*>(q)[i];
+  } else if (ES == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < have)
+        r[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[i] << (16 * (i & 1));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < have) r[i >> 2] |= (uint32_t)(uint8_t)q[i] << (8 * (i & 3));
+  }
+  return r;
+}
+
+__device__ __forceinline__ float scale_of(uint8_t e) {
+  // e8m0: 2^(e - 127); the quantiser writes 7..247, others are clamped into
+  // the exponents of normal numbers
+  const int c = e < 1 ? 1 : e > 254 ? 254 : e;
+  return __uint_as_float((uint32_t)c << 23);
+}
+
+// 4 e4m3 values to bf16, times a power of two: exact.
+__device__ __forceinline__ u32x2 fp8x4_to_bf16(uint32_t v, float scale) {
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
+  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+  u32x2 r;
+  r[0] = pack_bf16(lo[0] * scale, lo[1] * scale);
+  r[1] = pack_bf16(hi[0] * scale, hi[1] * scale);
+  return r;
+}
+
+// One step of the product: 16 bytes of k of each side per lane.  A lane's
+// bytes are k = 16 * (lane >> 4) bytes of 64; as both sides take the same
+// order of k, any order is right.
+template <int T>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (T == kF32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]),
+                                               __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+}
+
+// LDS tile with k along its rows: 128 rows of 8 chunks of 16 bytes.  Chunk c
+// of row r lies at c ^ (r & 7), so that 8 lanes reading one chunk of 8 rows
+// touch different banks.
+__device__ __forceinline__ int row_slot(int r, int c) {
+  return r * kSlab + ((c ^ (r & 7)) << 4);
+}
+
+// A [128 rows x slab] tile on its way to LDS, held in registers meanwhile.
+template <int T>
+struct RowTile {
+  static constexpr int kLoads = T == kFP8 ? 2 : 4;
+  u32x4 v[kLoads];
+  float scale[T == kFP8 ? 2 : 1];
+
+  __device__ __forceinline__ void load(const Rows& m, int64_t row0, int slab) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = threadIdx.x + 256 * i;
+      if constexpr (T == kFP8) {
+        // 64 columns to a slab once they are bf16: 4 chunks of 16
+        const int64_t row = row0 + (q >> 2);
+        v[i] = load16<1>(m, row, slab * 64 + (q & 3) * 16);
+        scale[i] = row < m.rows ? scale_of(m.scales[row * m.lds + (slab >> 1)]) : 0.f;
+      } else {
+        v[i] = load16<Elem<T>::size>(m, row0 + (q >> 3), slab * kSlab + (q & 7) * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = threadIdx.x + 256 * i;
+      if constexpr (T == kFP8) {
+        const int r = q >> 2, c = (q & 3) * 2;
+        const u32x2 a = fp8x4_to_bf16(v[i][0], scale[i]), b = fp8x4_to_bf16(v[i][1], scale[i]);
+        const u32x2 d = fp8x4_to_bf16(v[i][2], scale[i]), e = fp8x4_to_bf16(v[i][3], scale[i]);
+        *reinterpret_cast<u32x4*>(lds + row_slot(r, c)) = u32x4{a[0], a[1], b[0], b[1]};
+        *reinterpret_cast<u32x4*>(lds + row_slot(r, c + 1)) = u32x4{d[0], d[1], e[0], e[1]};
+      } else {
+        *reinterpret_cast<u32x4*>(lds + row_slot(q >> 3, q & 7)) = v[i];
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Scores: tiles of <table row, sample row>, and what is done with them.
+// ---------------------------------------------------------------------------
+enum Use { kLoss = 0, kCoef = 1, kStore = 2 };
+
+struct ScoreArgs {
+  Rows w, h;
+  int tiles_n, splits;      // tiles of samples; parts of the table's range
+  int64_t v_begin, v_end;   // the table rows of this launch
+  // kLoss: (max, sum of exp(s - max)) per part and sample
+  float2* part;
+  // kCoef
+  const void* targets;
+  int targets64;
+  int64_t ignore;
+  const float* lse;
+  const float* grad;
+  int grad_step;
+  const float* weight;      // one factor for all samples, or null
+  char* coef;               // [N][ldc], column 0 = table row v_begin
+  int64_t ldc;
+  // kStore
+  const float* col_scale;
+  char* out;
+  int64_t ldo;
+  int out_bf16;
+};
+
+__device__ __forceinline__ int64_t target_of(const void* t, int is64, int64_t n) {
+  return is64 ? reinterpret_cast<const int64_t*>(t)[n]
+              : (int64_t) reinterpret_cast<const int32_t*>(t)[n];
+}
+
+template <int TW, int TH, int USE>
+__global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
+  __shared__ __align__(16) char lds[2][2][kTileBytes];
+  constexpr int TC = TH;                       // what the instruction takes
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int r16 = lane & 15, g = lane >> 4;
+  // Workgroups go round the 8 XCDs; those of one XCD take all sample tiles of
+  // one part of the table before the next part, so that its L2 gets each
+  // table row from memory once.
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int tn = at % a.tiles_n, split = (at / a.tiles_n) * 8 + xcd;
+  if (split >= a.splits) return;
+  const int64_t tiles = (a.v_end - a.v_begin + kTile - 1) / kTile;
+  const int64_t t0 = tiles * split / a.splits, t1 = tiles * (split + 1) / a.splits;
+  const int64_t n0 = (int64_t)tn * kTile;
+  const int kb = a.h.kb;
+  const int slabs = (kb + kSlab - 1) / kSlab;
+
+  float top[4], sum[4];                        // kLoss
+  float lse[4], gg[4];                         // kCoef
+  int64_t yy[4];
+  if constexpr (USE == kLoss) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = -INFINITY, sum[j] = 0.f;
+  }
+  if constexpr (USE == kCoef) {
+    const float wt = a.weight ? *a.weight : 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = n0 + wn * 64 + j * 16 + r16;
+      lse[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
+      if (n < a.h.rows) {
+        const int64_t y = target_of(a.targets, a.targets64, n);
+        if (y != a.ignore && y >= 0 && y < a.w.rows) {
+          yy[j] = y;
+          lse[j] = a.lse[n];
+          gg[j] = a.grad[n * a.grad_step] * wt;
+        }
+      }
+    }
+  }
+
+  RowTile<TW> sw;
+  RowTile<TH> sh;
+  f32x4 acc[4][4];
+  const int64_t steps = (t1 - t0) * slabs;
+  int64_t tile = t0;
+  int slab = 0;
+  if (steps > 0) {
+    sw.load(a.w, a.v_begin + t0 * kTile, 0);
+    sh.load(a.h, n0, 0);
+    sw.store(lds[0][0]);
+    sh.store(lds[0][1]);
+  }
+  for (int64_t it = 0; it < steps; ++it) {
+    if (slab == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __syncthreads();
+    const bool more = it + 1 < steps;
+    const int next_slab = slab + 1 == slabs ? 0 : slab + 1;
+    const int64_t next_tile = slab + 1 == slabs ? tile + 1 : tile;
+    if (more) {
+      sw.load(a.w, a.v_begin + next_tile * kTile, next_slab);
+      sh.load(a.h, n0, next_slab);
+    }
+    const char* lw = lds[it & 1][0] + wm * 64 * kSlab;
+    const char* lh = lds[it & 1][1] + wn * 64 * kSlab;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 fa[4], fb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        fa[i] = *reinterpret_cast<const u32x4*>(lw + row_slot(i * 16 + r16, k * 4 + g));
+        fb[i] = *reinterpret_cast<const u32x4*>(lh + row_slot(i * 16 + r16, k * 4 + g));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mma<TC>(fa[i], fb[j], acc[i][j]);
+    }
+    if (slab + 1 == slabs) {
+      const int64_t v0 = a.v_begin + tile * kTile + wm * 64;
+      if constexpr (USE == kLoss) {
+        if (v0 + 64 > a.v_end) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (v0 + i * 16 + 4 * g + e >= a.v_end) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j][e] = -INFINITY;
+              }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float most = acc[0][j][0];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, acc[i][j][e]);
+          const float next = fmaxf(top[j], most);
+          // nothing but -inf so far: any finite reference will do
+          const float at0 = next == -INFINITY ? 0.f : next;
+          float s;
+          if (__any(fabsf(at0) > kFar)) {
+            s = sum[j] * exp_of(top[j] - at0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s += exp_of(acc[i][j][e] - at0);
+          } else {
+            const float ref = at0 * kLog2e;
+            s = sum[j] * __builtin_amdgcn_exp2f(__builtin_fmaf(top[j], kLog2e, -ref));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
+          }
+          sum[j] = s;
+          top[j] = next;
+        }
+      }
+      if constexpr (USE == kCoef) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = n0 + wn * 64 + j * 16 + r16;
+          if (n >= a.h.rows) continue;
+          const float lse2 = lse[j] * kLog2e;
+          const bool far = fabsf(lse[j]) > kFar;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t v = v0 + i * 16 + 4 * g;
+            float c[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // past kFar the logarithm's own rounding may pass 0
+              const float x = far ? fminf(acc[i][j][e] - lse[j], 0.f) * kLog2e
+                                  : __builtin_fmaf(acc[i][j][e], kLog2e, -lse2);
+              float p = __builtin_amdgcn_exp2f(x);
+              if (v + e == yy[j]) p -= 1.f;
+              c[e] = yy[j] < 0 || v + e >= a.v_end ? 0.f : p * gg[j];
+            }
+            const int64_t o = n * a.ldc + (v - a.v_begin);
+            if constexpr (TC == kF32)
+              *reinterpret_cast<f32x4*>(a.coef + o * 4) = f32x4{c[0], c[1], c[2], c[3]};
+            else
+              *reinterpret_cast<u32x2*>(a.coef + o * 2) =
+                  u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+          }
+        }
+      }
+      if constexpr (USE == kStore) {
+        const int es = a.out_bf16 ? 2 : 4;
+        const bool vec = (a.ldo & 3) == 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t v = v0 + i * 16 + 4 * g;
+          float cs[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            cs[e] = a.col_scale && v + e < a.v_end ? a.col_scale[v + e] : 1.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int64_t n = n0 + wn * 64 + j * 16 + r16;
+            if (n >= a.h.rows) continue;
+            char* o = a.out + (n * a.ldo + v) * es;
+            f32x4 s = acc[i][j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] *= cs[e];
+            if (vec && v + 3 < a.v_end) {
+              if (a.out_bf16)
+                *reinterpret_cast<u32x2*>(o) =
+                    u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+              else
+                *reinterpret_cast<f32x4*>(o) = s;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (v + e < a.v_end) {
+                  if (a.out_bf16)
+                    reinterpret_cast<__bf16*>(o)[e] = (__bf16)s[e];
+                  else
+                    reinterpret_cast<float*>(o)[e] = s[e];
+                }
+            }
+          }
+        }
+      }
+    }
+    if (more) {
+      sw.store(lds[(it + 1) & 1][0]);
+      sh.store(lds[(it + 1) & 1][1]);
+    }
+    slab = next_slab;
+    tile = next_tile;
+  }
+
+  if constexpr (USE == kLoss) {
+    // join the four lanes, then the two waves, that hold one sample
+    __syncthreads();
+    float2* red = reinterpret_cast<float2*>(&lds[0][0][0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int m = 16; m < 64; m <<= 1) {
+        const float t = __shfl_xor(top[j], m), s = __shfl_xor(sum[j], m);
+        join(top[j], sum[j], t, s);
+      }
+      if (g == 0) red[wave * 64 + j * 16 + r16] = make_float2(top[j], sum[j]);
+    }
+    __syncthreads();
+    if (threadIdx.x < kTile) {
+      const int half = threadIdx.x >> 6, c = threadIdx.x & 63;
+      float2 p = red[(half * 2) * 64 + c];
+      const float2 q = red[(half * 2 + 1) * 64 + c];
+      join(p.x, p.y, q.x, q.y);
+      a.part[(int64_t)split * a.tiles_n * kTile + n0 + threadIdx.x] = p;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the parts of one sample's softmax and takes its target's score off:
+// one wave per sample, four to a workgroup.
+// ---------------------------------------------------------------------------
+template <int T>
+__device__ __forceinline__ float elem(const char* p, int64_t i) {
+  if constexpr (T == kF32) return reinterpret_cast<const float*>(p)[i];
+  else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void loss_join_kernel(
+    Rows w, Rows h, const float2* part, int splits, int64_t ldp,
+    const void* targets, int targets64, int64_t ignore, float* loss, float* lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= h.rows) return;
+  float top = -INFINITY, sum = 0.f;
+  for (int s = lane; s < splits; s += 64) {
+    const float2 p = part[s * ldp + n];
+    join(top, sum, p.x, p.y);
+  }
+  const int64_t y = target_of(targets, targets64, n);
+  const bool ours = y != ignore && y >= 0 && y < w.rows;
+  float right = 0.f;
+  if (ours) {
+    const char* wr = w.p + y * w.ld;
+    const char* hr = h.p + n * h.ld;
+    for (int k = lane; k < h.kb / Elem<T>::size; k += 64)
+      right = __builtin_fmaf(elem<T>(wr, k), elem<T>(hr, k), right);
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const float t = __shfl_xor(top, m), s = __shfl_xor(sum, m);
+    right += __shfl_xor(right, m);
+    join(top, sum, t, s);
+  }
+  if (lane == 0) {
+    const float total = top + log2f(sum) * kLn2;
+    lse[n] = total;
+    loss[n] = y == ignore ? 0.f : ours ? total - right : NAN;
+  }
+}
+
+// Sum or mean over the samples that count, in 64 bits and a fixed order.
+// out[0] = the sum times out[1]; out[1] = 1 / count for the mean, 1 for the sum.
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(
+    const float* loss, const void* targets, int targets64, int64_t ignore,
+    int64_t n, int mean, float* out) {
+  __shared__ double sums[16];
+  __shared__ long long counts[16];
+  double s = 0;
+  long long c = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+    if (target_of(targets, targets64, i) != ignore) s += loss[i], ++c;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m), c += __shfl_xor(c, m);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i];
+    const double f = mean ? 1.0 / (double)c : 1.0;
+    out[0] = (float)(s * f);
+    out[1] = (float)f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products with the coefficients: out[r][d] = sum_k b(r, k) x[k][d]
+//   dh: r = sample, k = table row, b = coef[r][k]
+//   dw: r = table row, k = sample, b = coef[k][r]
+// x has k down its rows, so its tile is read from LDS transposed, as is b's
+// where it has too.
+// ---------------------------------------------------------------------------
+// LDS tile with k down its rows, 128 columns: bf16 64 rows of 256 bytes, f32
+// 32 rows of 512 bytes.  Blocks of 16 columns are permuted by the row so that
+// the 16 rows that one transposing read touches spread over the banks.
+template <int T>
+__device__ __forceinline__ int col_slot(int k, int c) {
+  if constexpr (T == kBF16) {
+    const int f = (k & 3) | ((k >> 3) & 1) << 2;
+    return k * 256 + (((c >> 1) ^ f) << 5) + ((c & 1) << 4);
+  } else {
+    return k * 512 + (((c >> 2) ^ ((k >> 2) & 7)) << 6) + ((c & 3) << 4);
+  }
+}
+
+// 16 columns (block m) x one step of k, as the instruction takes them.
+template <int T>
+__device__ __forceinline__ u32x4 col_frag(const char* lds, int m, int step, int lane) {
+  const int g = lane >> 4, i = lane & 15;
+  if constexpr (T == kBF16) {
+    const int k = step * 32 + 8 * g + (i >> 2);
+    const int f = (k & 3) | ((k >> 3) & 1) << 2;
+    const char* p = lds + k * 256 + ((m ^ f) << 5) + (i & 3) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 256));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  } else {
+    const int k = step * 16 + 4 * g;
+    const char* p = lds + k * 512 + ((m ^ ((k >> 2) & 7)) << 6) + i * 4;
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = *reinterpret_cast<const uint32_t*>(p + e * 512);
+    return r;
+  }
+}
+
+template <int T>
+struct ColTile {
+  static constexpr int kRowChunks = 128 * Elem<T>::size / 16;
+  u32x4 v[4];
+  __device__ __forceinline__ void load(const Rows& m, int64_t k0, int col0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = threadIdx.x + 256 * i;
+      v[i] = load16<Elem<T>::size>(m, k0 + q / kRowChunks,
+                                   col0 * Elem<T>::size + (q % kRowChunks) * 16);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = threadIdx.x + 256 * i;
+      *reinterpret_cast<u32x4*>(lds + col_slot<T>(q / kRowChunks, q % kRowChunks)) = v[i];
+    }
+  }
+};
+
+struct GradArgs {
+  Rows x;        // [K][D]
+  Rows b;        // coef: [R][K] or [K][R]
+  int64_t r, k;
+  int d;
+  int tiles_d, tiles_r, splits;
+  float* part;   // dh: [splits][R][ldp], added to where `add`
+  int64_t ldp;
+  int add;
+  char* out;     // dw: [R][D]
+  int64_t ldo;
+};
+
+template <int T, bool DW>
+__global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
+  __shared__ __align__(16) char lds[2][2][kTileBytes];
+  constexpr int ES = Elem<T>::size;
+  constexpr int KS = kSlab / ES;     // k per step of the loop
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int r16 = lane & 15, g = lane >> 4;
+  const int td = blockIdx.x % a.tiles_d;
+  const int tr = (blockIdx.x / a.tiles_d) % a.tiles_r;
+  const int split = blockIdx.x / (a.tiles_d * a.tiles_r);
+  const int64_t slabs = (a.k + KS - 1) / KS;
+  const int64_t s0 = slabs * split / a.splits, s1 = slabs * (split + 1) / a.splits;
+  const int64_t r0 = (int64_t)tr * kTile;
+  const int d0 = td * kTile;
+
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  ColTile<T> sx;
+  ColTile<T> sbc;
+  RowTile<T> sbr;
+  auto load = [&](int64_t s) {
+    sx.load(a.x, s * KS, d0);
+    if constexpr (DW) sbc.load(a.b, s * KS, (int)r0);
+    else sbr.load(a.b, r0, (int)s);
+  };
+  auto store = [&](int buf) {
+    sx.store(lds[buf][0]);
+    if constexpr (DW) sbc.store(lds[buf][1]);
+    else sbr.store(lds[buf][1]);
+  };
+  if (s0 < s1) {
+    load(s0);
+    store(0);
+  }
+  for (int64_t s = s0; s < s1; ++s) {
+    const int buf = (int)(s - s0) & 1;
+    __syncthreads();
+    if (s + 1 < s1) load(s + 1);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 fa[4], fb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        fa[i] = col_frag<T>(lds[buf][0], wm * 4 + i, k, lane);
+        if constexpr (DW)
+          fb[i] = col_frag<T>(lds[buf][1], wn * 4 + i, k, lane);
+        else
+          fb[i] = *reinterpret_cast<const u32x4*>(
+              lds[buf][1] + row_slot(wn * 64 + i * 16 + r16, k * 4 + g));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mma<T>(fa[i], fb[j], acc[i][j]);
+    }
+    if (s + 1 < s1) store(buf ^ 1);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = r0 + wn * 64 + j * 16 + r16;
+    if (r >= a.r) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + wm * 64 + i * 16 + 4 * g;
+      if (d >= a.d) continue;
+      if constexpr (!DW) {
+        f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
+        *o = a.add ? *o + acc[i][j] : acc[i][j];
+      } else {
+        char* o = a.out + (r * a.ldo + d) * ES;
+        if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
+          if constexpr (T == kF32)
+            *reinterpret_cast<f32x4*>(o) = acc[i][j];
+          else
+            *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(acc[i][j][0], acc[i][j][1]),
+                                                 pack_bf16(acc[i][j][2], acc[i][j][3])};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.d) {
+              if constexpr (T == kF32) reinterpret_cast<float*>(o)[e] = acc[i][j][e];
+              else reinterpret_cast<__bf16*>(o)[e] = (__bf16)acc[i][j][e];
+            }
+        }
+      }
+    }
+  }
+}
+
+// dh from its parts.
+template <int T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(
+    const float* part, int splits, int64_t rows, int64_t ldp, int d, char* out) {
+  const int64_t total = rows * d;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / d, c = i - r * d;
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += part[((int64_t)p * rows + r) * ldp + c];
+    if constexpr (T == kF32) reinterpret_cast<float*>(out)[i] = s;
+    else reinterpret_cast<__bf16*>(out)[i] = (__bf16)s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows in 8 bits.  16 lanes take one block of 128 columns, 8 to a lane.
+//   e = the least integer with max|x| <= 448 * 2^e, within [-120, 120]
+//   value = x / 2^e to the nearest e4m3, ties to even; NaN for what is not
+//   finite (the maximum is over the finite ones).  At e = 120 the value stops
+//   at 240: the next one would stand for 2^128, which float32 does not hold
+// TO_BF16 writes the values that the 8-bit rows stand for instead.
+// ---------------------------------------------------------------------------
+template <int T, bool TO_BF16>
+__global__ __launch_bounds__(256) void quantize_kernel(
+    Rows x, int cols, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
+  const int64_t total = x.rows * blocks;
+  const int sub = threadIdx.x & 15;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; i < total;
+       i += (int64_t)gridDim.x * 16) {
+    const int64_t row = i / blocks;
+    const int b = (int)(i - row * blocks);
+    const int c0 = b * 128 + sub * 8;
+    float v[8];
+    if constexpr (T == kBF16) {
+      const u32x4 q = load16<2>(x, row, c0 * 2);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = bf16_to_f32((uint16_t)(q[k >> 1] >> (16 * (k & 1))));
+    } else {
+      const u32x4 q = load16<4>(x, row, c0 * 4), r = load16<4>(x, row, c0 * 4 + 16);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(q[k]), v[4 + k] = __uint_as_float(r[k]);
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = __float_as_uint(v[k]) & 0x7fffffffu;
+      if (m < 0x7f800000u) most = m > most ? m : most;
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+      const uint32_t o = __shfl_xor(most, m);
+      most = o > most ? o : most;
+    }
+    // most = 1.f * 2^q; 448 = 1.75 * 2^8
+    int e = (int)(most >> 23) - 127 - 8 + ((most & 0x7fffffu) > 0x600000u);
+    e = e < -120 ? -120 : e > 120 ? 120 : e;
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float limit = e == 120 ? 240.f : 448.f;
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = __float_as_uint(v[k]) & 0x7fffffffu;
+      v[k] = m < 0x7f800000u ? __builtin_amdgcn_fmed3f(v[k] * inv, -limit, limit) : NAN;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+      w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], r, true);
+    }
+    if constexpr (TO_BF16) {
+      const float s = scale_of((uint8_t)(e + 127));
+      const u32x2 lo = fp8x4_to_bf16(w[0], s), hi = fp8x4_to_bf16(w[1], s);
+      if (c0 < ldv)      // ldv is a multiple of 8; columns past the last are 0
+        *reinterpret_cast<u32x4*>(values + (row * ldv + c0) * 2) =
+            u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      if (c0 < ldv)      // ldv is a multiple of 16
+        *reinterpret_cast<u32x2*>(values + row * ldv + c0) = u32x2{w[0], w[1]};
+      if (sub == 0) scales[row * lds + b] = (uint8_t)(e + 127);
+    }
+  }
+}
+
+template <int TO>
+__global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char* out, int64_t ldo) {
+  const int chunks = (cols + 15) / 16;
+  const int64_t total = x.rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / chunks;
+    const int c = (int)(i - row * chunks) * 16;
+    const u32x4 q = load16<1>(x, row, c);
+    const float s = scale_of(x.scales[row * x.lds + (c >> 7)]);
+    if constexpr (TO == kBF16) {
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x2 t = fp8x4_to_bf16(q[k], s);
+        w[2 * k] = t[0], w[2 * k + 1] = t[1];
+      }
+      uint16_t* o = reinterpret_cast<uint16_t*>(out) + row * ldo + c;
+      if ((ldo & 7) == 0 && c + 16 <= cols) {
+        reinterpret_cast<u32x4*>(o)[0] = u32x4{w[0], w[1], w[2], w[3]};
+        reinterpret_cast<u32x4*>(o)[1] = u32x4{w[4], w[5], w[6], w[7]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (c + k < cols) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+      }
+    } else {
+      float* o = reinterpret_cast<float*>(out) + row * ldo + c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[k], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[k], true);
+        const f32x4 t = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+        if ((ldo & 3) == 0 && c + 4 * k + 4 <= cols) {
+          reinterpret_cast<f32x4*>(o)[k] = t;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + 4 * k + e < cols) o[4 * k + e] = t[e];
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static Rows make_rows(uintptr_t p, int64_t ld_elems, int64_t rows, int64_t cols, int es) {
+  if (rows < 0 || cols < 1 || cols > (1 << 24) || ld_elems < 0)
+    throw std::runtime_error("bad shape");
+  Rows r{};
+  r.p = (const char*)p;
+  r.ld = ld_elems * es;
+  r.rows = rows;
+  r.kb = (int)cols * es;
+  r.vec = (p % 16 == 0) && (r.ld % 16 == 0);
+  return r;
+}
+
+static int grid_of(int64_t blocks) {
+  if (blocks < 1 || blocks > 0x7fffffff) throw std::runtime_error("grid out of range");
+  return (int)blocks;
+}
+
+static int score_grid(const ScoreArgs& a) {
+  return grid_of((int64_t)8 * a.tiles_n * ((a.splits + 7) / 8));
+}
+
+// part: [splits][round_up(n, 128)] pairs of float
+static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
+                         int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
+                         int64_t ignore, int splits, uintptr_t part, uintptr_t loss,
+                         uintptr_t lse, int reduce, uintptr_t reduced, uintptr_t stream_ptr) {
+  HIP_CLEAR_ERROR();
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  const int es = is_bf16 ? 2 : 4;
+  if (n > 0) {
+    ScoreArgs a{};
+    a.w = make_rows(w, ldw, v, d, es);
+    a.h = make_rows(h, ldh, n, d, es);
+    a.tiles_n = grid_of((n + kTile - 1) / kTile);
+    a.splits = splits;
+    a.v_begin = 0;
+    a.v_end = v;
+    a.part = (float2*)part;
+    const int64_t ldp = (int64_t)a.tiles_n * kTile;
+    const int joins = grid_of((n + 3) / 4);
+    if (is_bf16) {
+      scores_kernel<kBF16, kBF16, kLoss><<<score_grid(a), 256, 0, stream>>>(a);
+      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, splits, ldp,
+          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
+    } else {
+      scores_kernel<kF32, kF32, kLoss><<<score_grid(a), 256, 0, stream>>>(a);
+      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, splits, ldp,
+          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
+    }
+  }
+  if (reduce)      // 1: sum, 2: mean
+    loss_reduce_kernel<<<1, 1024, 0, stream>>>((const float*)loss, (const void*)targets,
+                                               targets64, ignore, n, reduce == 2, (float*)reduced);
+  HIP_CHECK(hipGetLastError());
+}
+
+// coef: [n][chunk] elements; part: [splits][n][ldp] floats
+static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
+                         int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
+                         int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
+                         uintptr_t weight, int64_t chunk, uintptr_t coef, int coef_parts,
+                         int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
+                         uintptr_t stream_ptr) {
+  HIP_CLEAR_ERROR();
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  const int es = is_bf16 ? 2 : 4;
+  if (chunk % kTile != 0 || ldp % 4 != 0) throw std::runtime_error("bad workspace shape");
+  if (n == 0) throw std::runtime_error("no rows");
+  const Rows rw = make_rows(w, ldw, v, d, es), rh = make_rows(h, ldh, n, d, es);
+  const int tiles_n = grid_of((n + kTile - 1) / kTile);
+  const int tiles_d = (int)((d + kTile - 1) / kTile);
+  for (int64_t v0 = 0; v0 < v; v0 += chunk) {
+    const int64_t v1 = std::min(v, v0 + chunk);
+    const int tiles_v = grid_of((v1 - v0 + kTile - 1) / kTile);
+    ScoreArgs a{};
+    a.w = rw;
+    a.h = rh;
+    a.tiles_n = tiles_n;
+    a.splits = std::min(coef_parts, tiles_v);
+    a.v_begin = v0;
+    a.v_end = v1;
+    a.targets = (const void*)targets;
+    a.targets64 = targets64;
+    a.ignore = ignore;
+    a.lse = (const float*)lse;
+    a.grad = (const float*)grad;
+    a.grad_step = grad_step;
+    a.weight = (const float*)weight;
+    a.coef = (char*)coef;
+    a.ldc = chunk;
+    if (is_bf16) scores_kernel<kBF16, kBF16, kCoef><<<score_grid(a), 256, 0, stream>>>(a);
+    else scores_kernel<kF32, kF32, kCoef><<<score_grid(a), 256, 0, stream>>>(a);
+    GradArgs b{};
+    b.d = (int)d;
+    b.tiles_d = tiles_d;
+    if (dh) {
+      b.x = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
+      b.b = make_rows(coef, chunk, n, v1 - v0, es);
+      b.r = n;
+      b.k = v1 - v0;
+      b.tiles_r = tiles_n;
+      b.splits = splits;
+      b.part = (float*)part;
+      b.ldp = ldp;
+      b.add = v0 > 0;
+      const int blocks = grid_of((int64_t)tiles_d * tiles_n * splits);
+      if (is_bf16) grad_kernel<kBF16, false><<<blocks, 256, 0, stream>>>(b);
+      else grad_kernel<kF32, false><<<blocks, 256, 0, stream>>>(b);
+    }
+    if (dw) {
+      b.x = rh;
+      b.b = make_rows(coef, chunk, n, v1 - v0, es);
+      b.r = v1 - v0;
+      b.k = n;
+      b.tiles_r = tiles_v;
+      b.splits = 1;
+      b.out = (char*)dw + v0 * d * es;
+      b.ldo = d;
+      const int blocks = grid_of((int64_t)tiles_d * tiles_v);
+      if (is_bf16) grad_kernel<kBF16, true><<<blocks, 256, 0, stream>>>(b);
+      else grad_kernel<kF32, true><<<blocks, 256, 0, stream>>>(b);
+    }
+  }
+  if (dh) {
+    const int blocks = (int)std::min<int64_t>((n * d + 255) / 256, 4096);
+    if (is_bf16) sum_parts_kernel<kBF16><<<blocks, 256, 0, stream>>>(
+        (const float*)part, splits, n, ldp, (int)d, (char*)dh);
+    else sum_parts_kernel<kF32><<<blocks, 256, 0, stream>>>(
+        (const float*)part, splits, n, ldp, (int)d, (char*)dh);
+  }
+  HIP_CHECK(hipGetLastError());
+}
+
+// to_bf16: values are bf16 rows, no scales are written
+static void quantize_rows(uintptr_t x, int64_t ldx, int64_t rows, int64_t cols, int is_bf16,
+                          uintptr_t values, int64_t ldv, uintptr_t scales, int64_t lds,
+                          int to_bf16, uintptr_t stream_ptr) {
+  HIP_CLEAR_ERROR();
+  if (rows == 0) return;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  if (ldv % (to_bf16 ? 8 : 16) != 0 || ldv < cols || values % 16 != 0)
+    throw std::runtime_error("bad layout of the values");
+  const Rows r = make_rows(x, ldx, rows, cols, is_bf16 ? 2 : 4);
+  const int blocks = (int)((cols + 127) / 128);
+  const int grid = (int)std::min<int64_t>((rows * blocks + 15) / 16, 8192);
+  auto go = [&](auto kernel) {
+    kernel<<<grid, 256, 0, stream>>>(r, (int)cols, blocks, (char*)values, ldv,
+                                     (uint8_t*)scales, lds);
+  };
+  if (is_bf16) to_bf16 ? go(quantize_kernel<kBF16, true>) : go(quantize_kernel<kBF16, false>);
+  else to_bf16 ? go(quantize_kernel<kF32, true>) : go(quantize_kernel<kF32, false>);
+  HIP_CHECK(hipGetLastError());
+}
+
+static Rows make_fp8(uintptr_t values, int64_t ldv, uintptr_t scales, int64_t lds, int64_t rows,
+                     int64_t cols) {
+  Rows r = make_rows(values, ldv, rows, cols, 1);
+  r.scales = (const uint8_t*)scales;
+  r.lds = lds;
+  return r;
+}
+
+static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int64_t lds,
+                            int64_t rows, int64_t cols, int is_bf16, uintptr_t out, int64_t ldo,
+                            uintptr_t stream_ptr) {
+  HIP_CLEAR_ERROR();
+  if (rows == 0) return;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  if (out % 16 != 0) throw std::runtime_error("bad layout of the output");
+  const Rows r = make_fp8(values, ldv, scales, lds, rows, cols);
+  const int grid = (int)std::min<int64_t>((rows * ((cols + 15) / 16) + 255) / 256, 8192);
+  if (is_bf16) dequantize_kernel<kBF16><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
+  else dequantize_kernel<kF32><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
+  HIP_CHECK(hipGetLastError());
+}
+
+// a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n]
+static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,
+                        uintptr_t scales, int64_t lds, int64_t n, int64_t k, uintptr_t col_scale,
+                        uintptr_t out, int out_bf16, uintptr_t stream_ptr) {
+  HIP_CLEAR_ERROR();
+  if (m == 0 || n == 0) return;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  if (out % 16 != 0) throw std::runtime_error("bad layout of the output");
+  ScoreArgs a{};
+  a.w = make_fp8(values, ldv, scales, lds, n, k);
+  a.h = make_rows(a_ptr, lda, m, k, 2);
+  a.tiles_n = grid_of((m + kTile - 1) / kTile);
+  const int64_t tiles_v = (n + kTile - 1) / kTile;
+  a.splits = (int)std::min<int64_t>(tiles_v, std::max<int64_t>(8, 4096 / a.tiles_n));
+  a.v_begin = 0;
+  a.v_end = n;
+  a.col_scale = (const float*)col_scale;
+  a.out = (char*)out;
+  a.ldo = n;
+  a.out_bf16 = out_bf16;
+  scores_kernel<kFP8, kBF16, kStore><<<score_grid(a), 256, 0, stream>>>(a);
+  HIP_CHECK(hipGetLastError());
+}
+
+PYBIND11_MODULE(_vocab_native, m) {
+  m.doc() = "MI355X (gfx950) kernels over the whole vocabulary";
+  m.def("softmax_loss", &softmax_loss);
+  m.def("softmax_grad", &softmax_grad);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("dequantize_rows", &dequantize_rows);
+  m.def("matmul_rows", &matmul_rows);
+}

@@ -5,9 +5,10 @@
 Builds:
   * glint_word2vec_amd._cpu_native     — pybind11 CPU SGNS trainer (always)
   * glint_word2vec_amd._hip_native     — HIP/CDNA4 fused kernels for gfx950
+  * glint_word2vec_amd._vocab_native   — HIP/CDNA4 whole-vocabulary kernels
     (whenever hipcc is available; cross-compiles fine without a GPU)
 
-The HIP extension is compiled by driving hipcc directly (not through
+The HIP extensions are compiled by driving hipcc directly (not through
 torch.utils.cpp_extension's JIT cache) so the resulting .so lives in-tree
 and travels with the repo snapshot to the GPU box.
 """
@@ -32,8 +33,13 @@ cpu_ext = Extension(
 )
 
 
-def build_hip_extension(force: bool = False) -> str | None:
-    """Compile the HIP extension in-tree with hipcc for gfx950.
+HIP_EXTENSIONS = {"_hip_native": "sgns_hip.hip",
+                  "_vocab_native": "vocab_hip.hip"}
+
+
+def build_hip_extension(name: str = "_hip_native",
+                        force: bool = False) -> str | None:
+    """Compile one HIP extension in-tree with hipcc for gfx950.
 
     Returns the path of the built .so, or None when hipcc is unavailable.
     Deliberately bypasses torch's JIT extension cache: the .so must live
@@ -44,14 +50,16 @@ def build_hip_extension(force: bool = False) -> str | None:
         return None
     import sysconfig
     ext_suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    src = os.path.join(ROOT, "csrc", "hip", "sgns_hip.hip")
-    out = os.path.join(PKG, "_hip_native" + ext_suffix)
+    src = os.path.join(ROOT, "csrc", "hip", HIP_EXTENSIONS[name])
+    out = os.path.join(PKG, name + ext_suffix)
     if not force and os.path.exists(out) and \
             os.path.getmtime(out) > os.path.getmtime(src):
         return out
     cmd = [
         hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
         "-shared", "-fvisibility=hidden",
+        # packed 32-bit float instructions stay off: scalar code only
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I", pybind11.get_include(),
         "-I", sysconfig.get_paths()["include"],
         "-x", "hip", src,
@@ -65,7 +73,8 @@ def build_hip_extension(force: bool = False) -> str | None:
 class BuildExt(build_ext):
     def run(self):
         super().run()
-        build_hip_extension()
+        for name in HIP_EXTENSIONS:
+            build_hip_extension(name)
 
 
 setup(

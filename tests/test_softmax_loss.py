@@ -1,0 +1,396 @@
+"""Softmax cross entropy over the whole vocabulary against a plain float64
+form.  Tolerances count roundings: a product's sum of D terms in float32 is off
+by at most D * 2^-24 of the sum of absolute terms, a stored number by half a
+step of its type."""
+import math
+
+import pytest
+import torch
+
+from glint_word2vec_amd.ops import softmax as S
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _inputs(n, v, d, dtype, seed=0, spread=1.5, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, d, generator=g) * spread / d ** 0.25
+    w = torch.randn(v, d, generator=g) * spread / d ** 0.25
+    y = torch.randint(0, v, (n,), generator=g)
+    return h.to(dtype).to(device), w.to(dtype).to(device), y.to(device)
+
+
+def _reference(h, w, y, ignore=-1, grad=None):
+    """Loss, lse, dh, dw of sum grad_n loss_n in float64, and how far the
+    kernels' may be from them."""
+    bf16 = h.dtype == torch.bfloat16
+    h, w, y = h.double().cpu(), w.double().cpu(), y.long().cpu()
+    n, d = h.shape
+    v = w.shape[0]
+    s = h @ w.T
+    # one score: d roundings of the running sum, and the products' own in f32
+    off_s = 2 * (d + 2) * U * (h.abs() @ w.abs().T)
+    lse = torch.logsumexp(s, 1)
+    # the sum over the vocabulary: every lane adds v / 8 terms or fewer, its
+    # exponentials are off by 2 steps and by the score's error
+    most = off_s.amax(1) if n else off_s.new_zeros(0)
+    off_lse = most + (v / 8 + 64) * U + 8 * U * (lse.abs() + 1) \
+        + 4 * U * s.abs().amax(1)
+    kept = y != ignore
+    yy = y.clamp(0, v - 1)
+    loss = torch.where(kept, lse - s.gather(1, yy[:, None])[:, 0], 0.0)
+    off_loss = off_lse + most + 2 * U * loss.abs()
+    if grad is None:
+        return loss, lse, off_loss, off_lse
+    grad = grad.double().cpu().expand(n) * kept
+    p = torch.exp(s - lse[:, None])
+    c = p.clone()
+    c[torch.arange(n), yy] -= 1
+    c = c * grad[:, None]
+    off_c = p * grad.abs()[:, None] * (
+        2 * (off_s + off_lse[:, None]) + 16 * U) + 4 * U * c.abs()
+    if bf16:
+        off_c = off_c + 2.0 ** -8 * (c.abs() + off_c)
+    step = 2.0 ** -8 if bf16 else U
+    dh, dw = c @ w, c.T @ h
+    off_dh = (off_c + 2 * (v + 2) * U * c.abs()) @ w.abs()
+    off_dw = (off_c + 2 * (n + 2) * U * c.abs()).T @ h.abs()
+    off_dh = off_dh + step * (dh.abs() + off_dh) + 1e-38
+    off_dw = off_dw + step * (dw.abs() + off_dw) + 1e-38
+    return loss, lse, off_loss, off_lse, dh, dw, off_dh, off_dw
+
+
+def _near(got, want, off, what):
+    got = got.double().cpu()
+    assert got.shape == want.shape
+    bad = (got - want).abs() > off
+    bad |= got.isnan()
+    assert not bad.any(), (
+        f"{what}: {int(bad.sum())} of {bad.numel()} off, worst "
+        f"{float(((got - want).abs() / off).max()):.3g} of the tolerance")
+
+
+def _check(h, w, y, ignore=-1, seed=1):
+    g = torch.randn(len(h), generator=torch.Generator().manual_seed(seed))
+    g = g.to(h.device)
+    loss, lse, ol, oe, dh, dw, oh, ow = _reference(h, w, y, ignore, g)
+    got, got_lse = S.softmax_loss_forward(h, w, y, ignore_index=ignore)
+    _near(got, loss, ol, "loss")
+    _near(got_lse, lse, oe, "lse")
+    a, b = S.softmax_loss_backward(h, w, y, got_lse, g, ignore_index=ignore)
+    assert a.dtype == h.dtype and b.dtype == w.dtype
+    _near(a, dh, oh, "dh")
+    _near(b, dw, ow, "dw")
+
+
+SHAPES = [(1, 1, 1), (1, 2, 3), (2, 127, 8), (3, 128, 100), (1, 129, 301),
+          (127, 129, 64), (128, 256, 128), (129, 257, 300), (17, 1000, 520),
+          (200, 3613, 100), (300, 5000, 65), (64, 777, 1024), (5, 300, 2048)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v,d", SHAPES)
+def test_matches_float64(n, v, d, dtype):
+    _check(*_inputs(n, v, d, dtype, seed=n + v + d))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_pieces_of_the_vocabulary(dtype, monkeypatch):
+    monkeypatch.setattr(S, "_COEF_BYTES", 1 << 16)
+    _check(*_inputs(70, 1500, 96, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_offsets(dtype):
+    """Padded rows with NaN behind the last column and above and below the
+    rows, odd starts, and columns that are not neighbours."""
+    n, v, d = 37, 200, 75
+    h, w, y = _inputs(n, v, d, dtype)
+
+    def inside(t, before, after):
+        big = torch.full((t.shape[0] + 2, t.shape[1] + before + after),
+                         math.nan, dtype=t.dtype, device=t.device)
+        big[1:-1, before:before + t.shape[1]] = t
+        return big[1:-1, before:before + t.shape[1]]
+    for before, after in ((0, 5), (0, 6), (8, 5), (1, 4), (3, 0)):
+        _check(inside(h, before, after), inside(w, before, after), y)
+    _check(h.T.contiguous().T, w.T.contiguous().T, y)
+    _check(h[::2], w, y[::2])
+    _check(h, w.flip(0)[::3], y % 67)
+    _check(h[:1].expand(n, d), w, y)
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+@pytest.mark.parametrize("ignore", [-1, -100, 0, 5])
+def test_ignored_targets(kind, ignore):
+    h, w, y = _inputs(150, 90, 40, torch.bfloat16)
+    y[::3] = ignore
+    _check(h, w, y.to(kind), ignore)
+    y[:] = ignore
+    _check(h, w, y.to(kind), ignore)
+
+
+@gpu
+def test_targets_out_of_range_give_nan_and_no_gradient():
+    h, w, y = _inputs(140, 50, 24, torch.float32)
+    y[3], y[100], y[7] = 50, -2, 2 ** 40
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    assert loss.isnan().nonzero().flatten().tolist() == [3, 7, 100]
+    assert lse.isfinite().all()
+    dh, dw = S.softmax_loss_backward(h, w, y, lse,
+                                     torch.ones(140, device="cuda"))
+    good = torch.ones(140, dtype=torch.bool)
+    good[[3, 7, 100]] = False
+    assert (dh[~good] == 0).all()
+    _, _, _, _, dh2, dw2, oh, ow = _reference(h[good], w, y[good],
+                                              grad=torch.ones(()))
+    _near(dh[good], dh2, oh, "dh")
+    _near(dw, dw2, ow, "dw")
+
+
+@gpu
+def test_extreme_scores():
+    """Scores far apart and far from 0 neither overflow nor vanish."""
+    h, w, y = _inputs(40, 300, 16, torch.float32, spread=60.0)
+    s = h.double() @ w.double().T
+    assert s.abs().max() > 5000
+    _check(h, w, y)
+    one = torch.zeros(4, 8, device="cuda")
+    one[:, 0] = torch.tensor([1e18, -1e18, 3e4, 0.0])
+    t = torch.zeros(130, 8, device="cuda")
+    t[:, 0] = -1e18
+    t[129, 0] = -2e18
+    loss, lse = S.softmax_loss_forward(one, t, torch.tensor(
+        [0, 129, 0, 0], device="cuda"))
+    assert lse.tolist()[:2] == pytest.approx([-1e36, 2e36], rel=1e-6)
+    assert loss[1].item() == pytest.approx(0, abs=2e36 * 2 ** -22)
+    assert lse[3].item() == pytest.approx(math.log(130), rel=1e-6)
+
+
+@gpu
+def test_rows_that_are_not_finite_stay_alone():
+    h, w, y = _inputs(130, 64, 32, torch.bfloat16)
+    h[5, 3] = math.nan
+    h[129, 0] = math.inf
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    good = torch.ones(130, dtype=torch.bool)
+    good[[5, 129]] = False
+    assert loss[~good].isnan().all()
+    a, b, oa, ob = _reference(h[good], w, y[good])
+    _near(loss[good], a, oa, "loss")
+    _near(lse[good], b, ob, "lse")
+    # cut off by their targets, they leave the table's gradient alone
+    y[[5, 129]] = -1
+    dh, dw = S.softmax_loss_backward(h, w, y, lse, torch.ones((),
+                                                              device="cuda"))
+    r = _reference(h[good], w, y[good], grad=torch.ones(()))
+    _near(dh[good], r[4], r[6], "dh")
+    # h = NaN times a coefficient of 0 is what the formula says for row 5:
+    # such rows have to be cut out of h, the targets alone do not do it
+    assert dw[:, 4:].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_autograd(reduction, dtype):
+    h, w, y = _inputs(75, 410, 50, dtype)
+    y[::4] = -1
+    h.requires_grad_()
+    w.requires_grad_()
+    up = torch.linspace(-1, 2, 75, device="cuda") if reduction == "none" \
+        else torch.tensor(1.7, device="cuda")
+    loss = S.softmax_loss(h, w, y, reduction=reduction)
+    loss.backward(up)
+    kept = int((y >= 0).sum())
+    g = up if reduction != "mean" else up / kept
+    each, _, off, _, dh, dw, oh, ow = _reference(h.detach(), w.detach(), y,
+                                                 grad=g)
+    if reduction == "none":
+        _near(loss.detach(), each, off, "loss")
+    else:
+        f = 1 if reduction == "sum" else 1 / kept
+        _near(loss.detach(), each.sum() * f,
+              off.sum() * f + 2 * U * each.sum() * f, "loss")
+    _near(h.grad, dh, oh + 4 * U * dh.abs(), "dh")
+    _near(w.grad, dw, ow + 4 * U * dw.abs(), "dw")
+
+
+@gpu
+def test_gradient_against_differences():
+    """(L(h + e u) - L(h - e u)) / 2e against <dh, u>, and the same for w."""
+    h, w, y = _inputs(20, 60, 12, torch.float32, spread=1.0)
+    e = 2.0 ** -6
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    dh, dw = S.softmax_loss_backward(h, w, y, lse,
+                                     torch.ones((), device="cuda"))
+    g = torch.Generator().manual_seed(3)
+    for which in ("h", "w"):
+        u = torch.randn(h.shape if which == "h" else w.shape,
+                        generator=g).cuda()
+        both = []
+        for sign in (1, -1):
+            a = h + sign * e * u if which == "h" else h
+            b = w + sign * e * u if which == "w" else w
+            both.append(S.softmax_loss_forward(a, b, y)[0].double().sum())
+        got = (both[0] - both[1]) / (2 * e)
+        want = ((dh if which == "h" else dw).double() * u.double()).sum()
+        # along u, the scores move by t and the third derivative of their
+        # log-sum-exp is t's third central moment under the softmax.  For
+        # numbers within a range R that is at most R^3 max_q q (1-q) |1-2q|
+        # = R^3 / (6 sqrt 3): all weight on the two ends.
+        t = (u @ w.T if which == "h" else h @ u.T).double()
+        wide = t.amax(1) - t.amin(1)
+        off = e * e / 6 * (wide ** 3).sum() / (6 * math.sqrt(3)) \
+            + 20 * 64 * U * float(loss.abs().max() + 8) / e
+        assert abs(got - want) < off
+        assert off < 0.2 * abs(want) + 0.5
+
+
+@gpu
+def test_no_rows():
+    h, w, y = _inputs(0, 30, 10, torch.float32)
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    assert loss.shape == lse.shape == (0,)
+    dh, dw = S.softmax_loss_backward(h, w, y, lse, torch.zeros(0).cuda())
+    assert dh.shape == (0, 10) and (dw == 0).all() and dw.shape == (30, 10)
+    assert S.softmax_loss(h, w, y, reduction="sum").item() == 0
+    assert math.isnan(S.softmax_loss(h, w, y).item())
+
+
+@gpu
+def test_only_what_is_needed():
+    h, w, y = _inputs(60, 200, 30, torch.bfloat16)
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    one = torch.ones((), device="cuda")
+    dh, dw = S.softmax_loss_backward(h, w, y, lse, one)
+    a, none = S.softmax_loss_backward(h, w, y, lse, one, need_w=False)
+    assert none is None and torch.equal(a, dh)
+    none, b = S.softmax_loss_backward(h, w, y, lse, one, need_h=False)
+    assert none is None and torch.equal(b, dw)
+    assert S.softmax_loss_backward(h, w, y, lse, one, need_h=False,
+                                   need_w=False) == (None, None)
+    w2 = w.clone().requires_grad_()
+    S.softmax_loss(h, w2, y, reduction="sum").backward()
+    assert torch.equal(w2.grad, dw)
+
+
+@gpu
+def test_the_same_on_every_run_and_on_another_stream():
+    h, w, y = _inputs(333, 2500, 120, torch.bfloat16)
+    one = torch.ones((), device="cuda")
+
+    def once():
+        loss, lse = S.softmax_loss_forward(h, w, y)
+        return (loss, lse, *S.softmax_loss_backward(h, w, y, lse, one))
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b, c in zip(first, second, once()):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@gpu
+def test_captured_step():
+    """A step in a graph gives the eager step's result on every replay, with
+    new inputs and eager work between."""
+    h, w, y = _inputs(100, 900, 72, torch.bfloat16)
+    one = torch.ones((), device="cuda")
+
+    def once(a, b, t):
+        loss, lse = S.softmax_loss_forward(a, b, t)
+        return (loss, *S.softmax_loss_backward(a, b, t, lse, one))
+    sh, sw, sy = h.clone(), w.clone(), y.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once(sh, sw, sy)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, once(sh, sw, sy)))
+    for k in range(4):
+        h, w, y = _inputs(100, 900, 72, torch.bfloat16, seed=10 + k)
+        sh.copy_(h), sw.copy_(w), sy.copy_(y)
+        for graph, out in graphs:
+            graph.replay()
+        want = once(h, w, y)
+        torch.cuda.synchronize()
+        for graph, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+@gpu
+def test_table_past_32_bits():
+    """A table of more than 2^32 bytes, with targets at its end."""
+    v, d = 7_200_000, 320
+    w = torch.empty(v, d, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for a in range(0, v, 900_000):
+        w[a:a + 900_000] = torch.randn(900_000, d, generator=g,
+                                       device="cuda") * 0.2
+    h = torch.randn(3, d, generator=g, device="cuda").to(torch.bfloat16)
+    y = torch.tensor([v - 1, 0, v - 2], device="cuda")
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    parts = [torch.logsumexp(h.double() @ w[a:a + 450_000].double().T, 1)
+             for a in range(0, v, 450_000)]
+    want = torch.logsumexp(torch.stack(parts), 0)
+    right = (h.double() * w[y].double()).sum(1)
+    # sums of v / 8 terms at most: see _reference
+    off = (v / 8 + 64) * U + 2 * (d + 2) * U * float(
+        (h.abs().double() @ w[-1000:].abs().double().T).max()) * 2 + 1e-5
+    assert ((lse - want).abs() < off).all()
+    assert ((loss - (want - right)).abs() < 2 * off).all()
+    # no error of a wrapped offset is that small
+    assert off < 0.1
+
+
+def test_refusals():
+    h, w = torch.zeros(4, 8), torch.zeros(10, 8)
+    y = torch.zeros(4, dtype=torch.long)
+    for bad, error in (
+            (([1.0], w, y), TypeError), ((h, w, [0]), TypeError),
+            ((h[0], w, y), ValueError), ((h, w[0], y), ValueError),
+            ((h, w, y[:, None]), ValueError),
+            ((h, w[:, :7], y), ValueError), ((h[:3], w, y), ValueError),
+            ((h, w[:0], y), ValueError), ((h[:, :0], w[:, :0], y), ValueError),
+            ((h.half(), w.half(), y), TypeError),
+            ((h.double(), w.double(), y), TypeError),
+            ((h, w.bfloat16(), y), TypeError),
+            ((h, w, y.to(torch.int16)), TypeError),
+            ((h, w, y.float()), TypeError), ((h, w, y), RuntimeError)):
+        with pytest.raises(error):
+            S.softmax_loss(*bad)
+        with pytest.raises(error):
+            S.softmax_loss_forward(*bad)
+    with pytest.raises(ValueError):
+        S.softmax_loss(h, w, y, reduction="avg")
+    with pytest.raises(RuntimeError):
+        S.softmax_loss_backward(h, w, y, torch.zeros(4), torch.zeros(4))
+
+
+@gpu
+def test_refusals_of_the_backward():
+    h, w, y = _inputs(4, 10, 8, torch.float32)
+    one, lse = torch.ones((), device="cuda"), torch.zeros(4, device="cuda")
+    for bad in ((lse[:3], one), (lse.double(), one), (lse, lse[:3]),
+                (lse, lse[:, None]), (lse, one.half())):
+        with pytest.raises(ValueError):
+            S.softmax_loss_backward(h, w, y, *bad)
+    with pytest.raises(TypeError):
+        S.softmax_loss_backward(h, w, y, lse, 1.0)
+    with pytest.raises(RuntimeError):
+        S.softmax_loss_backward(h, w, y, lse.cpu(), one)
+    with pytest.raises(RuntimeError):
+        S.softmax_loss(h, w.cpu(), y)
