@@ -208,9 +208,10 @@ enum Use { kLoss = 0, kCoef = 1, kStore = 2 };
 struct ScoreArgs {
   Rows w, h;
   int tiles_n, splits;      // tiles of samples; parts of the table's range
-  int64_t v_begin, v_end;   // the table rows of this launch
+  int v_begin, v_end;       // the table rows of this launch
   // kLoss: (max, sum of exp(s - max)) per part and sample
   float2* part;
+  int64_t ldp;              // samples of a part
   // kCoef
   const void* targets;
   int targets64;
@@ -233,6 +234,232 @@ __device__ __forceinline__ int64_t target_of(const void* t, int is64, int64_t n)
               : (int64_t) reinterpret_cast<const int32_t*>(t)[n];
 }
 
+// What a wave does with scores of NS blocks of 16 samples: a lane has sample
+// n + 16 j + (lane & 15) and table rows v + 16 i + 4 (lane >> 4) + e.
+template <int USE, int TC, int NS>
+struct Sink {
+  float top[NS], sum[NS];                      // kLoss
+  float lse[NS], gg[NS];                       // kCoef
+  int yy[NS];                                  // -1: no loss
+
+  __device__ __forceinline__ void start(const ScoreArgs& a, int64_t n) {
+    if constexpr (USE == kLoss) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) top[j] = -INFINITY, sum[j] = 0.f;
+    }
+    if constexpr (USE == kCoef) {
+      const float wt = a.weight ? *a.weight : 1.f;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int64_t m = n + j * 16;
+        lse[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
+        if (m < a.h.rows) {
+          const int64_t y = target_of(a.targets, a.targets64, m);
+          if (y != a.ignore && y >= 0 && y < a.w.rows) {
+            yy[j] = (int)y;
+            lse[j] = a.lse[m];
+            gg[j] = a.grad[m * a.grad_step] * wt;
+          }
+        }
+      }
+    }
+  }
+
+  template <int MR>
+  __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
+                                       int64_t n) {
+    if constexpr (USE == kLoss) take_loss(a, acc, v);
+    if constexpr (USE == kCoef) take_coef(a, acc, v, n);
+    if constexpr (USE == kStore) take_store(a, acc, v, n);
+  }
+
+  template <int MR>
+  __device__ __forceinline__ void take_loss(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v) {
+    if (__any(v + 16 * (MR - 1) + 4 > a.v_end)) {
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v + i * 16 + e >= a.v_end) {
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j][e] = -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      float most = acc[0][j][0];
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, acc[i][j][e]);
+      // The reference moves only when a score is above it, which gets rare.
+      if (__any(most > top[j])) {
+        const float next = fmaxf(top[j], most);
+        sum[j] *= top[j] == -INFINITY ? 0.f : exp_of(top[j] - next);
+        top[j] = next;
+      }
+      // nothing but -inf so far: any finite reference will do
+      const float at0 = top[j] == -INFINITY ? 0.f : top[j];
+      // the new terms are added to each other first: one rounding of the long
+      // sum for all of them
+      float s = 0.f;
+      if (__any(fabsf(at0) > kFar)) {
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s += exp_of(acc[i][j][e] - at0);
+      } else {
+        const float ref = at0 * kLog2e;
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
+      }
+      sum[j] += s;
+    }
+  }
+
+  template <int MR>
+  __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
+                                            int64_t n0) {
+    // from the first of the 16 rows, which is the same in all lanes, offsets
+    // have 32 bits: the coefficients of one launch take 128 MB, or 128 columns
+    constexpr int es = TC == kF32 ? 4 : 2;
+    const int64_t first = n0 - (threadIdx.x & 15);
+    const int64_t uniform = (int64_t)__builtin_amdgcn_readfirstlane((int)first);
+    char* to = a.coef + uniform * a.ldc * es;
+    const uint32_t row_bytes = (uint32_t)(a.ldc * es);
+    const uint32_t at = (threadIdx.x & 15) * row_bytes + (uint32_t)(v - a.v_begin) * es;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const int64_t n = n0 + j * 16;
+      if (n >= a.h.rows) continue;
+      const float lse2 = lse[j] * kLog2e;
+      const bool far = __any(fabsf(lse[j]) > kFar);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        const int vi = v + i * 16;
+        f32x4 c = acc[i][j];
+        if (far) {
+          // the logarithm's own rounding may pass 0 here
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = exp_of(fminf(c[e] - lse[j], 0.f));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], kLog2e, -lse2));
+        }
+        const int right = yy[j] - vi;
+        if (__any((unsigned)right < 4u)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] -= right == e ? 1.f : 0.f;
+        }
+        c *= gg[j];
+        // cut off, whatever its scores are; and behind the last word
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (yy[j] < 0 || vi + e >= a.v_end) c[e] = 0.f;
+        if (vi - a.v_begin >= a.ldc) continue;
+        char* o = to + at + (uint32_t)j * 16 * row_bytes + i * 16 * es;
+        if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(o) = c;
+        else
+          *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+      }
+    }
+  }
+
+  template <int MR>
+  __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
+                                             int64_t n0) {
+    const int es = a.out_bf16 ? 2 : 4;
+    const bool vec = (a.ldo & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      const int vi = v + i * 16;
+      float cs[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        cs[e] = a.col_scale && vi + e < a.v_end ? a.col_scale[vi + e] : 1.f;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int64_t n = n0 + j * 16;
+        if (n >= a.h.rows) continue;
+        char* o = a.out + (n * a.ldo + vi) * es;
+        f32x4 s = acc[i][j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] *= cs[e];
+        if (vec && vi + 3 < a.v_end) {
+          if (a.out_bf16)
+            *reinterpret_cast<u32x2*>(o) =
+                u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+          else
+            *reinterpret_cast<f32x4*>(o) = s;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (vi + e < a.v_end) {
+              if (a.out_bf16)
+                reinterpret_cast<__bf16*>(o)[e] = (__bf16)s[e];
+              else
+                reinterpret_cast<float*>(o)[e] = s[e];
+            }
+        }
+      }
+    }
+  }
+
+  // kLoss, after the last tile: joins the four lanes, then the waves, that
+  // hold one sample.  Wave `wave` has samples from 16 NS (wave / WV) on.
+  template <int WV>
+  __device__ __forceinline__ void finish_loss(const ScoreArgs& a, char* lds, int split,
+                                              int64_t n0) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kCols = NS * 16;
+    float2* red = reinterpret_cast<float2*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+#pragma unroll
+      for (int m = 16; m < 64; m <<= 1) {
+        const float t = __shfl_xor(top[j], m), s = __shfl_xor(sum[j], m);
+        join(top[j], sum[j], t, s);
+      }
+      if (lane < 16) red[wave * kCols + j * 16 + lane] = make_float2(top[j], sum[j]);
+    }
+    __syncthreads();
+    if (threadIdx.x < 4 / WV * kCols) {
+      const int group = threadIdx.x / kCols, c = threadIdx.x % kCols;
+      float2 p = red[group * WV * kCols + c];
+#pragma unroll
+      for (int i = 1; i < WV; ++i) {
+        const float2 q = red[(group * WV + i) * kCols + c];
+        join(p.x, p.y, q.x, q.y);
+      }
+      if (n0 + threadIdx.x < a.h.rows) a.part[split * a.ldp + n0 + threadIdx.x] = p;
+    }
+  }
+};
+
+// The workgroup's tile of samples and part of the table.  Workgroups go round
+// the 8 XCDs; those of one XCD take all sample tiles of one part of the table
+// before the next part, so that its L2 gets each table row from memory once.
+__device__ __forceinline__ bool place(const ScoreArgs& a, int& tn, int& split) {
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  tn = at % a.tiles_n;
+  split = (at / a.tiles_n) * 8 + xcd;
+  return split < a.splits;
+}
+
+// [t0, t1): part `split` of `splits` of the tiles.
+__device__ __forceinline__ void part_of(int tiles, int split, int splits, int& t0, int& t1) {
+  const int each = tiles / splits, more = tiles % splits;
+  t0 = split * each + min(split, more);
+  t1 = t0 + each + (split < more);
+}
+
+// Any type, size and alignment: both sides go through LDS in steps of 128
+// bytes of every row, by way of registers.
 template <int TW, int TH, int USE>
 __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
   __shared__ __align__(16) char lds[2][2][kTileBytes];
@@ -240,47 +467,21 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave & 1, wn = wave >> 1;
   const int r16 = lane & 15, g = lane >> 4;
-  // Workgroups go round the 8 XCDs; those of one XCD take all sample tiles of
-  // one part of the table before the next part, so that its L2 gets each
-  // table row from memory once.
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-  const int tn = at % a.tiles_n, split = (at / a.tiles_n) * 8 + xcd;
-  if (split >= a.splits) return;
-  const int64_t tiles = (a.v_end - a.v_begin + kTile - 1) / kTile;
-  const int64_t t0 = tiles * split / a.splits, t1 = tiles * (split + 1) / a.splits;
+  int tn, split;
+  if (!place(a, tn, split)) return;
+  int t0, t1;
+  part_of((a.v_end - a.v_begin + kTile - 1) / kTile, split, a.splits, t0, t1);
   const int64_t n0 = (int64_t)tn * kTile;
-  const int kb = a.h.kb;
-  const int slabs = (kb + kSlab - 1) / kSlab;
+  const int64_t n = n0 + wn * 64 + r16;
+  const int slabs = (a.h.kb + kSlab - 1) / kSlab;
 
-  float top[4], sum[4];                        // kLoss
-  float lse[4], gg[4];                         // kCoef
-  int64_t yy[4];
-  if constexpr (USE == kLoss) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top[j] = -INFINITY, sum[j] = 0.f;
-  }
-  if constexpr (USE == kCoef) {
-    const float wt = a.weight ? *a.weight : 1.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + wn * 64 + j * 16 + r16;
-      lse[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
-      if (n < a.h.rows) {
-        const int64_t y = target_of(a.targets, a.targets64, n);
-        if (y != a.ignore && y >= 0 && y < a.w.rows) {
-          yy[j] = y;
-          lse[j] = a.lse[n];
-          gg[j] = a.grad[n * a.grad_step] * wt;
-        }
-      }
-    }
-  }
-
+  Sink<USE, TC, 4> sink;
+  sink.start(a, n);
   RowTile<TW> sw;
   RowTile<TH> sh;
   f32x4 acc[4][4];
-  const int64_t steps = (t1 - t0) * slabs;
-  int64_t tile = t0;
+  const int64_t steps = (int64_t)(t1 - t0) * slabs;
+  int tile = t0;
   int slab = 0;
   if (steps > 0) {
     sw.load(a.w, a.v_begin + t0 * kTile, 0);
@@ -298,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
     __syncthreads();
     const bool more = it + 1 < steps;
     const int next_slab = slab + 1 == slabs ? 0 : slab + 1;
-    const int64_t next_tile = slab + 1 == slabs ? tile + 1 : tile;
+    const int next_tile = slab + 1 == slabs ? tile + 1 : tile;
     if (more) {
       sw.load(a.w, a.v_begin + next_tile * kTile, next_slab);
       sh.load(a.h, n0, next_slab);
@@ -318,116 +519,7 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = mma<TC>(fa[i], fb[j], acc[i][j]);
     }
-    if (slab + 1 == slabs) {
-      const int64_t v0 = a.v_begin + tile * kTile + wm * 64;
-      if constexpr (USE == kLoss) {
-        if (v0 + 64 > a.v_end) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (v0 + i * 16 + 4 * g + e >= a.v_end) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j][e] = -INFINITY;
-              }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float most = acc[0][j][0];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = fmaxf(most, acc[i][j][e]);
-          const float next = fmaxf(top[j], most);
-          // nothing but -inf so far: any finite reference will do
-          const float at0 = next == -INFINITY ? 0.f : next;
-          float s;
-          if (__any(fabsf(at0) > kFar)) {
-            s = sum[j] * exp_of(top[j] - at0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s += exp_of(acc[i][j][e] - at0);
-          } else {
-            const float ref = at0 * kLog2e;
-            s = sum[j] * __builtin_amdgcn_exp2f(__builtin_fmaf(top[j], kLog2e, -ref));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
-          }
-          sum[j] = s;
-          top[j] = next;
-        }
-      }
-      if constexpr (USE == kCoef) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t n = n0 + wn * 64 + j * 16 + r16;
-          if (n >= a.h.rows) continue;
-          const float lse2 = lse[j] * kLog2e;
-          const bool far = fabsf(lse[j]) > kFar;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t v = v0 + i * 16 + 4 * g;
-            float c[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // past kFar the logarithm's own rounding may pass 0
-              const float x = far ? fminf(acc[i][j][e] - lse[j], 0.f) * kLog2e
-                                  : __builtin_fmaf(acc[i][j][e], kLog2e, -lse2);
-              float p = __builtin_amdgcn_exp2f(x);
-              if (v + e == yy[j]) p -= 1.f;
-              c[e] = yy[j] < 0 || v + e >= a.v_end ? 0.f : p * gg[j];
-            }
-            const int64_t o = n * a.ldc + (v - a.v_begin);
-            if constexpr (TC == kF32)
-              *reinterpret_cast<f32x4*>(a.coef + o * 4) = f32x4{c[0], c[1], c[2], c[3]};
-            else
-              *reinterpret_cast<u32x2*>(a.coef + o * 2) =
-                  u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
-          }
-        }
-      }
-      if constexpr (USE == kStore) {
-        const int es = a.out_bf16 ? 2 : 4;
-        const bool vec = (a.ldo & 3) == 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t v = v0 + i * 16 + 4 * g;
-          float cs[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            cs[e] = a.col_scale && v + e < a.v_end ? a.col_scale[v + e] : 1.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int64_t n = n0 + wn * 64 + j * 16 + r16;
-            if (n >= a.h.rows) continue;
-            char* o = a.out + (n * a.ldo + v) * es;
-            f32x4 s = acc[i][j];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] *= cs[e];
-            if (vec && v + 3 < a.v_end) {
-              if (a.out_bf16)
-                *reinterpret_cast<u32x2*>(o) =
-                    u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
-              else
-                *reinterpret_cast<f32x4*>(o) = s;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (v + e < a.v_end) {
-                  if (a.out_bf16)
-                    reinterpret_cast<__bf16*>(o)[e] = (__bf16)s[e];
-                  else
-                    reinterpret_cast<float*>(o)[e] = s[e];
-                }
-            }
-          }
-        }
-      }
-    }
+    if (slab + 1 == slabs) sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n);
     if (more) {
       sw.store(lds[(it + 1) & 1][0]);
       sh.store(lds[(it + 1) & 1][1]);
@@ -435,29 +527,190 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
     slab = next_slab;
     tile = next_tile;
   }
+  if constexpr (USE == kLoss) sink.template finish_loss<2>(a, &lds[0][0][0], split, n0);
+}
 
-  if constexpr (USE == kLoss) {
-    // join the four lanes, then the two waves, that hold one sample
-    __syncthreads();
-    float2* red = reinterpret_cast<float2*>(&lds[0][0][0]);
+// 16 bytes a lane from global memory straight into LDS, 1 KB from `lds` on.
+// The hardware counts it as a load; wait_loads() waits for it.
+__device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint32_t lds) {
+  const uint64_t at = (uint64_t)p;
+  const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+
+// Rows of up to 32 KS columns of bf16 (or of 8 bits, on the table's side)
+// that start at multiples of 16 bytes.  A wave holds its 16 NS samples in
+// registers for the whole launch, so that LDS is read for the table alone:
+// one fragment of 16 table rows feeds NS instructions.  Table tiles of kRows
+// rows are loaded straight into LDS, one ahead of the tile at work; two
+// workgroups fit a CU, and one's exponentials run beside the other's
+// products.  WN of the four waves have different samples, the others share
+// them and take different rows of the tile.
+template <int KS, int NS, int WN, int USE, bool FP8>
+__global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
+  constexpr int WV = 4 / WN;
+  constexpr int kRows = KS <= 4 ? 128 : KS <= 10 ? 64 : 32;
+  constexpr int kPitch = KS * (FP8 ? 32 : 64);       // bytes of a row in LDS
+  constexpr int kChunks = kPitch / 16;
+  constexpr int kLoads = kRows / 4 * kChunks / 64;   // per lane and tile
+  constexpr int MR = kRows / WV >= 32 && KS * NS <= 24 ? 2 : 1;
+  constexpr int kBlocks = (KS + 3) / 4;              // scales of a row
+  constexpr int kScales = kRows * kBlocks;
+  static_assert(kRows / 4 * kChunks % 64 == 0 && kRows % (16 * MR * WV) == 0, "");
+  __shared__ __align__(16) char lds[2][kRows * kPitch];
+  __shared__ float scales[FP8 ? 2 : 1][FP8 ? kScales : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wv = wave % WV, wn = wave / WV;
+  const int r16 = lane & 15, g = lane >> 4;
+  int tn, split;
+  if (!place(a, tn, split)) return;
+  int t0, t1;
+  part_of((a.v_end - a.v_begin + kRows - 1) / kRows, split, a.splits, t0, t1);
+  const int64_t n0 = (int64_t)tn * (16 * NS * WN);
+  const int64_t n = n0 + wn * (16 * NS) + r16;
+
+  // Chunk c of LDS row r lies at swizzle(r, c): 8 lanes that read one chunk
+  // of 8 rows touch different banks.
+  auto swizzle = [](int r, int c) {
+    return kChunks % 8 == 0 ? c ^ (r & 7) : c ^ ((r >> 2) & 3);
+  };
+  // the order of k within 64 columns: 8-bit fragments are 16 columns wide
+  u32x4 fb[KS][NS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int m = 16; m < 64; m <<= 1) {
-        const float t = __shfl_xor(top[j], m), s = __shfl_xor(sum[j], m);
-        join(top[j], sum[j], t, s);
+    for (int j = 0; j < NS; ++j)
+      fb[k][j] = load16<2>(a.h, n + j * 16,
+                           FP8 ? (k >> 1) * 128 + g * 32 + (k & 1) * 16 : k * 64 + g * 16);
+  // what lies behind the last column of a table row is cut off here
+  u32x4 keep[2];
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int have = a.w.kb - ((KS - 2 + i) * 64 + g * 16 + q * 4);
+        keep[i][q] = have >= 4 ? 0xffffffffu : have == 2 ? 0xffffu : 0u;
       }
-      if (g == 0) red[wave * 64 + j * 16 + r16] = make_float2(top[j], sum[j]);
-    }
-    __syncthreads();
-    if (threadIdx.x < kTile) {
-      const int half = threadIdx.x >> 6, c = threadIdx.x & 63;
-      float2 p = red[(half * 2) * 64 + c];
-      const float2 q = red[(half * 2 + 1) * 64 + c];
-      join(p.x, p.y, q.x, q.y);
-      a.part[(int64_t)split * a.tiles_n * kTile + n0 + threadIdx.x] = p;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int have = a.w.kb - ((KS - 2) * 32 + g * 16 + q * 4);
+      keep[0][q] = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
     }
   }
+
+  const int last_chunk = (a.w.kb + 15) / 16;
+  float next_scale[(kScales + 255) / 256];
+  auto fetch = [&](int tile, int buf) {
+    const int v0 = a.v_begin + tile * kRows;
+    const char* base = a.w.p + v0 * a.w.ld;
+    const int last = min(kRows - 1, (int)a.w.rows - 1 - v0);
+    const uint32_t to = lds_address(&lds[buf][wave * (kRows / 4) * kPitch]);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int p = lane + 64 * i;
+      const int r = wave * (kRows / 4) + p / kChunks;
+      const int c = swizzle(r, p % kChunks);
+      if (c < last_chunk)
+        load_lds16(base, (uint32_t)(min(r, last) * (int)a.w.ld + c * 16), to + i * 1024);
+    }
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < (kScales + 255) / 256; ++i) {
+        const int p = threadIdx.x + 256 * i;
+        next_scale[i] = 0.f;
+        const int r = p / kBlocks, b = p % kBlocks;
+        if (p < kScales && v0 + r < a.w.rows && b * 128 < a.w.kb)
+          next_scale[i] = scale_of(a.w.scales[(v0 + r) * a.w.lds + b]);
+      }
+    }
+  };
+  auto put_scales = [&](int buf) {
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < (kScales + 255) / 256; ++i)
+        if (threadIdx.x + 256 * i < kScales) scales[buf][threadIdx.x + 256 * i] = next_scale[i];
+    }
+  };
+
+  Sink<USE, kBF16, NS> sink;
+  sink.start(a, n);
+  if (t0 < t1) {
+    fetch(t0, 0);
+    put_scales(0);
+  }
+  for (int tile = t0; tile < t1; ++tile) {
+    const int buf = (tile - t0) & 1;
+    // the tile has arrived for all waves, and all are done with the other one
+    wait_loads();
+    __syncthreads();
+    if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
+    const int v0 = a.v_begin + tile * kRows + 4 * g;
+#pragma unroll 1
+    for (int m = 0; m < kRows / (16 * MR * WV); ++m) {
+      const int row0 = (m * WV + wv) * 16 * MR;
+      f32x4 acc[MR][NS];
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!FP8) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          u32x4 fa[MR];
+#pragma unroll
+          for (int i = 0; i < MR; ++i) {
+            const int r = row0 + i * 16 + r16;
+            fa[i] = *reinterpret_cast<const u32x4*>(&lds[buf][r * kPitch + swizzle(r, k * 4 + g) * 16]);
+            if (k >= KS - 2) fa[i] &= keep[k - (KS - 2)];
+          }
+#pragma unroll
+          for (int i = 0; i < MR; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) acc[i][j] = mma<kBF16>(fa[i], fb[k][j], acc[i][j]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+#pragma unroll
+          for (int i = 0; i < MR; ++i) {
+            const int r = row0 + i * 16 + r16;
+            u32x4 q = *reinterpret_cast<const u32x4*>(
+                &lds[buf][r * kPitch + swizzle(r, k * 2 + g) * 16]);
+            if (k >= KS - 2) q &= keep[0];
+            const float s = scales[buf][r * kBlocks + k / 4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              u32x4 fa;
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                fa[2 * w] = __builtin_bit_cast(uint32_t,
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * half + w], s, false));
+                fa[2 * w + 1] = __builtin_bit_cast(uint32_t,
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * half + w], s, true));
+              }
+#pragma unroll
+              for (int j = 0; j < NS; ++j)
+                acc[i][j] = mma<kBF16>(fa, fb[k + half][j], acc[i][j]);
+            }
+          }
+        }
+      }
+      sink.template take<MR>(a, acc, v0 + row0, n);
+    }
+    put_scales(buf ^ 1);
+  }
+  if constexpr (USE == kLoss) sink.template finish_loss<WV>(a, lds[0], split, n0);
 }
 
 // ---------------------------------------------------------------------------
@@ -829,7 +1082,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char*
 // Host side
 // ---------------------------------------------------------------------------
 static Rows make_rows(uintptr_t p, int64_t ld_elems, int64_t rows, int64_t cols, int es) {
-  if (rows < 0 || cols < 1 || cols > (1 << 24) || ld_elems < 0)
+  if (rows < 0 || rows > 0x7fffffff || cols < 1 || cols > (1 << 24) || ld_elems < 0)
     throw std::runtime_error("bad shape");
   Rows r{};
   r.p = (const char*)p;
@@ -849,10 +1102,57 @@ static int score_grid(const ScoreArgs& a) {
   return grid_of((int64_t)8 * a.tiles_n * ((a.splits + 7) / 8));
 }
 
-// part: [splits][round_up(n, 128)] pairs of float
+// The widest rows that a wave can hold in registers, in steps of 32 columns.
+constexpr int kMostResident = 10;
+
+// Whether the kernel with resident samples takes these rows.  Its offsets
+// within a tile have 32 bits.
+static bool is_resident(const ScoreArgs& a, int64_t cols) {
+  return cols <= 32 * kMostResident && a.w.vec && a.w.ld < (1 << 23);
+}
+
+// Samples of a workgroup of the kernel with resident samples.
+static int resident_samples(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
+
+template <int KS, int USE, bool FP8>
+static void launch_resident_ks(const ScoreArgs& a, int samples, hipStream_t stream) {
+  const int grid = score_grid(a);
+  if (samples == 16) resident_kernel<KS, 1, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
+  else if (samples == 64) resident_kernel<KS, 4, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
+  else resident_kernel<KS, 4, 4, USE, FP8><<<grid, 256, 0, stream>>>(a);
+}
+
+// The parts of the table: about `want` workgroups, at most a.splits parts.
+static int parts_of(const ScoreArgs& a, int64_t rows, int want) {
+  const int64_t tiles = (a.v_end - a.v_begin + rows - 1) / rows;
+  return (int)std::min<int64_t>(std::min<int64_t>(tiles, a.splits),
+                                std::max(1, want / a.tiles_n));
+}
+
+template <int USE, bool FP8>
+static void launch_resident(ScoreArgs& a, int64_t cols, int want, hipStream_t stream) {
+  const int samples = resident_samples(a.h.rows);
+  a.tiles_n = grid_of((a.h.rows + samples - 1) / samples);
+  const int ks = (int)((cols + 63) / 64) * 2;
+  a.splits = parts_of(a, ks <= 4 ? 128 : 64, want);
+  if (ks == 2) launch_resident_ks<2, USE, FP8>(a, samples, stream);
+  else if (ks == 4) launch_resident_ks<4, USE, FP8>(a, samples, stream);
+  else if (ks == 6) launch_resident_ks<6, USE, FP8>(a, samples, stream);
+  else if (ks == 8) launch_resident_ks<8, USE, FP8>(a, samples, stream);
+  else launch_resident_ks<10, USE, FP8>(a, samples, stream);
+}
+
+template <int TW, int TH, int USE>
+static void launch_scores(ScoreArgs& a, int want, hipStream_t stream) {
+  a.tiles_n = grid_of((a.h.rows + kTile - 1) / kTile);
+  a.splits = parts_of(a, kTile, want);
+  scores_kernel<TW, TH, USE><<<score_grid(a), 256, 0, stream>>>(a);
+}
+
+// part: part_size pairs of float, n for each part of the table
 static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
-                         int64_t ignore, int splits, uintptr_t part, uintptr_t loss,
+                         int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t loss,
                          uintptr_t lse, int reduce, uintptr_t reduced, uintptr_t stream_ptr) {
   HIP_CLEAR_ERROR();
   hipStream_t stream = (hipStream_t)stream_ptr;
@@ -861,20 +1161,22 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     ScoreArgs a{};
     a.w = make_rows(w, ldw, v, d, es);
     a.h = make_rows(h, ldh, n, d, es);
-    a.tiles_n = grid_of((n + kTile - 1) / kTile);
-    a.splits = splits;
     a.v_begin = 0;
-    a.v_end = v;
+    a.v_end = (int)v;
     a.part = (float2*)part;
-    const int64_t ldp = (int64_t)a.tiles_n * kTile;
+    a.ldp = n;
+    const int want = 1024;
+    a.splits = (int)std::min<int64_t>(want, part_size / n);
+    if (a.splits < 1) throw std::runtime_error("workspace too small");
     const int joins = grid_of((n + 3) / 4);
     if (is_bf16) {
-      scores_kernel<kBF16, kBF16, kLoss><<<score_grid(a), 256, 0, stream>>>(a);
-      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, splits, ldp,
+      if (is_resident(a, d)) launch_resident<kLoss, false>(a, d, want, stream);
+      else launch_scores<kBF16, kBF16, kLoss>(a, want, stream);
+      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
           (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
     } else {
-      scores_kernel<kF32, kF32, kLoss><<<score_grid(a), 256, 0, stream>>>(a);
-      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, splits, ldp,
+      launch_scores<kF32, kF32, kLoss>(a, want, stream);
+      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
           (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
     }
   }
@@ -888,7 +1190,7 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
-                         uintptr_t weight, int64_t chunk, uintptr_t coef, int coef_parts,
+                         uintptr_t weight, int64_t chunk, uintptr_t coef,
                          int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
                          uintptr_t stream_ptr) {
   HIP_CLEAR_ERROR();
@@ -905,10 +1207,9 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     ScoreArgs a{};
     a.w = rw;
     a.h = rh;
-    a.tiles_n = tiles_n;
-    a.splits = std::min(coef_parts, tiles_v);
-    a.v_begin = v0;
-    a.v_end = v1;
+    a.splits = 1 << 20;
+    a.v_begin = (int)v0;
+    a.v_end = (int)v1;
     a.targets = (const void*)targets;
     a.targets64 = targets64;
     a.ignore = ignore;
@@ -918,8 +1219,9 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.weight = (const float*)weight;
     a.coef = (char*)coef;
     a.ldc = chunk;
-    if (is_bf16) scores_kernel<kBF16, kBF16, kCoef><<<score_grid(a), 256, 0, stream>>>(a);
-    else scores_kernel<kF32, kF32, kCoef><<<score_grid(a), 256, 0, stream>>>(a);
+    if (!is_bf16) launch_scores<kF32, kF32, kCoef>(a, 2048, stream);
+    else if (is_resident(a, d)) launch_resident<kCoef, false>(a, d, 1024, stream);
+    else launch_scores<kBF16, kBF16, kCoef>(a, 2048, stream);
     GradArgs b{};
     b.d = (int)d;
     b.tiles_d = tiles_d;
@@ -1015,16 +1317,15 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
   ScoreArgs a{};
   a.w = make_fp8(values, ldv, scales, lds, n, k);
   a.h = make_rows(a_ptr, lda, m, k, 2);
-  a.tiles_n = grid_of((m + kTile - 1) / kTile);
-  const int64_t tiles_v = (n + kTile - 1) / kTile;
-  a.splits = (int)std::min<int64_t>(tiles_v, std::max<int64_t>(8, 4096 / a.tiles_n));
+  a.splits = 1 << 20;
   a.v_begin = 0;
-  a.v_end = n;
+  a.v_end = (int)n;
   a.col_scale = (const float*)col_scale;
   a.out = (char*)out;
   a.ldo = n;
   a.out_bf16 = out_bf16;
-  scores_kernel<kFP8, kBF16, kStore><<<score_grid(a), 256, 0, stream>>>(a);
+  if (is_resident(a, k)) launch_resident<kStore, true>(a, k, 1024, stream);
+  else launch_scores<kFP8, kBF16, kStore>(a, 2048, stream);
   HIP_CHECK(hipGetLastError());
 }
 

@@ -26,6 +26,7 @@ import torch
 # this, half of the memory-side cache: they are written once and read twice.
 _COEF_BYTES = 128 << 20
 _TILE = 128
+_PARTS = 1024
 
 
 def _native():
@@ -92,17 +93,16 @@ def _forward(h, w, targets, ignore_index, reduce: int):
     lse = torch.empty_like(loss)
     reduced = torch.empty(2, dtype=torch.float32, device=h.device) \
         if reduce else None
-    tiles_n = max(1, _ceil(n, _TILE))
-    # enough workgroups for every CU, each with as many tiles as possible
-    splits = min(_ceil(v, _TILE), max(1, 1024 // tiles_n))
-    part = torch.empty(splits * tiles_n * _TILE * 2, dtype=torch.float32,
-                       device=h.device)
+    # a maximum and a sum of every row for each part of the vocabulary: parts
+    # for enough workgroups, of 128 or more words
+    parts = min(_ceil(v, 64), max(1, _PARTS // max(1, _ceil(n, 256))))
+    part = torch.empty(parts * n * 2, dtype=torch.float32, device=h.device)
     with torch.cuda.device(h.device):
         _native().softmax_loss(
             h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
             int(h.dtype == torch.bfloat16), targets.data_ptr(),
-            int(targets.dtype == torch.int64), int(ignore_index), splits,
-            part.data_ptr(), loss.data_ptr(), lse.data_ptr(), reduce,
+            int(targets.dtype == torch.int64), int(ignore_index),
+            part.data_ptr(), parts * n, loss.data_ptr(), lse.data_ptr(), reduce,
             0 if reduced is None else reduced.data_ptr(),
             torch.cuda.current_stream(h.device).cuda_stream)
     return loss, lse, reduced
@@ -136,7 +136,7 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
             int(targets.dtype == torch.int64), int(ignore_index),
             lse.data_ptr(), grad.data_ptr(), int(grad.dim() > 0),
             0 if weight is None else weight.data_ptr(), width,
-            coef.data_ptr(), max(8, 2048 // tiles_n), splits,
+            coef.data_ptr(), splits,
             part.data_ptr() if need_h else 0, ldp,
             0 if dh is None else dh.data_ptr(),
             0 if dw is None else dw.data_ptr(),
