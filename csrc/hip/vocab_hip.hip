@@ -220,8 +220,8 @@ struct ScoreArgs {
   const float* grad;
   int grad_step;
   const float* weight;      // one factor for all samples, or null
-  char* coef;               // [N][ldc], column 0 = table row v_begin
-  int64_t ldc;
+  char* coef;               // [coef_rows][ldc], column 0 = table row v_begin;
+  int64_t coef_rows, ldc;   // zeros in rows from N on
   // kStore
   const float* col_scale;
   char* out;
@@ -324,7 +324,7 @@ struct Sink {
   __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
                                             int64_t n0) {
     // from the first of the 16 rows, which is the same in all lanes, offsets
-    // have 32 bits: the coefficients of one launch take 128 MB, or 128 columns
+    // have 32 bits: the coefficients of one launch take 512 MB, or 256 columns
     constexpr int es = TC == kF32 ? 4 : 2;
     const int64_t first = n0 - (threadIdx.x & 15);
     const int64_t uniform = (int64_t)__builtin_amdgcn_readfirstlane((int)first);
@@ -334,7 +334,7 @@ struct Sink {
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const int64_t n = n0 + j * 16;
-      if (n >= a.h.rows) continue;
+      if (n >= a.coef_rows) continue;
       const float lse2 = lse[j] * kLog2e;
       const bool far = __any(fabsf(lse[j]) > kFar);
 #pragma unroll
@@ -949,6 +949,186 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
   }
 }
 
+// h for the gradient: rows [rows][ldo] of 16-byte multiples with zeros behind
+// the last column and row, and in rows that have no loss, whatever they hold:
+// a coefficient of 0 would not hide a NaN.
+template <int T>
+__global__ __launch_bounds__(256) void pack_kernel(
+    Rows h, const void* targets, int targets64, int64_t ignore, int64_t vocab, char* out,
+    int64_t rows, int ldo) {
+  constexpr int ES = Elem<T>::size;
+  const int chunks = ldo * ES / 16;
+  const int64_t total = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int c = (int)(i - r * chunks);
+    u32x4 v = {0, 0, 0, 0};
+    if (r < h.rows) {
+      const int64_t y = target_of(targets, targets64, r);
+      if (y != ignore && y >= 0 && y < vocab) v = load16<ES>(h, r, c * 16);
+    }
+    reinterpret_cast<u32x4*>(out)[i] = v;
+  }
+}
+
+template <int N> __device__ __forceinline__ void wait_loads_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+
+// The same product for bf16 rows that start at multiples of 16 bytes: 256 rows
+// r and 32 ND columns d per workgroup of eight waves, 64 x 16 ND per wave, so
+// that narrow tables are read once and the coefficients, the larger part, as
+// often as there are tiles of d.  Steps of 32 k go straight into LDS, three
+// steps ahead of the one at work.
+template <int ND, bool DW>
+__global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
+  constexpr int kRowsR = 256, kStep = 32, kAhead = 3;
+  constexpr int kPitchX = 64 * ND;                   // bytes of a row k
+  constexpr int kChunksX = kPitchX / 16;
+  constexpr int kBytesX = kStep * kPitchX, kBytesB = kStep * kRowsR * 2;
+  constexpr int kInstrX = kBytesX / 1024;            // loads of a whole wave
+  constexpr int kMoreX = kInstrX % 8;                // waves with one more
+  __shared__ __align__(16) char lds[kAhead + 1][kBytesX + kBytesB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wd = wave & 1, wr = wave >> 1;
+  const int r16 = lane & 15, g = lane >> 4;
+  // the parts of k go round the XCDs: the tiles of r that share rows of x are
+  // in one XCD at a time
+  const int tiles = a.tiles_d * a.tiles_r;
+  const int split = a.splits >= 8 ? (int)(blockIdx.x & 7) + 8 * (int)((blockIdx.x >> 3) / tiles)
+                                  : (int)blockIdx.x / tiles;
+  const int at = a.splits >= 8 ? (int)(blockIdx.x >> 3) % tiles : (int)blockIdx.x % tiles;
+  if (split >= a.splits) return;
+  const int td = at % a.tiles_d, tr = at / a.tiles_d;
+  int s0, s1;
+  part_of((int)((a.k + kStep - 1) / kStep), split, a.splits, s0, s1);
+  const int64_t r0 = (int64_t)tr * kRowsR;
+  const int d0 = td * 32 * ND;
+
+  // Blocks of 16 columns of row k lie at block ^ key(k): the rows of one
+  // transposing read spread over the banks.
+  auto key = [](int k, int pitch) {
+    return pitch % 256 == 0 ? (k & 3) | ((k >> 3) & 1) << 2
+                            : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+  };
+  // What lies outside is replaced by what is inside, and no lane sits out: the
+  // waits below count the loads of each wave.  Columns d and rows r past the
+  // end are not stored; past the last k, one side is zeros.
+  const int have_chunks = (a.x.kb - d0 * 2 + 15) / 16;     // columns of x from d0 on
+  const int have_b = DW ? (int)((a.b.kb - r0 * 2 + 15) / 16)     // chunks of a row
+                        : (int)min((int64_t)kRowsR, a.b.rows - r0);
+  auto fetch = [&](int s) {
+    char* buf = lds[(s - s0) & kAhead];
+    const int64_t k0 = (int64_t)s * kStep;
+    const char* xb = a.x.p + k0 * a.x.ld + d0 * 2;
+    const int last = (int)min((int64_t)kStep - 1, a.x.rows - 1 - k0);
+#pragma unroll
+    for (int i = 0; i < (kInstrX + 7) / 8; ++i) {
+      const int q = wave + 8 * i;
+      if (q < kInstrX) {
+        const int p = q * 64 + lane;
+        const int k = p / kChunksX, pos = p % kChunksX;
+        const int c = ((pos >> 1) ^ key(k, kPitchX)) * 2 + (pos & 1);
+        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + min(c, have_chunks - 1) * 16),
+                   lds_address(buf + q * 1024));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int q = wave + 8 * i;
+      const int p = q * 64 + lane;
+      if constexpr (DW) {
+        // rows k of 256 coefficients
+        const int k = p >> 5, pos = p & 31;
+        const int c = ((pos >> 1) ^ key(k, 512)) * 2 + (pos & 1);
+        const char* bb = a.b.p + k0 * a.b.ld + r0 * 2;
+        load_lds16(bb, (uint32_t)k * (uint32_t)a.b.ld + min(c, have_b - 1) * 16,
+                   lds_address(buf + kBytesX + q * 1024));
+      } else {
+        // rows r of 32 coefficients: chunk c at c ^ ((r >> 2) & 3)
+        const int r = p >> 2;
+        const int c = (p & 3) ^ ((r >> 2) & 3);
+        const char* bb = a.b.p + r0 * a.b.ld + k0 * 2;
+        load_lds16(bb, (uint32_t)min(r, have_b - 1) * (uint32_t)a.b.ld + c * 16,
+                   lds_address(buf + kBytesX + q * 1024));
+      }
+    }
+  };
+
+  f32x4 acc[ND][4];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (s0 + i < s1) fetch(s0 + i);
+  // a transposing read: 16 lanes take 4 rows k of one block of 16 columns
+  auto columns = [&](const char* p, int pitch, int block) {
+    const int k = 8 * g + (r16 >> 2);
+    const char* q = p + k * pitch + ((block ^ key(k, pitch)) << 5) + (r16 & 3) * 8;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * pitch));
+    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+    return u32x4{x[0], x[1], y[0], y[1]};
+  };
+  for (int s = s0; s < s1; ++s) {
+    // step s has arrived, two more may be on their way
+    if (s + kAhead - 1 < s1) {
+      if (wave < kMoreX) wait_loads_but<(kAhead - 1) * (kInstrX / 8 + 1 + 2)>();
+      else wait_loads_but<(kAhead - 1) * (kInstrX / 8 + 2)>();
+    } else {
+      wait_loads();
+    }
+    __syncthreads();
+    if (s + kAhead < s1) fetch(s + kAhead);
+    const char* x = lds[(s - s0) & kAhead];
+    const char* b = x + kBytesX;
+    u32x4 fb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DW) {
+        fb[j] = columns(b, 512, wr * 4 + j);
+      } else {
+        const int r = wr * 64 + j * 16 + r16;
+        fb[j] = *reinterpret_cast<const u32x4*>(b + r * 64 + ((g ^ ((r >> 2) & 3)) << 4));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const u32x4 fa = columns(x, kPitchX, wd * ND + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = mma<kBF16>(fa, fb[j], acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t r = r0 + wr * 64 + j * 16 + r16;
+    if (r >= a.r) continue;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int d = d0 + (wd * ND + i) * 16 + 4 * g;
+      if (d >= a.d) continue;
+      if constexpr (!DW) {
+        f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
+        *o = a.add ? *o + acc[i][j] : acc[i][j];
+      } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + r * a.ldo + d;
+        const uint32_t lo = pack_bf16(acc[i][j][0], acc[i][j][1]);
+        const uint32_t hi = pack_bf16(acc[i][j][2], acc[i][j][3]);
+        if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
+          *reinterpret_cast<u32x2*>(o) = u32x2{lo, hi};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.d) o[e] = (uint16_t)((e < 2 ? lo : hi) >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
 // dh from its parts.
 template <int T>
 __global__ __launch_bounds__(256) void sum_parts_kernel(
@@ -1112,13 +1292,17 @@ static bool is_resident(const ScoreArgs& a, int64_t cols) {
 }
 
 // Samples of a workgroup of the kernel with resident samples.
-static int resident_samples(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
+static int resident_samples(int64_t n, int use) {
+  // coefficients are written up to a multiple of 32 samples
+  return n <= 16 && use != kCoef ? 16 : n <= 64 ? 64 : 256;
+}
 
 template <int KS, int USE, bool FP8>
 static void launch_resident_ks(const ScoreArgs& a, int samples, hipStream_t stream) {
   const int grid = score_grid(a);
-  if (samples == 16) resident_kernel<KS, 1, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
-  else if (samples == 64) resident_kernel<KS, 4, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
+  if constexpr (USE != kCoef)
+    if (samples == 16) return resident_kernel<KS, 1, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
+  if (samples == 64) resident_kernel<KS, 4, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
   else resident_kernel<KS, 4, 4, USE, FP8><<<grid, 256, 0, stream>>>(a);
 }
 
@@ -1131,7 +1315,7 @@ static int parts_of(const ScoreArgs& a, int64_t rows, int want) {
 
 template <int USE, bool FP8>
 static void launch_resident(ScoreArgs& a, int64_t cols, int want, hipStream_t stream) {
-  const int samples = resident_samples(a.h.rows);
+  const int samples = resident_samples(a.h.rows, USE);
   a.tiles_n = grid_of((a.h.rows + samples - 1) / samples);
   const int ks = (int)((cols + 63) / 64) * 2;
   a.splits = parts_of(a, ks <= 4 ? 128 : 64, want);
@@ -1186,24 +1370,54 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
   HIP_CHECK(hipGetLastError());
 }
 
-// coef: [n][chunk] elements; part: [splits][n][ldp] floats
+// Tiles of 32 ND columns that cover d with the fewest wasted.
+static void wide_tiles(int d, int& nd, int& tiles) {
+  tiles = (d + 319) / 320;
+  nd = ((d + tiles - 1) / tiles + 63) / 64 * 2;
+}
+
+template <bool DW>
+static void launch_grad_wide(GradArgs b, hipStream_t stream) {
+  int nd;
+  wide_tiles(b.d, nd, b.tiles_d);
+  b.tiles_r = grid_of((b.r + 255) / 256);
+  const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
+  const int blocks = grid_of(b.splits >= 8 ? tiles * ((b.splits + 7) / 8) * 8 : tiles * b.splits);
+  if (nd == 2) grad_wide_kernel<2, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 4) grad_wide_kernel<4, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 6) grad_wide_kernel<6, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 8) grad_wide_kernel<8, DW><<<blocks, 512, 0, stream>>>(b);
+  else grad_wide_kernel<10, DW><<<blocks, 512, 0, stream>>>(b);
+}
+
+// packed: [np][dp] elements with np = n rounded up to 32, dp = d rounded up to
+// 64; coef: [np][chunk] elements; part: [splits][n][ldp] floats
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
-                         uintptr_t weight, int64_t chunk, uintptr_t coef,
+                         uintptr_t weight, uintptr_t packed, int64_t chunk, uintptr_t coef,
                          int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
                          uintptr_t stream_ptr) {
   HIP_CLEAR_ERROR();
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
-  if (chunk % kTile != 0 || ldp % 4 != 0) throw std::runtime_error("bad workspace shape");
+  if (chunk % kTile != 0 || ldp % 4 != 0 || packed % 16 != 0 || coef % 16 != 0)
+    throw std::runtime_error("bad workspace shape");
   if (n == 0) throw std::runtime_error("no rows");
-  const Rows rw = make_rows(w, ldw, v, d, es), rh = make_rows(h, ldh, n, d, es);
+  const int64_t np = (n + 31) / 32 * 32, dp = (d + 63) / 64 * 64;
+  const Rows rw = make_rows(w, ldw, v, d, es);
+  Rows rh = make_rows(h, ldh, n, d, es);
+  const int pack_blocks = (int)std::min<int64_t>((np * dp * es / 16 + 255) / 256, 4096);
+  if (is_bf16) pack_kernel<kBF16><<<pack_blocks, 256, 0, stream>>>(
+      rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
+  else pack_kernel<kF32><<<pack_blocks, 256, 0, stream>>>(
+      rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
+  rh = make_rows(packed, dp, n, d, es);
+  const bool wide = is_bf16 && rw.vec && rw.ld < (1 << 25);
   const int tiles_n = grid_of((n + kTile - 1) / kTile);
   const int tiles_d = (int)((d + kTile - 1) / kTile);
   for (int64_t v0 = 0; v0 < v; v0 += chunk) {
     const int64_t v1 = std::min(v, v0 + chunk);
-    const int tiles_v = grid_of((v1 - v0 + kTile - 1) / kTile);
     ScoreArgs a{};
     a.w = rw;
     a.h = rh;
@@ -1218,6 +1432,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.grad_step = grad_step;
     a.weight = (const float*)weight;
     a.coef = (char*)coef;
+    a.coef_rows = np;
     a.ldc = chunk;
     if (!is_bf16) launch_scores<kF32, kF32, kCoef>(a, 2048, stream);
     else if (is_resident(a, d)) launch_resident<kCoef, false>(a, d, 1024, stream);
@@ -1236,12 +1451,14 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.ldp = ldp;
       b.add = v0 > 0;
       const int blocks = grid_of((int64_t)tiles_d * tiles_n * splits);
-      if (is_bf16) grad_kernel<kBF16, false><<<blocks, 256, 0, stream>>>(b);
+      if (wide) launch_grad_wide<false>(b, stream);
+      else if (is_bf16) grad_kernel<kBF16, false><<<blocks, 256, 0, stream>>>(b);
       else grad_kernel<kF32, false><<<blocks, 256, 0, stream>>>(b);
     }
     if (dw) {
-      b.x = rh;
-      b.b = make_rows(coef, chunk, n, v1 - v0, es);
+      const int tiles_v = grid_of((v1 - v0 + kTile - 1) / kTile);
+      b.x = make_rows(packed, dp, np, dp, es);
+      b.b = make_rows(coef, chunk, np, v1 - v0, es);
       b.r = v1 - v0;
       b.k = n;
       b.tiles_r = tiles_v;
@@ -1249,7 +1466,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.out = (char*)dw + v0 * d * es;
       b.ldo = d;
       const int blocks = grid_of((int64_t)tiles_d * tiles_v);
-      if (is_bf16) grad_kernel<kBF16, true><<<blocks, 256, 0, stream>>>(b);
+      if (is_bf16) launch_grad_wide<true>(b, stream);
       else grad_kernel<kF32, true><<<blocks, 256, 0, stream>>>(b);
     }
   }

@@ -23,8 +23,8 @@ from typing import Optional, Tuple
 import torch
 
 # Pieces of the vocabulary are as wide as keeps their coefficients within
-# this, half of the memory-side cache: they are written once and read twice.
-_COEF_BYTES = 128 << 20
+# this.
+_COEF_BYTES = 512 << 20
 _TILE = 128
 _PARTS = 1024
 
@@ -120,13 +120,17 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     dw = torch.empty((v, d), dtype=w.dtype, device=w.device) \
         if need_w else None
     size = h.element_size()
-    tiles_n = _ceil(n, _TILE)
-    width = max(_TILE, _COEF_BYTES // (n * size) // _TILE * _TILE)
-    width = min(width, _ceil(v, _TILE) * _TILE)
-    coef = torch.empty(n * width * size, dtype=torch.uint8, device=h.device)
+    rows = _ceil(n, 32) * 32
+    packed = torch.empty(rows * _ceil(d, 64) * 64, dtype=h.dtype,
+                         device=h.device)
+    # equal pieces of the vocabulary, in whole tiles
+    pieces = _ceil(v, max(256, _COEF_BYTES // (rows * size)))
+    width = _ceil(_ceil(v, pieces), 256) * 256
+    coef = torch.empty(rows * width, dtype=h.dtype, device=h.device)
     ldp = _ceil(d, 4) * 4
-    splits = min(_ceil(width * size, _TILE),
-                 max(1, 512 // (tiles_n * _ceil(d, _TILE))), 64)
+    tiles = _ceil(n, 256) * _ceil(d, 320) if size == 2 else \
+        _ceil(n, 128) * _ceil(d, 128)
+    splits = min(_ceil(width, 128), max(1, (256 if size == 2 else 512) // tiles))
     part = torch.empty(splits * n * ldp if need_h else 0,
                        dtype=torch.float32, device=h.device)
     with torch.cuda.device(h.device):
@@ -135,7 +139,8 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
             int(h.dtype == torch.bfloat16), targets.data_ptr(),
             int(targets.dtype == torch.int64), int(ignore_index),
             lse.data_ptr(), grad.data_ptr(), int(grad.dim() > 0),
-            0 if weight is None else weight.data_ptr(), width,
+            0 if weight is None else weight.data_ptr(), packed.data_ptr(),
+            width,
             coef.data_ptr(), splits,
             part.data_ptr() if need_h else 0, ldp,
             0 if dh is None else dh.data_ptr(),
