@@ -25,7 +25,6 @@
 
 namespace py = pybind11;
 
-#define HIP_CLEAR_ERROR() (void)hipGetLastError()
 #define HIP_CHECK(expr)                                                     \
   do {                                                                      \
     hipError_t _e = (expr);                                                 \
@@ -1152,25 +1151,40 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
 //   at 240: the next one would stand for 2^128, which float32 does not hold
 // TO_BF16 writes the values that the 8-bit rows stand for instead.
 // ---------------------------------------------------------------------------
+//
+// A workgroup takes 64 blocks of 128 columns that follow each other, four to
+// a group of lanes with all loads first; the position of the first one is the
+// only division by a length of 64 bits.
 template <int T, bool TO_BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(
-    Rows x, int cols, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
-  const int64_t total = x.rows * blocks;
+    Rows x, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
+  constexpr int kEach = 4;
   const int sub = threadIdx.x & 15;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; i < total;
-       i += (int64_t)gridDim.x * 16) {
-    const int64_t row = i / blocks;
-    const int b = (int)(i - row * blocks);
-    const int c0 = b * 128 + sub * 8;
+  const int64_t first = (int64_t)blockIdx.x * (16 * kEach);
+  const int64_t row0 = first / blocks;
+  const int in0 = (int)(first - row0 * blocks);
+  int64_t row[kEach];
+  int b[kEach];
+  u32x4 q[kEach][T == kBF16 ? 1 : 2];
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int t = in0 + (threadIdx.x >> 4) + 16 * u;
+    const int r = t / blocks;
+    row[u] = row0 + r;
+    b[u] = t - r * blocks;
+    const int o = (b[u] * 128 + sub * 8) * Elem<T>::size;
+    q[u][0] = load16<Elem<T>::size>(x, row[u], o);
+    if constexpr (T == kF32) q[u][1] = load16<4>(x, row[u], o + 16);
+  }
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    if (row[u] >= x.rows) return;      // the same for the 16 lanes of a block
+    const int c0 = b[u] * 128 + sub * 8;
     float v[8];
-    if constexpr (T == kBF16) {
-      const u32x4 q = load16<2>(x, row, c0 * 2);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = bf16_to_f32((uint16_t)(q[k >> 1] >> (16 * (k & 1))));
-    } else {
-      const u32x4 q = load16<4>(x, row, c0 * 4), r = load16<4>(x, row, c0 * 4 + 16);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(q[k]), v[4 + k] = __uint_as_float(r[k]);
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (T == kBF16) v[k] = bf16_to_f32((uint16_t)(q[u][0][k >> 1] >> (16 * (k & 1))));
+      else v[k] = __uint_as_float(q[u][k >> 2][k & 3]);
     }
     uint32_t most = 0;
 #pragma unroll
@@ -1203,55 +1217,81 @@ __global__ __launch_bounds__(256) void quantize_kernel(
       const float s = scale_of((uint8_t)(e + 127));
       const u32x2 lo = fp8x4_to_bf16(w[0], s), hi = fp8x4_to_bf16(w[1], s);
       if (c0 < ldv)      // ldv is a multiple of 8; columns past the last are 0
-        *reinterpret_cast<u32x4*>(values + (row * ldv + c0) * 2) =
+        *reinterpret_cast<u32x4*>(values + (row[u] * ldv + c0) * 2) =
             u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
       if (c0 < ldv)      // ldv is a multiple of 16
-        *reinterpret_cast<u32x2*>(values + row * ldv + c0) = u32x2{w[0], w[1]};
-      if (sub == 0) scales[row * lds + b] = (uint8_t)(e + 127);
+        *reinterpret_cast<u32x2*>(values + row[u] * ldv + c0) = u32x2{w[0], w[1]};
+      if (sub == 0) scales[row[u] * lds + b[u]] = (uint8_t)(e + 127);
     }
   }
 }
 
+// 8 columns to a lane, four times: rows of bf16 or f32 that follow each other
+// without a gap are written in one stream.
 template <int TO>
 __global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char* out, int64_t ldo) {
-  const int chunks = (cols + 15) / 16;
-  const int64_t total = x.rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / chunks;
-    const int c = (int)(i - row * chunks) * 16;
-    const u32x4 q = load16<1>(x, row, c);
-    const float s = scale_of(x.scales[row * x.lds + (c >> 7)]);
-    if constexpr (TO == kBF16) {
-      uint32_t w[8];
+  constexpr int kEach = 4;
+  const int chunks = (cols + 7) / 8;
+  const int64_t first = (int64_t)blockIdx.x * (256 * kEach);
+  const int64_t row0 = first / chunks;
+  const int in0 = (int)(first - row0 * chunks);
+  int64_t row[kEach];
+  int c[kEach];
+  u32x2 q[kEach];
+  float s[kEach];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const u32x2 t = fp8x4_to_bf16(q[k], s);
-        w[2 * k] = t[0], w[2 * k + 1] = t[1];
+  for (int u = 0; u < kEach; ++u) {
+    const uint32_t t = in0 + threadIdx.x + 256 * u;
+    const uint32_t r = t / (uint32_t)chunks;
+    row[u] = row0 + r;
+    c[u] = (int)(t - r * chunks) * 8;
+    q[u] = u32x2{0, 0};
+    if (row[u] < x.rows) {
+      const char* p = x.p + row[u] * x.ld + c[u];
+      if (x.vec && c[u] + 8 <= cols) q[u] = *reinterpret_cast<const u32x2*>(p);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c[u] + e < cols) q[u][e >> 2] |= (uint32_t)(uint8_t)p[e] << (8 * (e & 3));
       }
-      uint16_t* o = reinterpret_cast<uint16_t*>(out) + row * ldo + c;
-      if ((ldo & 7) == 0 && c + 16 <= cols) {
-        reinterpret_cast<u32x4*>(o)[0] = u32x4{w[0], w[1], w[2], w[3]};
-        reinterpret_cast<u32x4*>(o)[1] = u32x4{w[4], w[5], w[6], w[7]};
+      s[u] = scale_of(x.scales[row[u] * x.lds + (c[u] >> 7)]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    if (row[u] >= x.rows) return;
+    const int have = cols - c[u];
+    if constexpr (TO == kBF16) {
+      const u32x2 lo = fp8x4_to_bf16(q[u][0], s[u]), hi = fp8x4_to_bf16(q[u][1], s[u]);
+      uint16_t* o = reinterpret_cast<uint16_t*>(out) + row[u] * ldo + c[u];
+      if ((ldo & 7) == 0 && have >= 8) {
+        *reinterpret_cast<u32x4*>(o) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      } else if ((ldo & 3) == 0 && have >= 4) {
+        *reinterpret_cast<u32x2*>(o) = lo;
+        if (have >= 8) *reinterpret_cast<u32x2*>(o + 4) = hi;
+        else
+#pragma unroll
+          for (int e = 4; e < 8; ++e)
+            if (e < have) o[e] = (uint16_t)(hi[(e - 4) >> 1] >> (16 * (e & 1)));
       } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (c + k < cols) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        for (int e = 0; e < 8; ++e)
+          if (e < have) o[e] = (uint16_t)((e < 4 ? lo : hi)[(e & 3) >> 1] >> (16 * (e & 1)));
       }
     } else {
-      float* o = reinterpret_cast<float*>(out) + row * ldo + c;
+      float* o = reinterpret_cast<float*>(out) + row[u] * ldo + c[u];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[k], false);
-        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[k], true);
-        const f32x4 t = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
-        if ((ldo & 3) == 0 && c + 4 * k + 4 <= cols) {
+      for (int k = 0; k < 2; ++k) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[u][k], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[u][k], true);
+        const f32x4 t = {lo[0] * s[u], lo[1] * s[u], hi[0] * s[u], hi[1] * s[u]};
+        if ((ldo & 3) == 0 && have >= 4 * k + 4) {
           reinterpret_cast<f32x4*>(o)[k] = t;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c + 4 * k + e < cols) o[4 * k + e] = t[e];
+            if (4 * k + e < have) o[4 * k + e] = t[e];
         }
       }
     }
@@ -1261,6 +1301,19 @@ __global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char*
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+// The tensors' device for the launches of one call.
+struct OnDevice {
+  int before = -1, device;
+  explicit OnDevice(int d) : device(d) {
+    (void)hipGetLastError();      // sticky: an older error is not ours
+    HIP_CHECK(hipGetDevice(&before));
+    if (before != device) HIP_CHECK(hipSetDevice(device));
+  }
+  ~OnDevice() {
+    if (before != device) (void)hipSetDevice(before);
+  }
+};
+
 static Rows make_rows(uintptr_t p, int64_t ld_elems, int64_t rows, int64_t cols, int es) {
   if (rows < 0 || rows > 0x7fffffff || cols < 1 || cols > (1 << 24) || ld_elems < 0)
     throw std::runtime_error("bad shape");
@@ -1337,8 +1390,8 @@ static void launch_scores(ScoreArgs& a, int want, hipStream_t stream) {
 static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t loss,
-                         uintptr_t lse, int reduce, uintptr_t reduced, uintptr_t stream_ptr) {
-  HIP_CLEAR_ERROR();
+                         uintptr_t lse, int reduce, uintptr_t reduced, int device, uintptr_t stream_ptr) {
+  const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
   if (n > 0) {
@@ -1397,8 +1450,8 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
                          uintptr_t weight, uintptr_t packed, int64_t chunk, uintptr_t coef,
                          int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
-                         uintptr_t stream_ptr) {
-  HIP_CLEAR_ERROR();
+                         int device, uintptr_t stream_ptr) {
+  const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
   if (chunk % kTile != 0 || ldp % 4 != 0 || packed % 16 != 0 || coef % 16 != 0)
@@ -1483,17 +1536,17 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
 // to_bf16: values are bf16 rows, no scales are written
 static void quantize_rows(uintptr_t x, int64_t ldx, int64_t rows, int64_t cols, int is_bf16,
                           uintptr_t values, int64_t ldv, uintptr_t scales, int64_t lds,
-                          int to_bf16, uintptr_t stream_ptr) {
-  HIP_CLEAR_ERROR();
+                          int to_bf16, int device, uintptr_t stream_ptr) {
+  const OnDevice on(device);
   if (rows == 0) return;
   hipStream_t stream = (hipStream_t)stream_ptr;
   if (ldv % (to_bf16 ? 8 : 16) != 0 || ldv < cols || values % 16 != 0)
     throw std::runtime_error("bad layout of the values");
   const Rows r = make_rows(x, ldx, rows, cols, is_bf16 ? 2 : 4);
   const int blocks = (int)((cols + 127) / 128);
-  const int grid = (int)std::min<int64_t>((rows * blocks + 15) / 16, 8192);
+  const int grid = grid_of((rows * blocks + 63) / 64);
   auto go = [&](auto kernel) {
-    kernel<<<grid, 256, 0, stream>>>(r, (int)cols, blocks, (char*)values, ldv,
+    kernel<<<grid, 256, 0, stream>>>(r, blocks, (char*)values, ldv,
                                      (uint8_t*)scales, lds);
   };
   if (is_bf16) to_bf16 ? go(quantize_kernel<kBF16, true>) : go(quantize_kernel<kBF16, false>);
@@ -1511,13 +1564,13 @@ static Rows make_fp8(uintptr_t values, int64_t ldv, uintptr_t scales, int64_t ld
 
 static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int64_t lds,
                             int64_t rows, int64_t cols, int is_bf16, uintptr_t out, int64_t ldo,
-                            uintptr_t stream_ptr) {
-  HIP_CLEAR_ERROR();
+                            int device, uintptr_t stream_ptr) {
+  const OnDevice on(device);
   if (rows == 0) return;
   hipStream_t stream = (hipStream_t)stream_ptr;
   if (out % 16 != 0) throw std::runtime_error("bad layout of the output");
   const Rows r = make_fp8(values, ldv, scales, lds, rows, cols);
-  const int grid = (int)std::min<int64_t>((rows * ((cols + 15) / 16) + 255) / 256, 8192);
+  const int grid = grid_of((rows * ((cols + 7) / 8) + 1023) / 1024);
   if (is_bf16) dequantize_kernel<kBF16><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
   else dequantize_kernel<kF32><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
   HIP_CHECK(hipGetLastError());
@@ -1526,8 +1579,8 @@ static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int
 // a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n]
 static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,
                         uintptr_t scales, int64_t lds, int64_t n, int64_t k, uintptr_t col_scale,
-                        uintptr_t out, int out_bf16, uintptr_t stream_ptr) {
-  HIP_CLEAR_ERROR();
+                        uintptr_t out, int out_bf16, int device, uintptr_t stream_ptr) {
+  const OnDevice on(device);
   if (m == 0 || n == 0) return;
   hipStream_t stream = (hipStream_t)stream_ptr;
   if (out % 16 != 0) throw std::runtime_error("bad layout of the output");

@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 
-from .softmax import _ceil, _native, _rows
+from .softmax import _ceil, _native, _place, _rows
 
 BLOCK = 128
 
@@ -83,10 +83,6 @@ def _check_rows(name: str, q) -> Fp8Rows:
     return Fp8Rows(_rows(values), _rows(scales))
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     """Rows [R, K] of float32 or bfloat16 in 8 bits.  Rows of the result start
     at multiples of 16 bytes.  A block's scale is the smallest power of two in
@@ -100,11 +96,10 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
                        device=x.device)
     scales = torch.empty((r, _ceil(k, BLOCK)), dtype=torch.uint8,
                          device=x.device)
-    with torch.cuda.device(x.device):
-        _native().quantize_rows(
-            x.data_ptr(), x.stride(0), r, k, int(x.dtype == torch.bfloat16),
-            held.data_ptr(), held.shape[1], scales.data_ptr(),
-            scales.shape[1], 0, _stream(x.device))
+    _native().quantize_rows(
+        x.data_ptr(), x.stride(0), r, k, int(x.dtype == torch.bfloat16),
+        held.data_ptr(), held.shape[1], scales.data_ptr(),
+        scales.shape[1], 0, *_place(x.device))
     return Fp8Rows(held.view(torch.float8_e4m3fn)[:, :k],
                    scales.view(torch.float8_e8m0fnu))
 
@@ -117,12 +112,11 @@ def dequantize_rows(q: Fp8Rows, dtype: torch.dtype = torch.float32
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"unsupported dtype {dtype}: float32 or bfloat16")
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        _native().dequantize_rows(
-            q.values.data_ptr(), q.values.stride(0), q.scales.data_ptr(),
-            q.scales.stride(0), q.shape[0], q.shape[1],
-            int(dtype == torch.bfloat16), out.data_ptr(), out.shape[1],
-            _stream(q.device))
+    _native().dequantize_rows(
+        q.values.data_ptr(), q.values.stride(0), q.scales.data_ptr(),
+        q.scales.stride(0), q.shape[0], q.shape[1],
+        int(dtype == torch.bfloat16), out.data_ptr(), out.shape[1],
+        *_place(q.device))
     return out
 
 
@@ -162,21 +156,20 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
     out = torch.empty((m, n), dtype=out_dtype, device=b.device)
     ld = _ceil(k, 8) * 8
     held = torch.empty((m, ld), dtype=torch.bfloat16, device=b.device)
-    native, stream = _native(), _stream(b.device)
-    with torch.cuda.device(b.device):
-        if isinstance(a, Fp8Rows):
-            native.dequantize_rows(
-                a.values.data_ptr(), a.values.stride(0), a.scales.data_ptr(),
-                a.scales.stride(0), m, k, 1, held.data_ptr(), ld, stream)
-        else:
-            a = _rows(a.detach())
-            native.quantize_rows(
-                a.data_ptr(), a.stride(0), m, k,
-                int(a.dtype == torch.bfloat16), held.data_ptr(), ld, 0, 0, 1,
-                stream)
-        native.matmul_rows(
-            held.data_ptr(), ld, m, b.values.data_ptr(), b.values.stride(0),
-            b.scales.data_ptr(), b.scales.stride(0), n, k,
-            0 if col_scale is None else col_scale.data_ptr(), out.data_ptr(),
-            int(out_dtype == torch.bfloat16), stream)
+    native, place = _native(), _place(b.device)
+    if isinstance(a, Fp8Rows):
+        native.dequantize_rows(
+            a.values.data_ptr(), a.values.stride(0), a.scales.data_ptr(),
+            a.scales.stride(0), m, k, 1, held.data_ptr(), ld, *place)
+    else:
+        a = _rows(a.detach())
+        native.quantize_rows(
+            a.data_ptr(), a.stride(0), m, k,
+            int(a.dtype == torch.bfloat16), held.data_ptr(), ld, 0, 0, 1,
+            *place)
+    native.matmul_rows(
+        held.data_ptr(), ld, m, b.values.data_ptr(), b.values.stride(0),
+        b.scales.data_ptr(), b.scales.stride(0), n, k,
+        0 if col_scale is None else col_scale.data_ptr(), out.data_ptr(),
+        int(out_dtype == torch.bfloat16), *place)
     return out

@@ -41,6 +41,11 @@ def _native():
         ) from e
 
 
+def _place(device: torch.device) -> Tuple[int, int]:
+    """Device and stream that a call is launched on."""
+    return device.index, torch.cuda.current_stream(device).cuda_stream
+
+
 def _ceil(a: int, b: int) -> int:
     return -(-a // b)
 
@@ -97,14 +102,13 @@ def _forward(h, w, targets, ignore_index, reduce: int):
     # for enough workgroups, of 128 or more words
     parts = min(_ceil(v, 64), max(1, _PARTS // max(1, _ceil(n, 256))))
     part = torch.empty(parts * n * 2, dtype=torch.float32, device=h.device)
-    with torch.cuda.device(h.device):
-        _native().softmax_loss(
-            h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-            int(h.dtype == torch.bfloat16), targets.data_ptr(),
-            int(targets.dtype == torch.int64), int(ignore_index),
-            part.data_ptr(), parts * n, loss.data_ptr(), lse.data_ptr(), reduce,
-            0 if reduced is None else reduced.data_ptr(),
-            torch.cuda.current_stream(h.device).cuda_stream)
+    _native().softmax_loss(
+        h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
+        int(h.dtype == torch.bfloat16), targets.data_ptr(),
+        int(targets.dtype == torch.int64), int(ignore_index),
+        part.data_ptr(), parts * n, loss.data_ptr(), lse.data_ptr(), reduce,
+        0 if reduced is None else reduced.data_ptr(),
+        *_place(h.device))
     return loss, lse, reduced
 
 
@@ -133,19 +137,18 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     splits = min(_ceil(width, 128), max(1, (256 if size == 2 else 512) // tiles))
     part = torch.empty(splits * n * ldp if need_h else 0,
                        dtype=torch.float32, device=h.device)
-    with torch.cuda.device(h.device):
-        _native().softmax_grad(
-            h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-            int(h.dtype == torch.bfloat16), targets.data_ptr(),
-            int(targets.dtype == torch.int64), int(ignore_index),
-            lse.data_ptr(), grad.data_ptr(), int(grad.dim() > 0),
-            0 if weight is None else weight.data_ptr(), packed.data_ptr(),
-            width,
-            coef.data_ptr(), splits,
-            part.data_ptr() if need_h else 0, ldp,
-            0 if dh is None else dh.data_ptr(),
-            0 if dw is None else dw.data_ptr(),
-            torch.cuda.current_stream(h.device).cuda_stream)
+    _native().softmax_grad(
+        h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
+        int(h.dtype == torch.bfloat16), targets.data_ptr(),
+        int(targets.dtype == torch.int64), int(ignore_index),
+        lse.data_ptr(), grad.data_ptr(), int(grad.dim() > 0),
+        0 if weight is None else weight.data_ptr(), packed.data_ptr(),
+        width,
+        coef.data_ptr(), splits,
+        part.data_ptr() if need_h else 0, ldp,
+        0 if dh is None else dh.data_ptr(),
+        0 if dw is None else dw.data_ptr(),
+        *_place(h.device))
     return dh, dw
 
 
