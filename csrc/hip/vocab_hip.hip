@@ -214,15 +214,17 @@ struct ScoreArgs {
   // kCoef
   const void* targets;
   int targets64;
-  int64_t ignore;
+  int64_t ignore, vocab;
   const float* lse;
   const float* grad;
   int grad_step;
   const float* weight;      // one factor for all samples, or null
-  char* coef;               // [coef_rows][ldc], column 0 = table row v_begin;
-  int64_t coef_rows, ldc;   // zeros in rows from N on
+  // [coef_rows][ldc], column 0 = table row v_begin, zeros in rows from N on;
+  // float32 in rows, bfloat16 in blocks of 16 x 16
+  char* coef;
+  int64_t coef_rows, ldc;
   // kStore
-  const float* col_scale;
+  const float* col_scale;   // or null
   char* out;
   int64_t ldo;
   int out_bf16;
@@ -254,7 +256,7 @@ struct Sink {
         lse[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
         if (m < a.h.rows) {
           const int64_t y = target_of(a.targets, a.targets64, m);
-          if (y != a.ignore && y >= 0 && y < a.w.rows) {
+          if (y != a.ignore && y >= 0 && y < a.vocab) {
             yy[j] = (int)y;
             lse[j] = a.lse[m];
             gg[j] = a.grad[m * a.grad_step] * wt;
@@ -266,10 +268,10 @@ struct Sink {
 
   template <int MR>
   __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                       int64_t n) {
+                                       int64_t n, const float* scale) {
     if constexpr (USE == kLoss) take_loss(a, acc, v);
     if constexpr (USE == kCoef) take_coef(a, acc, v, n);
-    if constexpr (USE == kStore) take_store(a, acc, v, n);
+    if constexpr (USE == kStore) take_store(a, acc, v, n, scale);
   }
 
   template <int MR>
@@ -322,14 +324,10 @@ struct Sink {
   template <int MR>
   __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
                                             int64_t n0) {
-    // from the first of the 16 rows, which is the same in all lanes, offsets
-    // have 32 bits: the coefficients of one launch take 512 MB, or 256 columns
-    constexpr int es = TC == kF32 ? 4 : 2;
-    const int64_t first = n0 - (threadIdx.x & 15);
-    const int64_t uniform = (int64_t)__builtin_amdgcn_readfirstlane((int)first);
-    char* to = a.coef + uniform * a.ldc * es;
-    const uint32_t row_bytes = (uint32_t)(a.ldc * es);
-    const uint32_t at = (threadIdx.x & 15) * row_bytes + (uint32_t)(v - a.v_begin) * es;
+    // the first of the wave's samples and rows, the same in all lanes
+    const int64_t n1 = __builtin_amdgcn_readfirstlane((int)(n0 - (threadIdx.x & 15)));
+    const int v1 = __builtin_amdgcn_readfirstlane(v - a.v_begin);
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const int64_t n = n0 + j * 16;
@@ -359,27 +357,30 @@ struct Sink {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (yy[j] < 0 || vi + e >= a.v_end) c[e] = 0.f;
-        if (vi - a.v_begin >= a.ldc) continue;
-        char* o = to + at + (uint32_t)j * 16 * row_bytes + i * 16 * es;
-        if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(o) = c;
-        else
-          *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+        if constexpr (TC == kF32) {
+          *reinterpret_cast<f32x4*>(a.coef + (n * a.ldc + (vi - a.v_begin)) * 4) = c;
+        } else {
+          // 16 samples x 16 table rows are 512 bytes in one piece, as a wave
+          // writes them and with the 16 bytes of 8 table rows whole, as the
+          // products read them
+          char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * 512;
+          *reinterpret_cast<u32x2*>(to + (lane & 15) * 32 + (lane >> 4) * 8) =
+              u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+        }
       }
     }
   }
 
+  // `scale`: the column scales of rows v .. in LDS
   template <int MR>
   __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                             int64_t n0) {
+                                             int64_t n0, const float* scale) {
     const int es = a.out_bf16 ? 2 : 4;
     const bool vec = (a.ldo & 3) == 0;
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
       const int vi = v + i * 16;
-      float cs[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        cs[e] = a.col_scale && vi + e < a.v_end ? a.col_scale[vi + e] : 1.f;
+      const f32x4 cs = *reinterpret_cast<const f32x4*>(scale + i * 16);
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         const int64_t n = n0 + j * 16;
@@ -457,11 +458,20 @@ __device__ __forceinline__ void part_of(int tiles, int split, int splits, int& t
   t1 = t0 + each + (split < more);
 }
 
+// One column scale for each of the first threads.
+__device__ __forceinline__ float col_scale_of(const ScoreArgs& a, int v) {
+  return a.col_scale && v < a.v_end ? a.col_scale[v] : 1.f;
+}
+__device__ __forceinline__ void put_col(const ScoreArgs& a, float* col, int v0) {
+  col[threadIdx.x] = col_scale_of(a, v0 + (int)threadIdx.x);
+}
+
 // Any type, size and alignment: both sides go through LDS in steps of 128
 // bytes of every row, by way of registers.
 template <int TW, int TH, int USE>
 __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
   __shared__ __align__(16) char lds[2][2][kTileBytes];
+  __shared__ __align__(16) float col[USE == kStore ? kTile : 4];
   constexpr int TC = TH;                       // what the instruction takes
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave & 1, wn = wave >> 1;
@@ -496,6 +506,8 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     __syncthreads();
+    if constexpr (USE == kStore)       // the barriers of one more step before use
+      if (slab == 0 && threadIdx.x < kTile) put_col(a, col, a.v_begin + tile * kTile);
     const bool more = it + 1 < steps;
     const int next_slab = slab + 1 == slabs ? 0 : slab + 1;
     const int next_tile = slab + 1 == slabs ? tile + 1 : tile;
@@ -518,7 +530,12 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = mma<TC>(fa[i], fb[j], acc[i][j]);
     }
-    if (slab + 1 == slabs) sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n);
+    if (slab + 1 == slabs) {
+      if constexpr (USE == kStore)
+        if (slabs == 1) __syncthreads();
+      sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n,
+                            USE == kStore ? col + wm * 64 + 4 * g : nullptr);
+    }
     if (more) {
       sw.store(lds[(it + 1) & 1][0]);
       sh.store(lds[(it + 1) & 1][1]);
@@ -540,6 +557,11 @@ __device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint3
 }
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+// Waits until only the last N loads and stores are outstanding: they end in
+// the order in which they were issued.
+template <int N> __device__ __forceinline__ void wait_loads_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return __builtin_amdgcn_readfirstlane(
@@ -567,6 +589,9 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   static_assert(kRows / 4 * kChunks % 64 == 0 && kRows % (16 * MR * WV) == 0, "");
   __shared__ __align__(16) char lds[2][kRows * kPitch];
   __shared__ float scales[FP8 ? 2 : 1][FP8 ? kScales : 1];
+  __shared__ __align__(16) float col[2][USE == kStore ? kRows : 4];
+  // stores of a wave for one whole tile
+  constexpr int kStores = USE == kLoss ? 0 : kRows / (16 * WV) * NS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wv = wave % WV, wn = wave / WV;
   const int r16 = lane & 15, g = lane >> 4;
@@ -609,7 +634,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   }
 
   const int last_chunk = (a.w.kb + 15) / 16;
-  float next_scale[(kScales + 255) / 256];
+  float next_scale[(kScales + 255) / 256], next_col = 1.f;
   auto fetch = [&](int tile, int buf) {
     const int v0 = a.v_begin + tile * kRows;
     const char* base = a.w.p + v0 * a.w.ld;
@@ -623,6 +648,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
       if (c < last_chunk)
         load_lds16(base, (uint32_t)(min(r, last) * (int)a.w.ld + c * 16), to + i * 1024);
     }
+    if constexpr (USE == kStore)
+      if (threadIdx.x < kRows) next_col = col_scale_of(a, v0 + (int)threadIdx.x);
     if constexpr (FP8) {
 #pragma unroll
       for (int i = 0; i < (kScales + 255) / 256; ++i) {
@@ -635,6 +662,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     }
   };
   auto put_scales = [&](int buf) {
+    if constexpr (USE == kStore)
+      if (threadIdx.x < kRows) col[buf][threadIdx.x] = next_col;
     if constexpr (FP8) {
 #pragma unroll
       for (int i = 0; i < (kScales + 255) / 256; ++i)
@@ -648,10 +677,15 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     fetch(t0, 0);
     put_scales(0);
   }
+  // Whether the wave makes all of kStores: then the last tile's stores, which
+  // come after this tile's loads, need not be waited for.
+  const bool whole = n0 + (wn + 1) * (16 * NS) <= a.h.rows && (USE != kStore || (a.ldo & 3) == 0);
   for (int tile = t0; tile < t1; ++tile) {
     const int buf = (tile - t0) & 1;
     // the tile has arrived for all waves, and all are done with the other one
-    wait_loads();
+    // (only the last tile of all may be cut short)
+    if (kStores > 0 && kStores < 64 && whole && tile > t0) wait_loads_but<kStores & 63>();
+    else wait_loads();
     __syncthreads();
     if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
     const int v0 = a.v_begin + tile * kRows + 4 * g;
@@ -705,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
           }
         }
       }
-      sink.template take<MR>(a, acc, v0 + row0, n);
+      sink.template take<MR>(a, acc, v0 + row0, n, &col[buf][USE == kStore ? row0 + 4 * g : 0]);
     }
     put_scales(buf ^ 1);
   }
@@ -948,9 +982,9 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
   }
 }
 
-// h for the gradient: rows [rows][ldo] of 16-byte multiples with zeros behind
-// the last column and row, and in rows that have no loss, whatever they hold:
-// a coefficient of 0 would not hide a NaN.
+// Rows for the gradient: [rows][ldo] of 16-byte multiples with zeros behind
+// the last column and row, and (with targets) in rows that have no loss,
+// whatever they hold: a coefficient of 0 would not hide a NaN.
 template <int T>
 __global__ __launch_bounds__(256) void pack_kernel(
     Rows h, const void* targets, int targets64, int64_t ignore, int64_t vocab, char* out,
@@ -964,15 +998,11 @@ __global__ __launch_bounds__(256) void pack_kernel(
     const int c = (int)(i - r * chunks);
     u32x4 v = {0, 0, 0, 0};
     if (r < h.rows) {
-      const int64_t y = target_of(targets, targets64, r);
-      if (y != ignore && y >= 0 && y < vocab) v = load16<ES>(h, r, c * 16);
+      const int64_t y = targets ? target_of(targets, targets64, r) : 0;
+      if (!targets || (y != ignore && y >= 0 && y < vocab)) v = load16<ES>(h, r, c * 16);
     }
     reinterpret_cast<u32x4*>(out)[i] = v;
   }
-}
-
-template <int N> __device__ __forceinline__ void wait_loads_but() {
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 
 // The same product for bf16 rows that start at multiples of 16 bytes: 256 rows
@@ -1015,6 +1045,7 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
   // waits below count the loads of each wave.  Columns d and rows r past the
   // end are not stored; past the last k, one side is zeros.
   const int have_chunks = (a.x.kb - d0 * 2 + 15) / 16;     // columns of x from d0 on
+  const int64_t block_row = a.b.ld * 16;                   // 16 rows of coefficients
   const int have_b = DW ? (int)((a.b.kb - r0 * 2 + 15) / 16)     // chunks of a row
                         : (int)min((int64_t)kRowsR, a.b.rows - r0);
   auto fetch = [&](int s) {
@@ -1038,18 +1069,22 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
       const int q = wave + 8 * i;
       const int p = q * 64 + lane;
       if constexpr (DW) {
-        // rows k of 256 coefficients
         const int k = p >> 5, pos = p & 31;
         const int c = ((pos >> 1) ^ key(k, 512)) * 2 + (pos & 1);
-        const char* bb = a.b.p + k0 * a.b.ld + r0 * 2;
-        load_lds16(bb, (uint32_t)k * (uint32_t)a.b.ld + min(c, have_b - 1) * 16,
+        // two rows of blocks, chunk c is half of block c / 2
+        const int in = min(c, have_b - 1);
+        load_lds16(a.b.p + (k0 >> 4) * block_row + r0 * 32,
+                   (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * 32 + (in >> 1) * 512 +
+                       (in & 1) * 16,
                    lds_address(buf + kBytesX + q * 1024));
       } else {
         // rows r of 32 coefficients: chunk c at c ^ ((r >> 2) & 3)
         const int r = p >> 2;
         const int c = (p & 3) ^ ((r >> 2) & 3);
-        const char* bb = a.b.p + r0 * a.b.ld + k0 * 2;
-        load_lds16(bb, (uint32_t)min(r, have_b - 1) * (uint32_t)a.b.ld + c * 16,
+        const int in = min(r, have_b - 1);
+        load_lds16(a.b.p + (r0 >> 4) * block_row + k0 * 32,
+                   (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * 32 + (c >> 1) * 512 +
+                       (c & 1) * 16,
                    lds_address(buf + kBytesX + q * 1024));
       }
     }
@@ -1444,11 +1479,12 @@ static void launch_grad_wide(GradArgs b, hipStream_t stream) {
 }
 
 // packed: [np][dp] elements with np = n rounded up to 32, dp = d rounded up to
-// 64; coef: [np][chunk] elements; part: [splits][n][ldp] floats
+// 64; packed_w: [chunk][dp] where bf16 rows of w do not start at multiples of
+// 16 bytes or lie 2^25 bytes apart, else null; coef: [np][chunk] elements; part: [splits][n][ldp] floats
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
-                         uintptr_t weight, uintptr_t packed, int64_t chunk, uintptr_t coef,
+                         uintptr_t weight, uintptr_t packed, uintptr_t packed_w, int64_t chunk, uintptr_t coef,
                          int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
                          int device, uintptr_t stream_ptr) {
   const OnDevice on(device);
@@ -1466,17 +1502,30 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
   else pack_kernel<kF32><<<pack_blocks, 256, 0, stream>>>(
       rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
   rh = make_rows(packed, dp, n, d, es);
-  const bool wide = is_bf16 && rw.vec && rw.ld < (1 << 25);
+  // the wide kernel's offsets within a step have 32 bits
+  const bool pack_w = is_bf16 && !(rw.vec && rw.ld < (1 << 25));
+  if (pack_w && !packed_w) throw std::runtime_error("no workspace for the table's rows");
   const int tiles_n = grid_of((n + kTile - 1) / kTile);
   const int tiles_d = (int)((d + kTile - 1) / kTile);
   for (int64_t v0 = 0; v0 < v; v0 += chunk) {
     const int64_t v1 = std::min(v, v0 + chunk);
+    // the table's rows from v0 on; v_begin and the targets count from row 0
+    Rows piece = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
+    if (pack_w) {
+      const int blocks = (int)std::min<int64_t>(((v1 - v0) * dp * es / 16 + 255) / 256, 8192);
+      pack_kernel<kBF16><<<blocks, 256, 0, stream>>>(piece, nullptr, 0, 0, 0, (char*)packed_w,
+                                                     v1 - v0, (int)dp);
+      piece = make_rows(packed_w, dp, v1 - v0, d, es);
+    }
     ScoreArgs a{};
-    a.w = rw;
+    a.w = piece;
+    a.w.p -= v0 * a.w.ld;
+    a.w.rows = v1;
     a.h = rh;
     a.splits = 1 << 20;
     a.v_begin = (int)v0;
     a.v_end = (int)v1;
+    a.vocab = v;
     a.targets = (const void*)targets;
     a.targets64 = targets64;
     a.ignore = ignore;
@@ -1494,7 +1543,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     b.d = (int)d;
     b.tiles_d = tiles_d;
     if (dh) {
-      b.x = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
+      b.x = piece;
       b.b = make_rows(coef, chunk, n, v1 - v0, es);
       b.r = n;
       b.k = v1 - v0;
@@ -1504,8 +1553,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.ldp = ldp;
       b.add = v0 > 0;
       const int blocks = grid_of((int64_t)tiles_d * tiles_n * splits);
-      if (wide) launch_grad_wide<false>(b, stream);
-      else if (is_bf16) grad_kernel<kBF16, false><<<blocks, 256, 0, stream>>>(b);
+      if (is_bf16) launch_grad_wide<false>(b, stream);
       else grad_kernel<kF32, false><<<blocks, 256, 0, stream>>>(b);
     }
     if (dw) {

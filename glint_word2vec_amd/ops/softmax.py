@@ -131,6 +131,10 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     pieces = _ceil(v, max(256, _COEF_BYTES // (rows * size)))
     width = _ceil(_ceil(v, pieces), 256) * 256
     coef = torch.empty(rows * width, dtype=h.dtype, device=h.device)
+    aligned = w.data_ptr() % 16 == 0 and w.stride(0) * size % 16 == 0 \
+        and w.stride(0) * size < 1 << 25
+    packed_w = None if size == 4 or aligned else \
+        torch.empty(width * _ceil(d, 64) * 64, dtype=w.dtype, device=w.device)
     ldp = _ceil(d, 4) * 4
     tiles = _ceil(n, 256) * _ceil(d, 320) if size == 2 else \
         _ceil(n, 128) * _ceil(d, 128)
@@ -140,15 +144,13 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     _native().softmax_grad(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
         int(h.dtype == torch.bfloat16), targets.data_ptr(),
-        int(targets.dtype == torch.int64), int(ignore_index),
-        lse.data_ptr(), grad.data_ptr(), int(grad.dim() > 0),
+        int(targets.dtype == torch.int64), int(ignore_index), lse.data_ptr(),
+        grad.data_ptr(), int(grad.dim() > 0),
         0 if weight is None else weight.data_ptr(), packed.data_ptr(),
-        width,
-        coef.data_ptr(), splits,
-        part.data_ptr() if need_h else 0, ldp,
+        0 if packed_w is None else packed_w.data_ptr(), width,
+        coef.data_ptr(), splits, part.data_ptr() if need_h else 0, ldp,
         0 if dh is None else dh.data_ptr(),
-        0 if dw is None else dw.data_ptr(),
-        *_place(h.device))
+        0 if dw is None else dw.data_ptr(), *_place(h.device))
     return dh, dw
 
 

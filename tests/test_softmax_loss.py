@@ -190,9 +190,8 @@ def test_rows_that_are_not_finite_stay_alone():
                                                               device="cuda"))
     r = _reference(h[good], w, y[good], grad=torch.ones(()))
     _near(dh[good], r[4], r[6], "dh")
-    # h = NaN times a coefficient of 0 is what the formula says for row 5:
-    # such rows have to be cut out of h, the targets alone do not do it
-    assert dw[:, 4:].isfinite().all()
+    _near(dw, r[5], r[7], "dw")
+    assert (dh[~good] == 0).all()
 
 
 @gpu
