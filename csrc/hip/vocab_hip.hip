@@ -240,7 +240,7 @@ __device__ __forceinline__ int64_t target_of(const void* t, int is64, int64_t n)
 template <int USE, int TC, int NS>
 struct Sink {
   float top[NS], sum[NS];                      // kLoss
-  float lse[NS], gg[NS];                       // kCoef
+  float lse2[NS], gg[NS];                      // kCoef; lse in powers of two
   int yy[NS];                                  // -1: no loss
 
   __device__ __forceinline__ void start(const ScoreArgs& a, int64_t n) {
@@ -253,12 +253,12 @@ struct Sink {
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         const int64_t m = n + j * 16;
-        lse[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
+        lse2[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
         if (m < a.h.rows) {
           const int64_t y = target_of(a.targets, a.targets64, m);
           if (y != a.ignore && y >= 0 && y < a.vocab) {
             yy[j] = (int)y;
-            lse[j] = a.lse[m];
+            lse2[j] = a.lse[m] * kLog2e;
             gg[j] = a.grad[m * a.grad_step] * wt;
           }
         }
@@ -332,8 +332,7 @@ struct Sink {
     for (int j = 0; j < NS; ++j) {
       const int64_t n = n0 + j * 16;
       if (n >= a.coef_rows) continue;
-      const float lse2 = lse[j] * kLog2e;
-      const bool far = __any(fabsf(lse[j]) > kFar);
+      const bool far = __any(fabsf(lse2[j]) > kFar);
 #pragma unroll
       for (int i = 0; i < MR; ++i) {
         const int vi = v + i * 16;
@@ -341,22 +340,24 @@ struct Sink {
         if (far) {
           // the logarithm's own rounding may pass 0 here
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = exp_of(fminf(c[e] - lse[j], 0.f));
+          for (int e = 0; e < 4; ++e)
+            c[e] = __builtin_amdgcn_exp2f(fminf(c[e] * kLog2e - lse2[j], 0.f));
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], kLog2e, -lse2));
+            c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], kLog2e, -lse2[j]));
         }
         const int right = yy[j] - vi;
         if (__any((unsigned)right < 4u)) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[e] -= right == e ? 1.f : 0.f;
         }
-        c *= gg[j];
-        // cut off, whatever its scores are; and behind the last word
+        c *= gg[j];      // 0 without a loss: the row of h is zeros then
+        if (__any(vi + 4 > a.v_end)) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (yy[j] < 0 || vi + e >= a.v_end) c[e] = 0.f;
+          for (int e = 0; e < 4; ++e)
+            if (vi + e >= a.v_end) c[e] = 0.f;
+        }
         if constexpr (TC == kF32) {
           *reinterpret_cast<f32x4*>(a.coef + (n * a.ldc + (vi - a.v_begin)) * 4) = c;
         } else {
@@ -607,6 +608,13 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   auto swizzle = [](int r, int c) {
     return kChunks % 8 == 0 ? c ^ (r & 7) : c ^ ((r >> 2) & 3);
   };
+  // of which a lane reads chunks g + 4 k of row r16 and of rows 16, 32, .. on:
+  // with groups of 8 chunks, at two places that alternate with k
+  const uint32_t at0 = r16 * kPitch + swizzle(r16, g) * 16;
+  const uint32_t at1 = kChunks % 8 == 0 ? at0 ^ 64 : at0 + 64;
+  auto chunk = [&](const char* rows, int k) {
+    return *reinterpret_cast<const u32x4*>(rows + (k & 1 ? at1 : at0) + (k >> 1) * 128);
+  };
   // the order of k within 64 columns: 8-bit fragments are 16 columns wide
   u32x4 fb[KS][NS];
 #pragma unroll
@@ -703,8 +711,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
           u32x4 fa[MR];
 #pragma unroll
           for (int i = 0; i < MR; ++i) {
-            const int r = row0 + i * 16 + r16;
-            fa[i] = *reinterpret_cast<const u32x4*>(&lds[buf][r * kPitch + swizzle(r, k * 4 + g) * 16]);
+            fa[i] = chunk(&lds[buf][(row0 + i * 16) * kPitch], k);
             if (k >= KS - 2) fa[i] &= keep[k - (KS - 2)];
           }
 #pragma unroll
@@ -718,8 +725,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 #pragma unroll
           for (int i = 0; i < MR; ++i) {
             const int r = row0 + i * 16 + r16;
-            u32x4 q = *reinterpret_cast<const u32x4*>(
-                &lds[buf][r * kPitch + swizzle(r, k * 2 + g) * 16]);
+            u32x4 q = chunk(&lds[buf][(row0 + i * 16) * kPitch], k / 2);
             if (k >= KS - 2) q &= keep[0];
             const float s = scales[buf][r * kBlocks + k / 4];
 #pragma unroll
@@ -1537,7 +1543,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.coef_rows = np;
     a.ldc = chunk;
     if (!is_bf16) launch_scores<kF32, kF32, kCoef>(a, 2048, stream);
-    else if (is_resident(a, d)) launch_resident<kCoef, false>(a, d, 1024, stream);
+    else if (is_resident(a, d)) launch_resident<kCoef, false>(a, d, 512, stream);
     else launch_scores<kBF16, kBF16, kCoef>(a, 2048, stream);
     GradArgs b{};
     b.d = (int)d;
