@@ -40,6 +40,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -63,14 +64,14 @@ template <> struct Elem<kF32> { using S = float; static constexpr int size = 4; 
 template <> struct Elem<kBF16> { using S = uint16_t; static constexpr int size = 2; };
 template <> struct Elem<kFP8> { using S = uint8_t; static constexpr int size = 1; };
 
-// Rows of a matrix in global memory.  `vec`: every row starts at a multiple
-// of 16 bytes.
+// Rows of a matrix in global memory, all of which start at multiples of
+// `align` bytes: 16, 4 or less.
 struct Rows {
   const char* p;
   int64_t ld;      // bytes from row to row
   int64_t rows;
   int kb;          // bytes of a row
-  int vec;
+  int align;
   const uint8_t* scales;   // 8-bit rows: exponents + 127, one per 128 columns
   int64_t lds;             // scales from row to row
 };
@@ -101,7 +102,19 @@ __device__ __forceinline__ u32x4 load16(const Rows& m, int64_t row, int o) {
   u32x4 r = {0, 0, 0, 0};
   if (row >= m.rows || o >= m.kb) return r;
   const char* q = m.p + row * m.ld + o;
-  if (m.vec && o + 16 <= m.kb) return *reinterpret_cast<const u32x4*>(q);
+  if (m.align == 16) {
+    // whole, as 16 bytes at a multiple of 16 are of one page; then cut
+    r = *reinterpret_cast<const u32x4*>(q);
+    if (o + 16 > m.kb) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int have = m.kb - o - 4 * i;
+        r[i] = have >= 4 ? r[i] : have <= 0 ? 0u : r[i] & ((1u << (8 * have)) - 1);
+      }
+    }
+    return r;
+  }
+  if (m.align == 4 && o + 16 <= m.kb) return *reinterpret_cast<const u32x4a4*>(q);
   const int have = (m.kb - o) / ES;
   if (ES == 4) {
 #pragma unroll
@@ -139,19 +152,34 @@ __device__ __forceinline__ u32x2 fp8x4_to_bf16(uint32_t v, float scale) {
 
 // One step of the product: 16 bytes of k of each side per lane.  A lane's
 // bytes are k = 16 * (lane >> 4) bytes of 64; as both sides take the same
-// order of k, any order is right.
-template <int T>
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+// order of k, any order is right.  float32 takes four instructions for it;
+// those for one result are kept apart.
+template <int T, int M, int N>
+__device__ __forceinline__ void mma_all(const u32x4 (&a)[M], const u32x4 (&b)[N],
+                                        f32x4 (&c)[M][N]) {
   if constexpr (T == kF32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]),
-                                               __uint_as_float(b[i]), c, 0, 0, 0);
-    return c;
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          c[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              __uint_as_float(a[i][e]), __uint_as_float(b[j][e]), c[i][j], 0, 0, 0);
   } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        c[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[j]), c[i][j], 0, 0, 0);
   }
+}
+
+template <int T, int N>
+__device__ __forceinline__ void mma_row(u32x4 a, const u32x4 (&b)[N], f32x4 (&c)[N]) {
+  const u32x4 a1[1] = {a};
+  mma_all<T>(a1, b, reinterpret_cast<f32x4(&)[1][N]>(c));
 }
 
 // LDS tile with k along its rows: 128 rows of 8 chunks of 16 bytes.  Chunk c
@@ -268,7 +296,7 @@ struct Sink {
 
   template <int MR>
   __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                       int64_t n, const float* scale) {
+                                       int64_t n, const f32x4 (&scale)[MR]) {
     if constexpr (USE == kLoss) take_loss(a, acc, v);
     if constexpr (USE == kCoef) take_coef(a, acc, v, n);
     if constexpr (USE == kStore) take_store(a, acc, v, n, scale);
@@ -372,24 +400,21 @@ struct Sink {
     }
   }
 
-  // `scale`: the column scales of rows v .. in LDS
+  // `scale`: the column scales of the lane's rows
   template <int MR>
   __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                             int64_t n0, const float* scale) {
+                                             int64_t n0, const f32x4 (&scale)[MR]) {
     const int es = a.out_bf16 ? 2 : 4;
     const bool vec = (a.ldo & 3) == 0;
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
       const int vi = v + i * 16;
-      const f32x4 cs = *reinterpret_cast<const f32x4*>(scale + i * 16);
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         const int64_t n = n0 + j * 16;
         if (n >= a.h.rows) continue;
         char* o = a.out + (n * a.ldo + vi) * es;
-        f32x4 s = acc[i][j];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] *= cs[e];
+        const f32x4 s = acc[i][j] * scale[i];
         if (vec && vi + 3 < a.v_end) {
           if (a.out_bf16)
             *reinterpret_cast<u32x2*>(o) =
@@ -526,16 +551,17 @@ __global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
         fa[i] = *reinterpret_cast<const u32x4*>(lw + row_slot(i * 16 + r16, k * 4 + g));
         fb[i] = *reinterpret_cast<const u32x4*>(lh + row_slot(i * 16 + r16, k * 4 + g));
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma<TC>(fa[i], fb[j], acc[i][j]);
+      mma_all<TC>(fa, fb, acc);
     }
     if (slab + 1 == slabs) {
       if constexpr (USE == kStore)
         if (slabs == 1) __syncthreads();
-      sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n,
-                            USE == kStore ? col + wm * 64 + 4 * g : nullptr);
+      f32x4 cs[4] = {};
+      if constexpr (USE == kStore)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          cs[i] = *reinterpret_cast<const f32x4*>(col + wm * 64 + i * 16 + 4 * g);
+      sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n, cs);
     }
     if (more) {
       sw.store(lds[(it + 1) & 1][0]);
@@ -714,10 +740,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
             fa[i] = chunk(&lds[buf][(row0 + i * 16) * kPitch], k);
             if (k >= KS - 2) fa[i] &= keep[k - (KS - 2)];
           }
-#pragma unroll
-          for (int i = 0; i < MR; ++i)
-#pragma unroll
-            for (int j = 0; j < NS; ++j) acc[i][j] = mma<kBF16>(fa[i], fb[k][j], acc[i][j]);
+          mma_all<kBF16>(fa, fb[k], acc);
         }
       } else {
 #pragma unroll
@@ -738,18 +761,135 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
                 fa[2 * w + 1] = __builtin_bit_cast(uint32_t,
                     __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * half + w], s, true));
               }
-#pragma unroll
-              for (int j = 0; j < NS; ++j)
-                acc[i][j] = mma<kBF16>(fa, fb[k + half][j], acc[i][j]);
+              mma_row<kBF16>(fa, fb[k + half], acc[i]);
             }
           }
         }
       }
-      sink.template take<MR>(a, acc, v0 + row0, n, &col[buf][USE == kStore ? row0 + 4 * g : 0]);
+      f32x4 cs[MR] = {};
+      if constexpr (USE == kStore)
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+          cs[i] = *reinterpret_cast<const f32x4*>(&col[buf][row0 + i * 16 + 4 * g]);
+      sink.template take<MR>(a, acc, v0 + row0, n, cs);
     }
     put_scales(buf ^ 1);
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV>(a, lds[0], split, n0);
+}
+
+// Few samples: bound by the bytes of the table, which go from memory to the
+// registers of the one wave that needs them.  A wave takes 16 rows at a time,
+// eight loads of 16 bytes a lane ahead of the eight at work; the samples lie
+// in LDS as the instruction takes them.  Any type, size and alignment; VEC:
+// table rows start at multiples of 16 bytes.
+template <int TW, int TC, int NS, int USE, bool VEC>
+__global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
+  constexpr int kAhead = 8;
+  constexpr int kSteps = TW == kFP8 ? 2 : 1;         // instructions for 16 bytes of a row
+  extern __shared__ __align__(16) char samples[];    // [step][NS][64 lanes][16 bytes]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r16 = lane & 15, g = lane >> 4;
+  int tn, split;
+  if (!place(a, tn, split)) return;
+  const int64_t n0 = (int64_t)tn * (16 * NS);
+  const int64_t n = n0 + r16;
+  const int chunks = (a.w.kb + 63) / 64;             // per lane and row
+  for (int i = threadIdx.x; i < chunks * kSteps * NS * 64; i += 256) {
+    const int f = i >> 6, l = i & 63, j = f % NS, k = f / NS;
+    const int o = TW == kFP8 ? (k >> 1) * 128 + (l >> 4) * 32 + (k & 1) * 16
+                             : k * 64 + (l >> 4) * 16;
+    reinterpret_cast<u32x4*>(samples)[i] =
+        load16<Elem<TC>::size>(a.h, n0 + j * 16 + (l & 15), o);
+  }
+  Sink<USE, TC, NS> sink;
+  sink.start(a, n);
+  __syncthreads();
+
+  int t0, t1;
+  part_of((a.v_end - a.v_begin + 63) / 64, split, a.splits, t0, t1);
+  // this wave's rows are 16 of every 64
+  const int groups = t1 - t0;
+  const int v_first = a.v_begin + t0 * 64 + wave * 16;
+  u32x4 next[kAhead];
+  uint8_t next_scale[TW == kFP8 ? kAhead : 1];
+  // rows and columns past the end are replaced by the last ones: such rows
+  // are not used, such columns are cut off below
+  u32x4 keep;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int have = a.w.kb - ((chunks - 1) * 64 + g * 16 + q * 4);
+    keep[q] = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+  }
+  const int last_byte = (a.w.kb - 1) & ~15;
+  auto fetch = [&](int group, int k0) {
+    const int64_t row = v_first + group * 64 + r16;
+    const int64_t at = min(row, a.w.rows - 1);
+    const char* p = a.w.p + at * a.w.ld;
+    const uint8_t* ps = a.w.scales + at * a.w.lds;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int o = (k0 + i) * 64 + g * 16;
+      if constexpr (VEC) next[i] = *reinterpret_cast<const u32x4*>(p + min(o, last_byte));
+      else next[i] = load16<Elem<TW>::size>(a.w, row, o);
+      if constexpr (TW == kFP8)
+        next_scale[i] = ps[min((k0 + i) * 64, a.w.kb - 1) >> 7];
+    }
+  };
+  if (groups > 0) fetch(0, 0);
+  for (int group = 0; group < groups; ++group) {
+    f32x4 acc[1][NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int v = v_first + group * 64 + 4 * g;
+    f32x4 cs[1] = {};
+    for (int k0 = 0; k0 < chunks; k0 += kAhead) {
+      u32x4 now[kAhead];
+      float scale[TW == kFP8 ? kAhead : 1];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) now[i] = next[i];
+      if constexpr (TW == kFP8)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) scale[i] = scale_of(next_scale[i]);
+      if (k0 + kAhead < chunks) fetch(group, k0 + kAhead);
+      else if (group + 1 < groups) fetch(group + 1, 0);
+      if constexpr (USE == kStore)
+        if (k0 + kAhead >= chunks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cs[0][e] = col_scale_of(a, v + e);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (k0 + i >= chunks) break;
+        if (VEC && k0 + i == chunks - 1) now[i] &= keep;
+        const char* fb = samples + (size_t)(k0 + i) * (kSteps * NS * 1024) + lane * 16;
+        if constexpr (TW == kFP8) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            u32x4 fa;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              fa[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                  now[i][2 * half + w], scale[i], false));
+              fa[2 * w + 1] = __builtin_bit_cast(uint32_t,
+                  __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(now[i][2 * half + w], scale[i], true));
+            }
+            u32x4 f[NS];
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+              f[j] = *reinterpret_cast<const u32x4*>(fb + (half * NS + j) * 1024);
+            mma_row<TC>(fa, f, acc[0]);
+          }
+        } else {
+          u32x4 f[NS];
+#pragma unroll
+          for (int j = 0; j < NS; ++j) f[j] = *reinterpret_cast<const u32x4*>(fb + j * 1024);
+          mma_row<TC>(now[i], f, acc[0]);
+        }
+      }
+    }
+    sink.template take<1>(a, acc, v, n, cs);
+  }
+  if constexpr (USE == kLoss) sink.template finish_loss<4>(a, samples, split, n0);
 }
 
 // ---------------------------------------------------------------------------
@@ -888,10 +1028,10 @@ struct GradArgs {
   int64_t r, k;
   int d;
   int tiles_d, tiles_r, splits;
-  float* part;   // dh: [splits][R][ldp], added to where `add`
+  float* part;   // [splits][R][ldp], added to where `add`; or null, and
   int64_t ldp;
   int add;
-  char* out;     // dw: [R][D]
+  char* out;     // [R][D], of the rows' type
   int64_t ldo;
 };
 
@@ -949,10 +1089,7 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
           fb[i] = *reinterpret_cast<const u32x4*>(
               lds[buf][1] + row_slot(wn * 64 + i * 16 + r16, k * 4 + g));
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma<T>(fa[i], fb[j], acc[i][j]);
+      mma_all<T>(fa, fb, acc);
     }
     if (s + 1 < s1) store(buf ^ 1);
   }
@@ -964,7 +1101,7 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
     for (int i = 0; i < 4; ++i) {
       const int d = d0 + wm * 64 + i * 16 + 4 * g;
       if (d >= a.d) continue;
-      if constexpr (!DW) {
+      if (a.part) {
         f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
         *o = a.add ? *o + acc[i][j] : acc[i][j];
       } else {
@@ -1138,8 +1275,7 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const u32x4 fa = columns(x, kPitchX, wd * ND + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mma<kBF16>(fa, fb[j], acc[i][j]);
+      mma_row<kBF16>(fa, fb, acc[i]);
     }
   }
 #pragma unroll
@@ -1150,7 +1286,7 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
     for (int i = 0; i < ND; ++i) {
       const int d = d0 + (wd * ND + i) * 16 + 4 * g;
       if (d >= a.d) continue;
-      if constexpr (!DW) {
+      if (a.part) {
         f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
         *o = a.add ? *o + acc[i][j] : acc[i][j];
       } else {
@@ -1290,7 +1426,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char*
     q[u] = u32x2{0, 0};
     if (row[u] < x.rows) {
       const char* p = x.p + row[u] * x.ld + c[u];
-      if (x.vec && c[u] + 8 <= cols) q[u] = *reinterpret_cast<const u32x2*>(p);
+      if (x.align == 16 && c[u] + 8 <= cols) q[u] = *reinterpret_cast<const u32x2*>(p);
       else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -1363,7 +1499,7 @@ static Rows make_rows(uintptr_t p, int64_t ld_elems, int64_t rows, int64_t cols,
   r.ld = ld_elems * es;
   r.rows = rows;
   r.kb = (int)cols * es;
-  r.vec = (p % 16 == 0) && (r.ld % 16 == 0);
+  r.align = p % 16 == 0 && r.ld % 16 == 0 ? 16 : p % 4 == 0 && r.ld % 4 == 0 ? 4 : 1;
   return r;
 }
 
@@ -1376,55 +1512,103 @@ static int score_grid(const ScoreArgs& a) {
   return grid_of((int64_t)8 * a.tiles_n * ((a.splits + 7) / 8));
 }
 
+// How many workgroups of a kernel the card holds at a time.
+template <typename K>
+static int slots_of(K kernel, int threads, int lds) {
+  int per_cu = 0, cus = 0, device = 0;
+  HIP_CHECK(hipGetDevice(&device));
+  HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
+  HIP_CHECK(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, lds));
+  return std::max(1, per_cu * cus);
+}
+
+// Cuts the table into at most a.splits parts of whole tiles of `rows` rows.
+// With `slots` workgroups at a time, R rounds of them leave room for
+// R slots / tiles_n parts; of one to four rounds the one is taken in which the
+// longest workgroups end first.  A workgroup's start counts as one tile.
+static void cut(ScoreArgs& a, int64_t rows, int slots) {
+  const int64_t tiles = (a.v_end - a.v_begin + rows - 1) / rows;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    int64_t parts = std::max<int64_t>(1, rounds * slots / a.tiles_n);
+    parts = std::min(std::min<int64_t>(parts, a.splits), tiles);
+    const int64_t each = (tiles + parts - 1) / parts;
+    const int64_t time = (parts * a.tiles_n + slots - 1) / slots * (each + 1);
+    if (time < least) least = time, best = parts;
+  }
+  a.splits = (int)best;
+}
+
 // The widest rows that a wave can hold in registers, in steps of 32 columns.
 constexpr int kMostResident = 10;
 
 // Whether the kernel with resident samples takes these rows.  Its offsets
 // within a tile have 32 bits.
 static bool is_resident(const ScoreArgs& a, int64_t cols) {
-  return cols <= 32 * kMostResident && a.w.vec && a.w.ld < (1 << 23);
+  return cols <= 32 * kMostResident && a.w.align == 16 && a.w.ld < (1 << 23);
 }
 
-// Samples of a workgroup of the kernel with resident samples.
-static int resident_samples(int64_t n, int use) {
-  // coefficients are written up to a multiple of 32 samples
-  return n <= 16 && use != kCoef ? 16 : n <= 64 ? 64 : 256;
-}
-
-template <int KS, int USE, bool FP8>
-static void launch_resident_ks(const ScoreArgs& a, int samples, hipStream_t stream) {
-  const int grid = score_grid(a);
-  if constexpr (USE != kCoef)
-    if (samples == 16) return resident_kernel<KS, 1, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
-  if (samples == 64) resident_kernel<KS, 4, 1, USE, FP8><<<grid, 256, 0, stream>>>(a);
-  else resident_kernel<KS, 4, 4, USE, FP8><<<grid, 256, 0, stream>>>(a);
-}
-
-// The parts of the table: about `want` workgroups, at most a.splits parts.
-static int parts_of(const ScoreArgs& a, int64_t rows, int want) {
-  const int64_t tiles = (a.v_end - a.v_begin + rows - 1) / rows;
-  return (int)std::min<int64_t>(std::min<int64_t>(tiles, a.splits),
-                                std::max(1, want / a.tiles_n));
+template <int KS, int NS, int WN, int USE, bool FP8>
+static void launch_resident_k(ScoreArgs& a, hipStream_t stream) {
+  constexpr auto kernel = resident_kernel<KS, NS, WN, USE, FP8>;
+  static const int slots = slots_of(kernel, 256, 0);
+  a.tiles_n = grid_of((a.h.rows + 16 * NS * WN - 1) / (16 * NS * WN));
+  cut(a, KS <= 4 ? 128 : 64, slots);
+  kernel<<<score_grid(a), 256, 0, stream>>>(a);
 }
 
 template <int USE, bool FP8>
-static void launch_resident(ScoreArgs& a, int64_t cols, int want, hipStream_t stream) {
-  const int samples = resident_samples(a.h.rows, USE);
-  a.tiles_n = grid_of((a.h.rows + samples - 1) / samples);
+static void launch_resident(ScoreArgs& a, int64_t cols, hipStream_t stream) {
   const int ks = (int)((cols + 63) / 64) * 2;
-  a.splits = parts_of(a, ks <= 4 ? 128 : 64, want);
-  if (ks == 2) launch_resident_ks<2, USE, FP8>(a, samples, stream);
-  else if (ks == 4) launch_resident_ks<4, USE, FP8>(a, samples, stream);
-  else if (ks == 6) launch_resident_ks<6, USE, FP8>(a, samples, stream);
-  else if (ks == 8) launch_resident_ks<8, USE, FP8>(a, samples, stream);
-  else launch_resident_ks<10, USE, FP8>(a, samples, stream);
+  const bool few = a.h.rows <= 64, least = a.h.rows <= 16;
+#define CASE_KS(K)                                                              \
+  if (ks == K) {                                                                \
+    if constexpr (USE != kCoef)                                                 \
+      if (least) return launch_resident_k<K, 1, 1, USE, FP8>(a, stream);        \
+    if (few) return launch_resident_k<K, 4, 1, USE, FP8>(a, stream);            \
+    return launch_resident_k<K, 4, 4, USE, FP8>(a, stream);                     \
+  }
+  CASE_KS(2) CASE_KS(4) CASE_KS(6) CASE_KS(8) CASE_KS(10)
+#undef CASE_KS
+  throw std::runtime_error("rows too wide");
 }
 
 template <int TW, int TH, int USE>
-static void launch_scores(ScoreArgs& a, int want, hipStream_t stream) {
+static void launch_scores(ScoreArgs& a, hipStream_t stream) {
+  constexpr auto kernel = scores_kernel<TW, TH, USE>;
+  static const int slots = slots_of(kernel, 256, 0);
   a.tiles_n = grid_of((a.h.rows + kTile - 1) / kTile);
-  a.splits = parts_of(a, kTile, want);
-  scores_kernel<TW, TH, USE><<<score_grid(a), 256, 0, stream>>>(a);
+  cut(a, kTile, slots);
+  kernel<<<score_grid(a), 256, 0, stream>>>(a);
+}
+
+// LDS that the samples of the streaming kernel take; 4 KB at least, for the
+// joining of the softmax.
+static int64_t stream_bytes(const ScoreArgs& a, int ns, bool fp8) {
+  return std::max<int64_t>(4096, (int64_t)(a.w.kb + 63) / 64 * (fp8 ? 2 : 1) * ns * 1024);
+}
+constexpr int64_t kMostStream = 64 << 10;
+
+template <int TW, int TC, int NS, int USE, bool VEC>
+static void launch_stream(ScoreArgs& a, hipStream_t stream) {
+  constexpr auto kernel = stream_kernel<TW, TC, NS, USE, VEC>;
+  const int lds = (int)stream_bytes(a, NS, TW == kFP8);
+  a.tiles_n = grid_of((a.h.rows + 16 * NS - 1) / (16 * NS));
+  cut(a, 64, slots_of(kernel, 256, lds));
+  kernel<<<score_grid(a), 256, lds, stream>>>(a);
+}
+
+// The kernel for scores of these samples and table rows.
+template <int TW, int TC, int USE>
+static void launch_any(ScoreArgs& a, int64_t cols, hipStream_t stream) {
+  constexpr bool fp8 = TW == kFP8;
+  if constexpr (TC == kBF16)
+    if (is_resident(a, cols)) return launch_resident<USE, fp8>(a, cols, stream);
+  if constexpr (USE != kCoef)
+    if (a.h.rows <= 16 && stream_bytes(a, 1, fp8) <= kMostStream)
+      return a.w.align == 16 ? launch_stream<TW, TC, 1, USE, true>(a, stream)
+                             : launch_stream<TW, TC, 1, USE, false>(a, stream);
+  launch_scores<TW, TC, USE>(a, stream);
 }
 
 // part: part_size pairs of float, n for each part of the table
@@ -1443,17 +1627,15 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.v_end = (int)v;
     a.part = (float2*)part;
     a.ldp = n;
-    const int want = 1024;
-    a.splits = (int)std::min<int64_t>(want, part_size / n);
+    a.splits = (int)std::min<int64_t>(1 << 20, part_size / n);
     if (a.splits < 1) throw std::runtime_error("workspace too small");
     const int joins = grid_of((n + 3) / 4);
     if (is_bf16) {
-      if (is_resident(a, d)) launch_resident<kLoss, false>(a, d, want, stream);
-      else launch_scores<kBF16, kBF16, kLoss>(a, want, stream);
+      launch_any<kBF16, kBF16, kLoss>(a, d, stream);
       loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
           (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
     } else {
-      launch_scores<kF32, kF32, kLoss>(a, want, stream);
+      launch_any<kF32, kF32, kLoss>(a, d, stream);
       loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
           (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
     }
@@ -1462,6 +1644,13 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     loss_reduce_kernel<<<1, 1024, 0, stream>>>((const float*)loss, (const void*)targets,
                                                targets64, ignore, n, reduce == 2, (float*)reduced);
   HIP_CHECK(hipGetLastError());
+}
+
+static void launch_sum_parts(const float* part, int splits, int64_t rows, int64_t ldp, int64_t d,
+                             int is_bf16, char* out, hipStream_t stream) {
+  const int blocks = (int)std::min<int64_t>((rows * d + 255) / 256, 4096);
+  if (is_bf16) sum_parts_kernel<kBF16><<<blocks, 256, 0, stream>>>(part, splits, rows, ldp, (int)d, out);
+  else sum_parts_kernel<kF32><<<blocks, 256, 0, stream>>>(part, splits, rows, ldp, (int)d, out);
 }
 
 // Tiles of 32 ND columns that cover d with the fewest wasted.
@@ -1486,12 +1675,14 @@ static void launch_grad_wide(GradArgs b, hipStream_t stream) {
 
 // packed: [np][dp] elements with np = n rounded up to 32, dp = d rounded up to
 // 64; packed_w: [chunk][dp] where bf16 rows of w do not start at multiples of
-// 16 bytes or lie 2^25 bytes apart, else null; coef: [np][chunk] elements; part: [splits][n][ldp] floats
+// 16 bytes or lie 2^25 bytes apart, else null; coef: [np][chunk] elements; part: [splits][n][ldp]
+// floats; part_w: [splits_w][chunk][ldp] where splits_w > 1
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
                          uintptr_t weight, uintptr_t packed, uintptr_t packed_w, int64_t chunk, uintptr_t coef,
-                         int splits, uintptr_t part, int64_t ldp, uintptr_t dh, uintptr_t dw,
+                         int splits, uintptr_t part, int splits_w, uintptr_t part_w, int64_t ldp,
+                         uintptr_t dh, uintptr_t dw,
                          int device, uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
@@ -1509,7 +1700,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
   rh = make_rows(packed, dp, n, d, es);
   // the wide kernel's offsets within a step have 32 bits
-  const bool pack_w = is_bf16 && !(rw.vec && rw.ld < (1 << 25));
+  const bool pack_w = is_bf16 && !(rw.align == 16 && rw.ld < (1 << 25));
   if (pack_w && !packed_w) throw std::runtime_error("no workspace for the table's rows");
   const int tiles_n = grid_of((n + kTile - 1) / kTile);
   const int tiles_d = (int)((d + kTile - 1) / kTile);
@@ -1542,9 +1733,8 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.coef = (char*)coef;
     a.coef_rows = np;
     a.ldc = chunk;
-    if (!is_bf16) launch_scores<kF32, kF32, kCoef>(a, 2048, stream);
-    else if (is_resident(a, d)) launch_resident<kCoef, false>(a, d, 512, stream);
-    else launch_scores<kBF16, kBF16, kCoef>(a, 2048, stream);
+    if (is_bf16) launch_any<kBF16, kBF16, kCoef>(a, d, stream);
+    else launch_any<kF32, kF32, kCoef>(a, d, stream);
     GradArgs b{};
     b.d = (int)d;
     b.tiles_d = tiles_d;
@@ -1569,21 +1759,21 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.r = v1 - v0;
       b.k = n;
       b.tiles_r = tiles_v;
-      b.splits = 1;
+      b.splits = splits_w;
+      b.add = 0;
+      b.part = splits_w > 1 ? (float*)part_w : nullptr;
+      b.ldp = ldp;
       b.out = (char*)dw + v0 * d * es;
       b.ldo = d;
-      const int blocks = grid_of((int64_t)tiles_d * tiles_v);
+      const int blocks = grid_of((int64_t)tiles_d * tiles_v * splits_w);
       if (is_bf16) launch_grad_wide<true>(b, stream);
       else grad_kernel<kF32, true><<<blocks, 256, 0, stream>>>(b);
+      if (splits_w > 1)
+        launch_sum_parts(b.part, splits_w, v1 - v0, ldp, d, is_bf16, b.out, stream);
     }
   }
-  if (dh) {
-    const int blocks = (int)std::min<int64_t>((n * d + 255) / 256, 4096);
-    if (is_bf16) sum_parts_kernel<kBF16><<<blocks, 256, 0, stream>>>(
-        (const float*)part, splits, n, ldp, (int)d, (char*)dh);
-    else sum_parts_kernel<kF32><<<blocks, 256, 0, stream>>>(
-        (const float*)part, splits, n, ldp, (int)d, (char*)dh);
-  }
+  if (dh)
+    launch_sum_parts((const float*)part, splits, n, ldp, d, is_bf16, (char*)dh, stream);
   HIP_CHECK(hipGetLastError());
 }
 
@@ -1648,8 +1838,7 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
   a.out = (char*)out;
   a.ldo = n;
   a.out_bf16 = out_bf16;
-  if (is_resident(a, k)) launch_resident<kStore, true>(a, k, 1024, stream);
-  else launch_scores<kFP8, kBF16, kStore>(a, 2048, stream);
+  launch_any<kFP8, kBF16, kStore>(a, k, stream);
   HIP_CHECK(hipGetLastError());
 }
 

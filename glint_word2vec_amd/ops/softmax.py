@@ -26,7 +26,7 @@ import torch
 # this.
 _COEF_BYTES = 512 << 20
 _TILE = 128
-_PARTS = 1024
+_PARTS = 4096
 
 
 def _native():
@@ -88,6 +88,17 @@ def _check(h, w, targets) -> None:
                            f"{h.device}, {w.device}, {targets.device}")
 
 
+def _parts(tiles: int, slots: int, most: int) -> int:
+    """Parts of a product's long axis for `tiles` results on `slots` places:
+    the fewest that fill nine tenths of what any number up to `most` fills."""
+    if tiles >= 2 * slots:
+        return 1
+    most = max(1, min(most, _ceil(2 * slots, tiles), 64))
+    full = [tiles * s / (_ceil(tiles * s, slots) * slots)
+            for s in range(1, most + 1)]
+    return next(i for i, f in enumerate(full, 1) if f >= 0.9 * max(full))
+
+
 def _forward(h, w, targets, ignore_index, reduce: int):
     """(loss [N], lse [N], [reduced loss, factor] or None)."""
     _check(h, w, targets)
@@ -100,7 +111,7 @@ def _forward(h, w, targets, ignore_index, reduce: int):
         if reduce else None
     # a maximum and a sum of every row for each part of the vocabulary: parts
     # for enough workgroups, of 128 or more words
-    parts = min(_ceil(v, 64), max(1, _PARTS // max(1, _ceil(n, 256))))
+    parts = min(_ceil(v, 64), max(1, _PARTS // max(1, _ceil(n, 128))))
     part = torch.empty(parts * n * 2, dtype=torch.float32, device=h.device)
     _native().softmax_loss(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
@@ -136,11 +147,16 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     packed_w = None if size == 4 or aligned else \
         torch.empty(width * _ceil(d, 64) * 64, dtype=w.dtype, device=w.device)
     ldp = _ceil(d, 4) * 4
-    tiles = _ceil(n, 256) * _ceil(d, 320) if size == 2 else \
-        _ceil(n, 128) * _ceil(d, 128)
-    splits = min(_ceil(width, 128), max(1, (256 if size == 2 else 512) // tiles))
+    # tiles of the products' results, and workgroups that the card holds
+    edge, cols, slots = (256, 320, 256) if size == 2 else (128, 128, 512)
+    splits = _parts(_ceil(n, edge) * _ceil(d, cols), slots,
+                    _ceil(width, 256)) if need_h else 1
+    splits_w = _parts(_ceil(min(v, width), edge) * _ceil(d, cols), slots,
+                      _ceil(n, 256)) if need_w else 1
     part = torch.empty(splits * n * ldp if need_h else 0,
                        dtype=torch.float32, device=h.device)
+    part_w = torch.empty(splits_w * width * ldp if splits_w > 1 else 0,
+                         dtype=torch.float32, device=h.device)
     _native().softmax_grad(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
         int(h.dtype == torch.bfloat16), targets.data_ptr(),
@@ -148,7 +164,8 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
         grad.data_ptr(), int(grad.dim() > 0),
         0 if weight is None else weight.data_ptr(), packed.data_ptr(),
         0 if packed_w is None else packed_w.data_ptr(), width,
-        coef.data_ptr(), splits, part.data_ptr() if need_h else 0, ldp,
+        coef.data_ptr(), splits, part.data_ptr() if need_h else 0, splits_w,
+        part_w.data_ptr() if splits_w > 1 else 0, ldp,
         0 if dh is None else dh.data_ptr(),
         0 if dw is None else dw.data_ptr(), *_place(h.device))
     return dh, dw
