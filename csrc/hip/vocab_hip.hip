@@ -50,9 +50,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 // which costs at most |m| 2^-25 in the exponent.  Past this |m| the exponent
 // is (s - m) log2e instead: one instruction more, but it cannot overflow.
 constexpr float kFar = 1e6f;
-constexpr int kTile = 128;       // rows of either side per workgroup
-constexpr int kSlab = 128;       // bytes of every row per step of the k loop
-constexpr int kTileBytes = kTile * kSlab;
 
 enum Type { kF32 = 0, kBF16 = 1, kFP8 = 2 };
 
@@ -142,12 +139,15 @@ __device__ __forceinline__ float scale_of(uint8_t e) {
 
 // 4 e4m3 values to bf16, times a power of two: exact.
 __device__ __forceinline__ u32x2 fp8x4_to_bf16(uint32_t v, float scale) {
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
-  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
   u32x2 r;
-  r[0] = pack_bf16(lo[0] * scale, lo[1] * scale);
-  r[1] = pack_bf16(hi[0] * scale, hi[1] * scale);
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, scale, false));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, scale, true));
   return r;
+}
+// 8 of them as the instruction takes them.
+__device__ __forceinline__ u32x4 fp8x8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
+  const u32x2 a = fp8x4_to_bf16(lo, scale), b = fp8x4_to_bf16(hi, scale);
+  return u32x4{a[0], a[1], b[0], b[1]};
 }
 
 // One step of the product: 16 bytes of k of each side per lane.  A lane's
@@ -182,51 +182,6 @@ __device__ __forceinline__ void mma_row(u32x4 a, const u32x4 (&b)[N], f32x4 (&c)
   mma_all<T>(a1, b, reinterpret_cast<f32x4(&)[1][N]>(c));
 }
 
-// LDS tile with k along its rows: 128 rows of 8 chunks of 16 bytes.  Chunk c
-// of row r lies at c ^ (r & 7), so that 8 lanes reading one chunk of 8 rows
-// touch different banks.
-__device__ __forceinline__ int row_slot(int r, int c) {
-  return r * kSlab + ((c ^ (r & 7)) << 4);
-}
-
-// A [128 rows x slab] tile on its way to LDS, held in registers meanwhile.
-template <int T>
-struct RowTile {
-  static constexpr int kLoads = T == kFP8 ? 2 : 4;
-  u32x4 v[kLoads];
-  float scale[T == kFP8 ? 2 : 1];
-
-  __device__ __forceinline__ void load(const Rows& m, int64_t row0, int slab) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int q = threadIdx.x + 256 * i;
-      if constexpr (T == kFP8) {
-        // 64 columns to a slab once they are bf16: 4 chunks of 16
-        const int64_t row = row0 + (q >> 2);
-        v[i] = load16<1>(m, row, slab * 64 + (q & 3) * 16);
-        scale[i] = row < m.rows ? scale_of(m.scales[row * m.lds + (slab >> 1)]) : 0.f;
-      } else {
-        v[i] = load16<Elem<T>::size>(m, row0 + (q >> 3), slab * kSlab + (q & 7) * 16);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int q = threadIdx.x + 256 * i;
-      if constexpr (T == kFP8) {
-        const int r = q >> 2, c = (q & 3) * 2;
-        const u32x2 a = fp8x4_to_bf16(v[i][0], scale[i]), b = fp8x4_to_bf16(v[i][1], scale[i]);
-        const u32x2 d = fp8x4_to_bf16(v[i][2], scale[i]), e = fp8x4_to_bf16(v[i][3], scale[i]);
-        *reinterpret_cast<u32x4*>(lds + row_slot(r, c)) = u32x4{a[0], a[1], b[0], b[1]};
-        *reinterpret_cast<u32x4*>(lds + row_slot(r, c + 1)) = u32x4{d[0], d[1], e[0], e[1]};
-      } else {
-        *reinterpret_cast<u32x4*>(lds + row_slot(q >> 3, q & 7)) = v[i];
-      }
-    }
-  }
-};
-
 // ---------------------------------------------------------------------------
 // Scores: tiles of <table row, sample row>, and what is done with them.
 // ---------------------------------------------------------------------------
@@ -234,6 +189,7 @@ enum Use { kLoss = 0, kCoef = 1, kStore = 2 };
 
 struct ScoreArgs {
   Rows w, h;
+  int64_t n;                // samples; h may have rows of zeros behind them
   int tiles_n, splits;      // tiles of samples; parts of the table's range
   int v_begin, v_end;       // the table rows of this launch
   // kLoss: (max, sum of exp(s - max)) per part and sample
@@ -247,8 +203,8 @@ struct ScoreArgs {
   const float* grad;
   int grad_step;
   const float* weight;      // one factor for all samples, or null
-  // [coef_rows][ldc], column 0 = table row v_begin, zeros in rows from N on;
-  // float32 in rows, bfloat16 in blocks of 16 x 16
+  // [coef_rows][ldc] in blocks of 16 x 16, column 0 = table row v_begin,
+  // zeros in rows from N on
   char* coef;
   int64_t coef_rows, ldc;
   // kStore
@@ -282,7 +238,7 @@ struct Sink {
       for (int j = 0; j < NS; ++j) {
         const int64_t m = n + j * 16;
         lse2[j] = 0.f, gg[j] = 0.f, yy[j] = -1;
-        if (m < a.h.rows) {
+        if (m < a.n) {
           const int64_t y = target_of(a.targets, a.targets64, m);
           if (y != a.ignore && y >= 0 && y < a.vocab) {
             yy[j] = (int)y;
@@ -386,16 +342,15 @@ struct Sink {
           for (int e = 0; e < 4; ++e)
             if (vi + e >= a.v_end) c[e] = 0.f;
         }
-        if constexpr (TC == kF32) {
-          *reinterpret_cast<f32x4*>(a.coef + (n * a.ldc + (vi - a.v_begin)) * 4) = c;
-        } else {
-          // 16 samples x 16 table rows are 512 bytes in one piece, as a wave
-          // writes them and with the 16 bytes of 8 table rows whole, as the
-          // products read them
-          char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * 512;
-          *reinterpret_cast<u32x2*>(to + (lane & 15) * 32 + (lane >> 4) * 8) =
-              u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
-        }
+        // 16 samples x 16 table rows are 512 bytes (1 KB) in one piece, as a
+        // wave writes them and with every 16 bytes of one sample, as the
+        // products read them
+        constexpr int es = TC == kF32 ? 4 : 2;
+        char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es) +
+                   (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
+        if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
+        else
+          *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
       }
     }
   }
@@ -412,7 +367,7 @@ struct Sink {
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         const int64_t n = n0 + j * 16;
-        if (n >= a.h.rows) continue;
+        if (n >= a.n) continue;
         char* o = a.out + (n * a.ldo + vi) * es;
         const f32x4 s = acc[i][j] * scale[i];
         if (vec && vi + 3 < a.v_end) {
@@ -437,7 +392,7 @@ struct Sink {
 
   // kLoss, after the last tile: joins the four lanes, then the waves, that
   // hold one sample.  Wave `wave` has samples from 16 NS (wave / WV) on.
-  template <int WV>
+  template <int WV, int kWaves = 4>
   __device__ __forceinline__ void finish_loss(const ScoreArgs& a, char* lds, int split,
                                               int64_t n0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -454,7 +409,7 @@ struct Sink {
       if (lane < 16) red[wave * kCols + j * 16 + lane] = make_float2(top[j], sum[j]);
     }
     __syncthreads();
-    if (threadIdx.x < 4 / WV * kCols) {
+    if (threadIdx.x < kWaves / WV * kCols) {
       const int group = threadIdx.x / kCols, c = threadIdx.x % kCols;
       float2 p = red[group * WV * kCols + c];
 #pragma unroll
@@ -462,7 +417,7 @@ struct Sink {
         const float2 q = red[(group * WV + i) * kCols + c];
         join(p.x, p.y, q.x, q.y);
       }
-      if (n0 + threadIdx.x < a.h.rows) a.part[split * a.ldp + n0 + threadIdx.x] = p;
+      if (n0 + threadIdx.x < a.n) a.part[split * a.ldp + n0 + threadIdx.x] = p;
     }
   }
 };
@@ -484,93 +439,9 @@ __device__ __forceinline__ void part_of(int tiles, int split, int splits, int& t
   t1 = t0 + each + (split < more);
 }
 
-// One column scale for each of the first threads.
+// The factor of table row v in stored scores.
 __device__ __forceinline__ float col_scale_of(const ScoreArgs& a, int v) {
   return a.col_scale && v < a.v_end ? a.col_scale[v] : 1.f;
-}
-__device__ __forceinline__ void put_col(const ScoreArgs& a, float* col, int v0) {
-  col[threadIdx.x] = col_scale_of(a, v0 + (int)threadIdx.x);
-}
-
-// Any type, size and alignment: both sides go through LDS in steps of 128
-// bytes of every row, by way of registers.
-template <int TW, int TH, int USE>
-__global__ __launch_bounds__(256, 2) void scores_kernel(ScoreArgs a) {
-  __shared__ __align__(16) char lds[2][2][kTileBytes];
-  __shared__ __align__(16) float col[USE == kStore ? kTile : 4];
-  constexpr int TC = TH;                       // what the instruction takes
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave & 1, wn = wave >> 1;
-  const int r16 = lane & 15, g = lane >> 4;
-  int tn, split;
-  if (!place(a, tn, split)) return;
-  int t0, t1;
-  part_of((a.v_end - a.v_begin + kTile - 1) / kTile, split, a.splits, t0, t1);
-  const int64_t n0 = (int64_t)tn * kTile;
-  const int64_t n = n0 + wn * 64 + r16;
-  const int slabs = (a.h.kb + kSlab - 1) / kSlab;
-
-  Sink<USE, TC, 4> sink;
-  sink.start(a, n);
-  RowTile<TW> sw;
-  RowTile<TH> sh;
-  f32x4 acc[4][4];
-  const int64_t steps = (int64_t)(t1 - t0) * slabs;
-  int tile = t0;
-  int slab = 0;
-  if (steps > 0) {
-    sw.load(a.w, a.v_begin + t0 * kTile, 0);
-    sh.load(a.h, n0, 0);
-    sw.store(lds[0][0]);
-    sh.store(lds[0][1]);
-  }
-  for (int64_t it = 0; it < steps; ++it) {
-    if (slab == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    __syncthreads();
-    if constexpr (USE == kStore)       // the barriers of one more step before use
-      if (slab == 0 && threadIdx.x < kTile) put_col(a, col, a.v_begin + tile * kTile);
-    const bool more = it + 1 < steps;
-    const int next_slab = slab + 1 == slabs ? 0 : slab + 1;
-    const int next_tile = slab + 1 == slabs ? tile + 1 : tile;
-    if (more) {
-      sw.load(a.w, a.v_begin + next_tile * kTile, next_slab);
-      sh.load(a.h, n0, next_slab);
-    }
-    const char* lw = lds[it & 1][0] + wm * 64 * kSlab;
-    const char* lh = lds[it & 1][1] + wn * 64 * kSlab;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      u32x4 fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = *reinterpret_cast<const u32x4*>(lw + row_slot(i * 16 + r16, k * 4 + g));
-        fb[i] = *reinterpret_cast<const u32x4*>(lh + row_slot(i * 16 + r16, k * 4 + g));
-      }
-      mma_all<TC>(fa, fb, acc);
-    }
-    if (slab + 1 == slabs) {
-      if constexpr (USE == kStore)
-        if (slabs == 1) __syncthreads();
-      f32x4 cs[4] = {};
-      if constexpr (USE == kStore)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          cs[i] = *reinterpret_cast<const f32x4*>(col + wm * 64 + i * 16 + 4 * g);
-      sink.template take<4>(a, acc, a.v_begin + tile * kTile + wm * 64 + 4 * g, n, cs);
-    }
-    if (more) {
-      sw.store(lds[(it + 1) & 1][0]);
-      sh.store(lds[(it + 1) & 1][1]);
-    }
-    slab = next_slab;
-    tile = next_tile;
-  }
-  if constexpr (USE == kLoss) sink.template finish_loss<2>(a, &lds[0][0][0], split, n0);
 }
 
 // 16 bytes a lane from global memory straight into LDS, 1 KB from `lds` on.
@@ -584,6 +455,14 @@ __device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint3
 }
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+// The same, 4 bytes a lane.
+__device__ __forceinline__ void load_lds4(const char* p, uint32_t offset, uint32_t lds) {
+  const uint64_t at = (uint64_t)p;
+  const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2"
+               :: "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 // Waits until only the last N loads and stores are outstanding: they end in
 // the order in which they were issued.
@@ -713,7 +592,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   }
   // Whether the wave makes all of kStores: then the last tile's stores, which
   // come after this tile's loads, need not be waited for.
-  const bool whole = n0 + (wn + 1) * (16 * NS) <= a.h.rows && (USE != kStore || (a.ldo & 3) == 0);
+  const bool whole = n0 + (wn + 1) * (16 * NS) <= a.n && (USE != kStore || (a.ldo & 3) == 0);
   for (int tile = t0; tile < t1; ++tile) {
     const int buf = (tile - t0) & 1;
     // the tile has arrived for all waves, and all are done with the other one
@@ -753,14 +632,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
             const float s = scales[buf][r * kBlocks + k / 4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              u32x4 fa;
-#pragma unroll
-              for (int w = 0; w < 2; ++w) {
-                fa[2 * w] = __builtin_bit_cast(uint32_t,
-                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * half + w], s, false));
-                fa[2 * w + 1] = __builtin_bit_cast(uint32_t,
-                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * half + w], s, true));
-              }
+              const u32x4 fa = fp8x8_to_bf16(q[2 * half], q[2 * half + 1], s);
               mma_row<kBF16>(fa, fb[k + half], acc[i]);
             }
           }
@@ -776,6 +648,144 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     put_scales(buf ^ 1);
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV>(a, lds[0], split, n0);
+}
+
+// Rows of any width, both sides by way of LDS: 64 WV table rows x 16 NS WN
+// samples per workgroup, 64 x 16 NS per wave.  Steps of 64 bytes of a sample's
+// row go straight into LDS, three steps ahead of the one at work.  Both sides'
+// rows start at multiples of 16 bytes; 8-bit table rows are converted when
+// they are read from LDS, and their scales lie by block of columns, then row.
+template <int TW, int TC, int USE, int WV, int WN, int NS>
+__global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
+  constexpr int kWaves = WV * WN, kAhead = 3, MR = 4;
+  constexpr int kV = 64 * WV, kN = 16 * NS * WN;
+  constexpr int kWideW = TW == kFP8 ? 32 : 64, kWideH = 64;   // bytes per step
+  constexpr int kBytesW = kV * kWideW, kBytesH = kN * kWideH;
+  constexpr int kBytesS = TW == kFP8 ? kV : 0;
+  constexpr int kInstr = (kBytesW + kBytesH) / 1024;          // loads of a whole wave
+  constexpr int kEach = kInstr / kWaves, kMore = kInstr % kWaves;
+  // the scales are one more load, of the last wave
+  constexpr int kScaleWave = TW == kFP8 ? kWaves - 1 : -1;
+  static_assert(kBytesW % 1024 == 0 && kBytesH % 1024 == 0 && kMore < kWaves, "");
+  static_assert(TW != kFP8 || kV == 256, "");
+  __shared__ __align__(16) char lds[kAhead + 1][kBytesW + kBytesH + kBytesS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = wave % WV, wn = wave / WV;
+  const int r16 = lane & 15, g = lane >> 4;
+  int tn, split;
+  if (!place(a, tn, split)) return;
+  int t0, t1;
+  part_of((a.v_end - a.v_begin + kV - 1) / kV, split, a.splits, t0, t1);
+  const int64_t n0 = (int64_t)tn * kN;
+  const int64_t n = n0 + wn * (16 * NS) + r16;
+  const int steps = (a.h.kb + kWideH - 1) / kWideH;
+  const int64_t all = (int64_t)(t1 - t0) * steps;
+  const int last_h = (int)min((int64_t)kN - 1, a.h.rows - 1 - n0);
+
+  // What lies outside is replaced by what is inside, and no lane sits out: the
+  // waits below count the loads of each wave.
+  int fetch_tile = t0, fetch_step = 0;
+  auto fetch = [&](int buf) {
+    const int v0 = a.v_begin + fetch_tile * kV;
+    const int last_w = min(kV - 1, (int)a.w.rows - 1 - v0);
+    const int ow = fetch_step * kWideW, oh = fetch_step * kWideH;
+    const char* bw = a.w.p + v0 * a.w.ld + ow;
+    const char* bh = a.h.p + n0 * a.h.ld + oh;
+    const int end_w = ((a.w.kb - 1) & ~15) - ow, end_h = ((a.h.kb - 1) & ~15) - oh;
+#pragma unroll
+    for (int i = 0; i < kEach + (kMore > 0); ++i) {
+      const int q = wave + kWaves * i;
+      if (q * 1024 < kBytesW) {
+        const int p = q * 64 + lane;
+        const int r = TW == kFP8 ? p >> 1 : p >> 2;
+        const int c = TW == kFP8 ? p & 1 : (p & 3) ^ ((r >> 2) & 3);
+        load_lds16(bw, (uint32_t)(min(r, last_w) * (int)a.w.ld + min(c * 16, end_w)),
+                   lds_address(&lds[buf][q * 1024]));
+      } else if (q < kInstr) {
+        const int p = (q - kBytesW / 1024) * 64 + lane;
+        const int r = p >> 2, c = (p & 3) ^ ((r >> 2) & 3);
+        load_lds16(bh, (uint32_t)(min(r, last_h) * (int)a.h.ld + min(c * 16, end_h)),
+                   lds_address(&lds[buf][q * 1024]));
+      }
+    }
+    if constexpr (TW == kFP8) {
+      // kV bytes, four to a lane; rows past the end have room
+      if (wave == kScaleWave)
+        load_lds4((const char*)a.w.scales + (int64_t)(ow >> 7) * a.w.lds + v0,
+                  (uint32_t)lane * 4, lds_address(&lds[buf][kBytesW + kBytesH]));
+    }
+    if (++fetch_step == steps) fetch_step = 0, ++fetch_tile;
+  };
+
+  Sink<USE, TC, NS> sink;
+  sink.start(a, n);
+  f32x4 acc[MR][NS];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (i < all) fetch(i);
+  int tile = t0, step = 0;
+  for (int64_t s = 0; s < all; ++s) {
+    // step s has arrived, two more may be on their way
+    if (s + kAhead - 1 < all) {
+      if (wave < kMore || wave == kScaleWave) wait_loads_but<(kAhead - 1) * (kEach + 1)>();
+      else wait_loads_but<(kAhead - 1) * kEach>();
+    } else {
+      wait_loads();
+    }
+    __syncthreads();
+    if (s + kAhead < all) fetch((int)(s + kAhead) & kAhead);
+    if (step == 0) {
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const char* buf = lds[s & kAhead];
+    const char* lh = buf + kBytesW + wn * (16 * NS) * kWideH;
+    const int at = r16 * 64 + ((g ^ (r16 >> 2)) << 4);
+    u32x4 fa[MR], fb[NS];
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      if constexpr (TW == kFP8) {
+        const int r = wv * 64 + i * 16 + r16;
+        const u32x2 q = *reinterpret_cast<const u32x2*>(buf + r * 32 + g * 8);
+        const uint8_t e = *reinterpret_cast<const uint8_t*>(buf + kBytesW + kBytesH + r);
+        fa[i] = fp8x8_to_bf16(q[0], q[1], scale_of(e));
+      } else {
+        fa[i] = *reinterpret_cast<const u32x4*>(buf + (wv * 64 + i * 16) * 64 + at);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+      fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64 + at);
+    if (step + 1 == steps && (a.h.kb & 63) != 0) {
+      // columns past the last one, whatever they hold
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
+        const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+#pragma unroll
+        for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
+      }
+    }
+    mma_all<TC>(fa, fb, acc);
+    if (++step == steps) {
+      const int v = a.v_begin + tile * kV + wv * 64 + 4 * g;
+      f32x4 cs[MR] = {};
+      if constexpr (USE == kStore)
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cs[i][e] = col_scale_of(a, v + i * 16 + e);
+      sink.template take<MR>(a, acc, v, n, cs);
+      step = 0;
+      ++tile;
+    }
+  }
+  if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
 }
 
 // Few samples: bound by the bytes of the table, which go from memory to the
@@ -865,14 +875,7 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
         if constexpr (TW == kFP8) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            u32x4 fa;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              fa[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-                  now[i][2 * half + w], scale[i], false));
-              fa[2 * w + 1] = __builtin_bit_cast(uint32_t,
-                  __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(now[i][2 * half + w], scale[i], true));
-            }
+            const u32x4 fa = fp8x8_to_bf16(now[i][2 * half], now[i][2 * half + 1], scale[i]);
             u32x4 f[NS];
 #pragma unroll
             for (int j = 0; j < NS; ++j)
@@ -964,67 +967,12 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(
 //   dh: r = sample, k = table row, b = coef[r][k]
 //   dw: r = table row, k = sample, b = coef[k][r]
 // x has k down its rows, so its tile is read from LDS transposed, as is b's
-// where it has too.
+// for dw.
 // ---------------------------------------------------------------------------
-// LDS tile with k down its rows, 128 columns: bf16 64 rows of 256 bytes, f32
-// 32 rows of 512 bytes.  Blocks of 16 columns are permuted by the row so that
-// the 16 rows that one transposing read touches spread over the banks.
-template <int T>
-__device__ __forceinline__ int col_slot(int k, int c) {
-  if constexpr (T == kBF16) {
-    const int f = (k & 3) | ((k >> 3) & 1) << 2;
-    return k * 256 + (((c >> 1) ^ f) << 5) + ((c & 1) << 4);
-  } else {
-    return k * 512 + (((c >> 2) ^ ((k >> 2) & 7)) << 6) + ((c & 3) << 4);
-  }
-}
-
-// 16 columns (block m) x one step of k, as the instruction takes them.
-template <int T>
-__device__ __forceinline__ u32x4 col_frag(const char* lds, int m, int step, int lane) {
-  const int g = lane >> 4, i = lane & 15;
-  if constexpr (T == kBF16) {
-    const int k = step * 32 + 8 * g + (i >> 2);
-    const int f = (k & 3) | ((k >> 3) & 1) << 2;
-    const char* p = lds + k * 256 + ((m ^ f) << 5) + (i & 3) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 256));
-    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-    return u32x4{a[0], a[1], b[0], b[1]};
-  } else {
-    const int k = step * 16 + 4 * g;
-    const char* p = lds + k * 512 + ((m ^ ((k >> 2) & 7)) << 6) + i * 4;
-    u32x4 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = *reinterpret_cast<const uint32_t*>(p + e * 512);
-    return r;
-  }
-}
-
-template <int T>
-struct ColTile {
-  static constexpr int kRowChunks = 128 * Elem<T>::size / 16;
-  u32x4 v[4];
-  __device__ __forceinline__ void load(const Rows& m, int64_t k0, int col0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = threadIdx.x + 256 * i;
-      v[i] = load16<Elem<T>::size>(m, k0 + q / kRowChunks,
-                                   col0 * Elem<T>::size + (q % kRowChunks) * 16);
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = threadIdx.x + 256 * i;
-      *reinterpret_cast<u32x4*>(lds + col_slot<T>(q / kRowChunks, q % kRowChunks)) = v[i];
-    }
-  }
-};
-
 struct GradArgs {
-  Rows x;        // [K][D]
-  Rows b;        // coef: [R][K] or [K][R]
+  Rows x;              // [K][D]
+  const char* coef;    // in blocks of 16 samples x 16 table rows
+  int64_t ldc;         // table rows of 16 samples' blocks
   int64_t r, k;
   int d;
   int tiles_d, tiles_r, splits;
@@ -1034,96 +982,6 @@ struct GradArgs {
   char* out;     // [R][D], of the rows' type
   int64_t ldo;
 };
-
-template <int T, bool DW>
-__global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
-  __shared__ __align__(16) char lds[2][2][kTileBytes];
-  constexpr int ES = Elem<T>::size;
-  constexpr int KS = kSlab / ES;     // k per step of the loop
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave & 1, wn = wave >> 1;
-  const int r16 = lane & 15, g = lane >> 4;
-  const int td = blockIdx.x % a.tiles_d;
-  const int tr = (blockIdx.x / a.tiles_d) % a.tiles_r;
-  const int split = blockIdx.x / (a.tiles_d * a.tiles_r);
-  const int64_t slabs = (a.k + KS - 1) / KS;
-  const int64_t s0 = slabs * split / a.splits, s1 = slabs * (split + 1) / a.splits;
-  const int64_t r0 = (int64_t)tr * kTile;
-  const int d0 = td * kTile;
-
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  ColTile<T> sx;
-  ColTile<T> sbc;
-  RowTile<T> sbr;
-  auto load = [&](int64_t s) {
-    sx.load(a.x, s * KS, d0);
-    if constexpr (DW) sbc.load(a.b, s * KS, (int)r0);
-    else sbr.load(a.b, r0, (int)s);
-  };
-  auto store = [&](int buf) {
-    sx.store(lds[buf][0]);
-    if constexpr (DW) sbc.store(lds[buf][1]);
-    else sbr.store(lds[buf][1]);
-  };
-  if (s0 < s1) {
-    load(s0);
-    store(0);
-  }
-  for (int64_t s = s0; s < s1; ++s) {
-    const int buf = (int)(s - s0) & 1;
-    __syncthreads();
-    if (s + 1 < s1) load(s + 1);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      u32x4 fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = col_frag<T>(lds[buf][0], wm * 4 + i, k, lane);
-        if constexpr (DW)
-          fb[i] = col_frag<T>(lds[buf][1], wn * 4 + i, k, lane);
-        else
-          fb[i] = *reinterpret_cast<const u32x4*>(
-              lds[buf][1] + row_slot(wn * 64 + i * 16 + r16, k * 4 + g));
-      }
-      mma_all<T>(fa, fb, acc);
-    }
-    if (s + 1 < s1) store(buf ^ 1);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t r = r0 + wn * 64 + j * 16 + r16;
-    if (r >= a.r) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = d0 + wm * 64 + i * 16 + 4 * g;
-      if (d >= a.d) continue;
-      if (a.part) {
-        f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
-        *o = a.add ? *o + acc[i][j] : acc[i][j];
-      } else {
-        char* o = a.out + (r * a.ldo + d) * ES;
-        if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
-          if constexpr (T == kF32)
-            *reinterpret_cast<f32x4*>(o) = acc[i][j];
-          else
-            *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(acc[i][j][0], acc[i][j][1]),
-                                                 pack_bf16(acc[i][j][2], acc[i][j][3])};
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < a.d) {
-              if constexpr (T == kF32) reinterpret_cast<float*>(o)[e] = acc[i][j][e];
-              else reinterpret_cast<__bf16*>(o)[e] = (__bf16)acc[i][j][e];
-            }
-        }
-      }
-    }
-  }
-}
 
 // Rows for the gradient: [rows][ldo] of 16-byte multiples with zeros behind
 // the last column and row, and (with targets) in rows that have no loss,
@@ -1148,21 +1006,24 @@ __global__ __launch_bounds__(256) void pack_kernel(
   }
 }
 
-// The same product for bf16 rows that start at multiples of 16 bytes: 256 rows
-// r and 32 ND columns d per workgroup of eight waves, 64 x 16 ND per wave, so
-// that narrow tables are read once and the coefficients, the larger part, as
-// often as there are tiles of d.  Steps of 32 k go straight into LDS, three
-// steps ahead of the one at work.
-template <int ND, bool DW>
-__global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
-  constexpr int kRowsR = 256, kStep = 32, kAhead = 3;
-  constexpr int kPitchX = 64 * ND;                   // bytes of a row k
-  constexpr int kChunksX = kPitchX / 16;
-  constexpr int kBytesX = kStep * kPitchX, kBytesB = kStep * kRowsR * 2;
+// 256 rows r and 32 ND columns d per workgroup of eight waves, 64 x 16 ND per
+// wave, so that narrow tables are read once and the coefficients, the larger
+// part, as often as there are tiles of d.  Steps of 64 bytes of k (32 of bf16,
+// 16 of float32) go straight into LDS, three steps ahead of the one at work.
+template <int T, int ND, bool DW>
+__global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
+  constexpr int ES = Elem<T>::size;
+  constexpr int kRowsR = 256, kStep = 64 / ES, kAhead = 3;
+  constexpr int kPitchX = 32 * ND * ES, kPitchB = kRowsR * ES;   // bytes of a row k
+  constexpr int kChunksX = kPitchX / 16, kChunksB = kPitchB / 16;
+  constexpr int kBytesX = kStep * kPitchX, kBytesB = kStep * kPitchB;
   constexpr int kInstrX = kBytesX / 1024;            // loads of a whole wave
   constexpr int kMoreX = kInstrX % 8;                // waves with one more
+  constexpr int kBlock = 256 * ES;                   // bytes of 16 x 16 coefficients
+  constexpr int kLine = 16 * ES;                     // of which one sample's
   __shared__ __align__(16) char lds[kAhead + 1][kBytesX + kBytesB];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wd = wave & 1, wr = wave >> 1;
   const int r16 = lane & 15, g = lane >> 4;
   // the parts of k go round the XCDs: the tiles of r that share rows of x are
@@ -1178,23 +1039,25 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
   const int64_t r0 = (int64_t)tr * kRowsR;
   const int d0 = td * 32 * ND;
 
-  // Blocks of 16 columns of row k lie at block ^ key(k): the rows of one
-  // transposing read spread over the banks.
+  // Blocks of 16 columns (of kLine bytes) of row k lie at block ^ key(k): the
+  // rows that one transposing read touches spread over the banks.
   auto key = [](int k, int pitch) {
-    return pitch % 256 == 0 ? (k & 3) | ((k >> 3) & 1) << 2
-                            : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+    if constexpr (T == kF32) return (k >> 2) & 3;
+    else return pitch % 256 == 0 ? (k & 3) | ((k >> 3) & 1) << 2
+                                 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
   };
+  constexpr int kPer = kLine / 16;                   // chunks of a block's row
   // What lies outside is replaced by what is inside, and no lane sits out: the
   // waits below count the loads of each wave.  Columns d and rows r past the
   // end are not stored; past the last k, one side is zeros.
-  const int have_chunks = (a.x.kb - d0 * 2 + 15) / 16;     // columns of x from d0 on
-  const int64_t block_row = a.b.ld * 16;                   // 16 rows of coefficients
-  const int have_b = DW ? (int)((a.b.kb - r0 * 2 + 15) / 16)     // chunks of a row
-                        : (int)min((int64_t)kRowsR, a.b.rows - r0);
+  const int have_x = (a.x.kb - d0 * ES + 15) / 16;   // chunks of x from d0 on
+  const int64_t block_row = a.ldc * kLine;           // 16 samples' coefficients
+  const int have_b = (int)min((int64_t)(DW ? kChunksB : kRowsR),
+                              DW ? ((a.r - r0) * ES + 15) / 16 : a.r - r0);
   auto fetch = [&](int s) {
     char* buf = lds[(s - s0) & kAhead];
     const int64_t k0 = (int64_t)s * kStep;
-    const char* xb = a.x.p + k0 * a.x.ld + d0 * 2;
+    const char* xb = a.x.p + k0 * a.x.ld + d0 * ES;
     const int last = (int)min((int64_t)kStep - 1, a.x.rows - 1 - k0);
 #pragma unroll
     for (int i = 0; i < (kInstrX + 7) / 8; ++i) {
@@ -1202,8 +1065,8 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
       if (q < kInstrX) {
         const int p = q * 64 + lane;
         const int k = p / kChunksX, pos = p % kChunksX;
-        const int c = ((pos >> 1) ^ key(k, kPitchX)) * 2 + (pos & 1);
-        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + min(c, have_chunks - 1) * 16),
+        const int c = ((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer;
+        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + min(c, have_x - 1) * 16),
                    lds_address(buf + q * 1024));
       }
     }
@@ -1212,22 +1075,22 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
       const int q = wave + 8 * i;
       const int p = q * 64 + lane;
       if constexpr (DW) {
-        const int k = p >> 5, pos = p & 31;
-        const int c = ((pos >> 1) ^ key(k, 512)) * 2 + (pos & 1);
-        // two rows of blocks, chunk c is half of block c / 2
+        // samples k, chunk c of 256 table rows
+        const int k = p / kChunksB, pos = p % kChunksB;
+        const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
         const int in = min(c, have_b - 1);
-        load_lds16(a.b.p + (k0 >> 4) * block_row + r0 * 32,
-                   (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * 32 + (in >> 1) * 512 +
-                       (in & 1) * 16,
+        load_lds16(a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock,
+                   (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * kLine +
+                       in / kPer * kBlock + in % kPer * 16,
                    lds_address(buf + kBytesX + q * 1024));
       } else {
-        // rows r of 32 coefficients: chunk c at c ^ ((r >> 2) & 3)
+        // 64 bytes of samples r: chunk c at c ^ ((r >> 2) & 3)
         const int r = p >> 2;
         const int c = (p & 3) ^ ((r >> 2) & 3);
         const int in = min(r, have_b - 1);
-        load_lds16(a.b.p + (r0 >> 4) * block_row + k0 * 32,
-                   (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * 32 + (c >> 1) * 512 +
-                       (c & 1) * 16,
+        load_lds16(a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock,
+                   (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * kLine +
+                       c / kPer * kBlock + c % kPer * 16,
                    lds_address(buf + kBytesX + q * 1024));
       }
     }
@@ -1241,14 +1104,23 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
     if (s0 + i < s1) fetch(s0 + i);
-  // a transposing read: 16 lanes take 4 rows k of one block of 16 columns
+  // 16 columns x one step of k: for bf16 by transposing reads, in which 16
+  // lanes take 4 rows k of one block; for float32 a word at a time
   auto columns = [&](const char* p, int pitch, int block) {
-    const int k = 8 * g + (r16 >> 2);
-    const char* q = p + k * pitch + ((block ^ key(k, pitch)) << 5) + (r16 & 3) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * pitch));
-    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-    return u32x4{x[0], x[1], y[0], y[1]};
+    if constexpr (T == kBF16) {
+      const int k = 8 * g + (r16 >> 2);
+      const char* q = p + k * pitch + ((block ^ key(k, pitch)) << 5) + (r16 & 3) * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 4 * pitch));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      return u32x4{x[0], x[1], y[0], y[1]};
+    } else {
+      const char* q = p + 4 * g * pitch + ((block ^ key(4 * g, pitch)) << 6) + r16 * 4;
+      u32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const uint32_t*>(q + e * pitch);
+      return x;
+    }
   };
   for (int s = s0; s < s1; ++s) {
     // step s has arrived, two more may be on their way
@@ -1266,7 +1138,7 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (DW) {
-        fb[j] = columns(b, 512, wr * 4 + j);
+        fb[j] = columns(b, kPitchB, wr * 4 + j);
       } else {
         const int r = wr * 64 + j * 16 + r16;
         fb[j] = *reinterpret_cast<const u32x4*>(b + r * 64 + ((g ^ ((r >> 2) & 3)) << 4));
@@ -1275,7 +1147,7 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
       const u32x4 fa = columns(x, kPitchX, wd * ND + i);
-      mma_row<kBF16>(fa, fb, acc[i]);
+      mma_row<T>(fa, fb, acc[i]);
     }
   }
 #pragma unroll
@@ -1289,11 +1161,20 @@ __global__ __launch_bounds__(512, 2) void grad_wide_kernel(GradArgs a) {
       if (a.part) {
         f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
         *o = a.add ? *o + acc[i][j] : acc[i][j];
+      } else if constexpr (T == kF32) {
+        float* o = reinterpret_cast<float*>(a.out) + r * a.ldo + d;
+        if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
+          *reinterpret_cast<f32x4*>(o) = acc[i][j];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.d) o[e] = acc[i][j][e];
+        }
       } else {
         uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + r * a.ldo + d;
         const uint32_t lo = pack_bf16(acc[i][j][0], acc[i][j][1]);
         const uint32_t hi = pack_bf16(acc[i][j][2], acc[i][j][3]);
-        if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
+        if ((a.ldo & 3) == 0) {
           *reinterpret_cast<u32x2*>(o) = u32x2{lo, hi};
         } else {
 #pragma unroll
@@ -1552,7 +1433,7 @@ template <int KS, int NS, int WN, int USE, bool FP8>
 static void launch_resident_k(ScoreArgs& a, hipStream_t stream) {
   constexpr auto kernel = resident_kernel<KS, NS, WN, USE, FP8>;
   static const int slots = slots_of(kernel, 256, 0);
-  a.tiles_n = grid_of((a.h.rows + 16 * NS * WN - 1) / (16 * NS * WN));
+  a.tiles_n = grid_of((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
   cut(a, KS <= 4 ? 128 : 64, slots);
   kernel<<<score_grid(a), 256, 0, stream>>>(a);
 }
@@ -1560,7 +1441,7 @@ static void launch_resident_k(ScoreArgs& a, hipStream_t stream) {
 template <int USE, bool FP8>
 static void launch_resident(ScoreArgs& a, int64_t cols, hipStream_t stream) {
   const int ks = (int)((cols + 63) / 64) * 2;
-  const bool few = a.h.rows <= 64, least = a.h.rows <= 16;
+  const bool few = a.n <= 64, least = a.n <= 16;
 #define CASE_KS(K)                                                              \
   if (ks == K) {                                                                \
     if constexpr (USE != kCoef)                                                 \
@@ -1573,13 +1454,26 @@ static void launch_resident(ScoreArgs& a, int64_t cols, hipStream_t stream) {
   throw std::runtime_error("rows too wide");
 }
 
-template <int TW, int TH, int USE>
-static void launch_scores(ScoreArgs& a, hipStream_t stream) {
-  constexpr auto kernel = scores_kernel<TW, TH, USE>;
-  static const int slots = slots_of(kernel, 256, 0);
-  a.tiles_n = grid_of((a.h.rows + kTile - 1) / kTile);
-  cut(a, kTile, slots);
-  kernel<<<score_grid(a), 256, 0, stream>>>(a);
+template <int TW, int TC, int USE, int WV, int WN, int NS>
+static void launch_tile_k(ScoreArgs& a, hipStream_t stream) {
+  constexpr auto kernel = tile_kernel<TW, TC, USE, WV, WN, NS>;
+  static const int slots = slots_of(kernel, 64 * WV * WN, 0);
+  a.tiles_n = grid_of((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
+  cut(a, 64 * WV, slots);
+  kernel<<<score_grid(a), 64 * WV * WN, 0, stream>>>(a);
+}
+
+template <int TW, int TC, int USE>
+static void launch_tile(ScoreArgs& a, hipStream_t stream) {
+  for (const Rows* r : {&a.w, &a.h})
+    if (r->align != 16 || r->ld >= (1 << 23)) throw std::runtime_error("rows not aligned");
+  const int64_t rows = a.v_end - a.v_begin;
+  if (a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
+  // 256 x 256 needs 256 of them to fill the card
+  if constexpr (TW != kFP8)
+    if (((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
+      return launch_tile_k<TW, TC, USE, 2, 2, 4>(a, stream);
+  launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
 }
 
 // LDS that the samples of the streaming kernel take; 4 KB at least, for the
@@ -1589,11 +1483,12 @@ static int64_t stream_bytes(const ScoreArgs& a, int ns, bool fp8) {
 }
 constexpr int64_t kMostStream = 64 << 10;
 
-template <int TW, int TC, int NS, int USE, bool VEC>
+template <int TW, int TC, int NS, int USE>
 static void launch_stream(ScoreArgs& a, hipStream_t stream) {
-  constexpr auto kernel = stream_kernel<TW, TC, NS, USE, VEC>;
+  const auto kernel = a.w.align == 16 ? stream_kernel<TW, TC, NS, USE, true>
+                                      : stream_kernel<TW, TC, NS, USE, false>;
   const int lds = (int)stream_bytes(a, NS, TW == kFP8);
-  a.tiles_n = grid_of((a.h.rows + 16 * NS - 1) / (16 * NS));
+  a.tiles_n = grid_of((a.n + 16 * NS - 1) / (16 * NS));
   cut(a, 64, slots_of(kernel, 256, lds));
   kernel<<<score_grid(a), 256, lds, stream>>>(a);
 }
@@ -1605,40 +1500,76 @@ static void launch_any(ScoreArgs& a, int64_t cols, hipStream_t stream) {
   if constexpr (TC == kBF16)
     if (is_resident(a, cols)) return launch_resident<USE, fp8>(a, cols, stream);
   if constexpr (USE != kCoef)
-    if (a.h.rows <= 16 && stream_bytes(a, 1, fp8) <= kMostStream)
-      return a.w.align == 16 ? launch_stream<TW, TC, 1, USE, true>(a, stream)
-                             : launch_stream<TW, TC, 1, USE, false>(a, stream);
-  launch_scores<TW, TC, USE>(a, stream);
+    if (a.n <= 16 && stream_bytes(a, 1, fp8) <= kMostStream)
+      return launch_stream<TW, TC, 1, USE>(a, stream);
+  if constexpr (fp8) throw std::runtime_error("no workspace for the scales");
+  else launch_tile<TW, TC, USE>(a, stream);
 }
 
-// part: part_size pairs of float, n for each part of the table
+// rows [np][dp] at `to`, see pack_kernel
+static Rows pack(const Rows& r, int is_bf16, const void* targets, int targets64, int64_t ignore,
+                 int64_t vocab, uintptr_t to, int64_t np, int64_t dp, hipStream_t stream) {
+  const int es = is_bf16 ? 2 : 4;
+  if (to % 16 != 0) throw std::runtime_error("no workspace for rows");
+  const int blocks = (int)std::min<int64_t>((np * dp * es / 16 + 255) / 256, 8192);
+  if (is_bf16) pack_kernel<kBF16><<<blocks, 256, 0, stream>>>(
+      r, targets, targets64, ignore, vocab, (char*)to, np, (int)dp);
+  else pack_kernel<kF32><<<blocks, 256, 0, stream>>>(
+      r, targets, targets64, ignore, vocab, (char*)to, np, (int)dp);
+  Rows packed = r;
+  packed.p = (const char*)to;
+  packed.ld = dp * es;
+  packed.rows = np;
+  packed.align = 16;
+  return packed;
+}
+
+// part: part_size pairs of float, n for each part of the table.  packed_h
+// [n][dp] and packed_w [piece][dp], with dp = d rounded up to 64, or null where
+// rows can be read as they lie: they start at multiples of 16 bytes and less
+// than 2^23 bytes apart, or the streaming kernel takes them.
 static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
-                         int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t loss,
-                         uintptr_t lse, int reduce, uintptr_t reduced, int device, uintptr_t stream_ptr) {
+                         int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t packed_h,
+                         uintptr_t packed_w, int64_t piece, uintptr_t loss, uintptr_t lse,
+                         int reduce, uintptr_t reduced, int device, uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
+  const int64_t dp = (d + 63) / 64 * 64;
   if (n > 0) {
+    const Rows rw = make_rows(w, ldw, v, d, es), rh = make_rows(h, ldh, n, d, es);
     ScoreArgs a{};
-    a.w = make_rows(w, ldw, v, d, es);
-    a.h = make_rows(h, ldh, n, d, es);
-    a.v_begin = 0;
-    a.v_end = (int)v;
-    a.part = (float2*)part;
+    a.n = n;
+    a.h = rh;
     a.ldp = n;
-    a.splits = (int)std::min<int64_t>(1 << 20, part_size / n);
-    if (a.splits < 1) throw std::runtime_error("workspace too small");
-    const int joins = grid_of((n + 3) / 4);
-    if (is_bf16) {
-      launch_any<kBF16, kBF16, kLoss>(a, d, stream);
-      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
-          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
-    } else {
-      launch_any<kF32, kF32, kLoss>(a, d, stream);
-      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(a.w, a.h, a.part, a.splits, a.ldp,
-          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
+    const bool pack_w = packed_w != 0;
+    if (packed_h)
+      a.h = pack(rh, is_bf16, nullptr, 0, 0, 0, packed_h, n, dp, stream);
+    if (!pack_w) piece = v;
+    const int64_t pieces = (v + piece - 1) / piece;
+    int parts = 0;
+    for (int64_t v0 = 0; v0 < v; v0 += piece) {
+      const int64_t v1 = std::min(v, v0 + piece);
+      a.w = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
+      if (pack_w)
+        a.w = pack(a.w, is_bf16, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
+      a.v_begin = 0;
+      a.v_end = (int)(v1 - v0);
+      a.part = (float2*)part + parts * n;
+      a.splits = (int)std::min<int64_t>(1 << 20, part_size / n / pieces);
+      if (a.splits < 1) throw std::runtime_error("workspace too small");
+      if (is_bf16) launch_any<kBF16, kBF16, kLoss>(a, d, stream);
+      else launch_any<kF32, kF32, kLoss>(a, d, stream);
+      parts += a.splits;
     }
+    const int joins = grid_of((n + 3) / 4);
+    if (is_bf16)
+      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(rw, rh, (const float2*)part, parts, n,
+          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
+    else
+      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(rw, rh, (const float2*)part, parts, n,
+          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
   }
   if (reduce)      // 1: sum, 2: mean
     loss_reduce_kernel<<<1, 1024, 0, stream>>>((const float*)loss, (const void*)targets,
@@ -1659,66 +1590,54 @@ static void wide_tiles(int d, int& nd, int& tiles) {
   nd = ((d + tiles - 1) / tiles + 63) / 64 * 2;
 }
 
-template <bool DW>
-static void launch_grad_wide(GradArgs b, hipStream_t stream) {
+template <int T, bool DW>
+static void launch_grad(GradArgs b, hipStream_t stream) {
   int nd;
   wide_tiles(b.d, nd, b.tiles_d);
   b.tiles_r = grid_of((b.r + 255) / 256);
   const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
   const int blocks = grid_of(b.splits >= 8 ? tiles * ((b.splits + 7) / 8) * 8 : tiles * b.splits);
-  if (nd == 2) grad_wide_kernel<2, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 4) grad_wide_kernel<4, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 6) grad_wide_kernel<6, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 8) grad_wide_kernel<8, DW><<<blocks, 512, 0, stream>>>(b);
-  else grad_wide_kernel<10, DW><<<blocks, 512, 0, stream>>>(b);
+  if (nd == 2) grad_kernel<T, 2, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 4) grad_kernel<T, 4, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 6) grad_kernel<T, 6, DW><<<blocks, 512, 0, stream>>>(b);
+  else if (nd == 8) grad_kernel<T, 8, DW><<<blocks, 512, 0, stream>>>(b);
+  else grad_kernel<T, 10, DW><<<blocks, 512, 0, stream>>>(b);
 }
 
 // packed: [np][dp] elements with np = n rounded up to 32, dp = d rounded up to
-// 64; packed_w: [chunk][dp] where bf16 rows of w do not start at multiples of
-// 16 bytes or lie 2^25 bytes apart, else null; coef: [np][chunk] elements; part: [splits][n][ldp]
-// floats; part_w: [splits_w][chunk][ldp] where splits_w > 1
+// 64; packed_w: [chunk][dp], or null where rows of w start at multiples of 16
+// bytes and less than 2^23 bytes apart; coef: [np][chunk] elements; part:
+// [splits][n][ldp] floats; part_w: [splits_w][chunk][ldp] where splits_w > 1
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
-                         uintptr_t weight, uintptr_t packed, uintptr_t packed_w, int64_t chunk, uintptr_t coef,
-                         int splits, uintptr_t part, int splits_w, uintptr_t part_w, int64_t ldp,
-                         uintptr_t dh, uintptr_t dw,
-                         int device, uintptr_t stream_ptr) {
+                         uintptr_t weight, uintptr_t packed, uintptr_t packed_w, int64_t chunk,
+                         uintptr_t coef, int splits, uintptr_t part, int splits_w,
+                         uintptr_t part_w, int64_t ldp, uintptr_t dh, uintptr_t dw, int device,
+                         uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
-  if (chunk % kTile != 0 || ldp % 4 != 0 || packed % 16 != 0 || coef % 16 != 0)
+  if (chunk % 256 != 0 || ldp % 4 != 0 || coef % 16 != 0)
     throw std::runtime_error("bad workspace shape");
   if (n == 0) throw std::runtime_error("no rows");
   const int64_t np = (n + 31) / 32 * 32, dp = (d + 63) / 64 * 64;
   const Rows rw = make_rows(w, ldw, v, d, es);
-  Rows rh = make_rows(h, ldh, n, d, es);
-  const int pack_blocks = (int)std::min<int64_t>((np * dp * es / 16 + 255) / 256, 4096);
-  if (is_bf16) pack_kernel<kBF16><<<pack_blocks, 256, 0, stream>>>(
-      rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
-  else pack_kernel<kF32><<<pack_blocks, 256, 0, stream>>>(
-      rh, (const void*)targets, targets64, ignore, v, (char*)packed, np, (int)dp);
-  rh = make_rows(packed, dp, n, d, es);
-  // the wide kernel's offsets within a step have 32 bits
-  const bool pack_w = is_bf16 && !(rw.align == 16 && rw.ld < (1 << 25));
-  if (pack_w && !packed_w) throw std::runtime_error("no workspace for the table's rows");
-  const int tiles_n = grid_of((n + kTile - 1) / kTile);
-  const int tiles_d = (int)((d + kTile - 1) / kTile);
+  const Rows rh = pack(make_rows(h, ldh, n, d, es), is_bf16, (const void*)targets, targets64,
+                       ignore, v, packed, np, dp, stream);
+  const bool pack_w = packed_w != 0;
   for (int64_t v0 = 0; v0 < v; v0 += chunk) {
     const int64_t v1 = std::min(v, v0 + chunk);
     // the table's rows from v0 on; v_begin and the targets count from row 0
     Rows piece = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
-    if (pack_w) {
-      const int blocks = (int)std::min<int64_t>(((v1 - v0) * dp * es / 16 + 255) / 256, 8192);
-      pack_kernel<kBF16><<<blocks, 256, 0, stream>>>(piece, nullptr, 0, 0, 0, (char*)packed_w,
-                                                     v1 - v0, (int)dp);
-      piece = make_rows(packed_w, dp, v1 - v0, d, es);
-    }
+    if (pack_w)
+      piece = pack(piece, is_bf16, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
     ScoreArgs a{};
     a.w = piece;
     a.w.p -= v0 * a.w.ld;
     a.w.rows = v1;
     a.h = rh;
+    a.n = n;
     a.splits = 1 << 20;
     a.v_begin = (int)v0;
     a.v_end = (int)v1;
@@ -1736,38 +1655,31 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     if (is_bf16) launch_any<kBF16, kBF16, kCoef>(a, d, stream);
     else launch_any<kF32, kF32, kCoef>(a, d, stream);
     GradArgs b{};
+    b.coef = (const char*)coef;
+    b.ldc = chunk;
     b.d = (int)d;
-    b.tiles_d = tiles_d;
+    b.ldp = ldp;
     if (dh) {
       b.x = piece;
-      b.b = make_rows(coef, chunk, n, v1 - v0, es);
       b.r = n;
       b.k = v1 - v0;
-      b.tiles_r = tiles_n;
       b.splits = splits;
       b.part = (float*)part;
-      b.ldp = ldp;
       b.add = v0 > 0;
-      const int blocks = grid_of((int64_t)tiles_d * tiles_n * splits);
-      if (is_bf16) launch_grad_wide<false>(b, stream);
-      else grad_kernel<kF32, false><<<blocks, 256, 0, stream>>>(b);
+      if (is_bf16) launch_grad<kBF16, false>(b, stream);
+      else launch_grad<kF32, false>(b, stream);
     }
     if (dw) {
-      const int tiles_v = grid_of((v1 - v0 + kTile - 1) / kTile);
-      b.x = make_rows(packed, dp, np, dp, es);
-      b.b = make_rows(coef, chunk, np, v1 - v0, es);
+      b.x = rh;
       b.r = v1 - v0;
       b.k = n;
-      b.tiles_r = tiles_v;
       b.splits = splits_w;
-      b.add = 0;
       b.part = splits_w > 1 ? (float*)part_w : nullptr;
-      b.ldp = ldp;
+      b.add = 0;
       b.out = (char*)dw + v0 * d * es;
       b.ldo = d;
-      const int blocks = grid_of((int64_t)tiles_d * tiles_v * splits_w);
-      if (is_bf16) launch_grad_wide<true>(b, stream);
-      else grad_kernel<kF32, true><<<blocks, 256, 0, stream>>>(b);
+      if (is_bf16) launch_grad<kBF16, true>(b, stream);
+      else launch_grad<kF32, true>(b, stream);
       if (splits_w > 1)
         launch_sum_parts(b.part, splits_w, v1 - v0, ldp, d, is_bf16, b.out, stream);
     }
@@ -1820,10 +1732,21 @@ static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int
   HIP_CHECK(hipGetLastError());
 }
 
-// a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n]
+// The scales of 8-bit rows by block of columns, as the tile kernel takes them.
+__global__ __launch_bounds__(256) void turn_scales_kernel(
+    const uint8_t* scales, int64_t lds, int64_t rows, int blocks, uint8_t* out, int64_t ldo) {
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int b = 0; b < blocks; ++b)
+    out[b * ldo + r] = scales[min(r, rows - 1) * lds + b];
+}
+
+// a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n]; turned: a byte for
+// every block of 128 columns and row, rows rounded up to 256, or null where
+// k <= 320, or m <= 16 and k <= 2048
 static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,
                         uintptr_t scales, int64_t lds, int64_t n, int64_t k, uintptr_t col_scale,
-                        uintptr_t out, int out_bf16, int device, uintptr_t stream_ptr) {
+                        uintptr_t out, int out_bf16, uintptr_t turned, int device,
+                        uintptr_t stream_ptr) {
   const OnDevice on(device);
   if (m == 0 || n == 0) return;
   hipStream_t stream = (hipStream_t)stream_ptr;
@@ -1831,6 +1754,7 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
   ScoreArgs a{};
   a.w = make_fp8(values, ldv, scales, lds, n, k);
   a.h = make_rows(a_ptr, lda, m, k, 2);
+  a.n = m;
   a.splits = 1 << 20;
   a.v_begin = 0;
   a.v_end = (int)n;
@@ -1838,7 +1762,16 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
   a.out = (char*)out;
   a.ldo = n;
   a.out_bf16 = out_bf16;
-  launch_any<kFP8, kBF16, kStore>(a, k, stream);
+  if (turned) {
+    const int64_t ldo = (n + 255) / 256 * 256;
+    turn_scales_kernel<<<grid_of(ldo / 256), 256, 0, stream>>>(
+        a.w.scales, a.w.lds, n, (int)((k + 127) / 128), (uint8_t*)turned, ldo);
+    a.w.scales = (const uint8_t*)turned;
+    a.w.lds = ldo;
+    launch_tile<kFP8, kBF16, kStore>(a, stream);
+  } else {
+    launch_any<kFP8, kBF16, kStore>(a, k, stream);
+  }
   HIP_CHECK(hipGetLastError());
 }
 

@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 
-from .softmax import _ceil, _native, _place, _rows
+from .softmax import _aligned, _ceil, _native, _place, _rows
 
 BLOCK = 128
 
@@ -154,6 +154,15 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
                                f"{b.device}")
         col_scale = col_scale.detach().contiguous()
     out = torch.empty((m, n), dtype=out_dtype, device=b.device)
+    values, scales = b
+    if not _aligned(values):
+        values = torch.empty((n, _ceil(k, 16) * 16), dtype=torch.uint8,
+                             device=b.device)
+        values[:, :k] = b.values.view(torch.uint8)
+    # the scales by block of columns, for the kernel that takes wide rows
+    turned = None if k <= 320 or (m <= 16 and k <= 2048) else \
+        torch.empty(_ceil(k, BLOCK) * _ceil(n, 256) * 256, dtype=torch.uint8,
+                    device=b.device)
     ld = _ceil(k, 8) * 8
     held = torch.empty((m, ld), dtype=torch.bfloat16, device=b.device)
     native, place = _native(), _place(b.device)
@@ -168,8 +177,9 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
             int(a.dtype == torch.bfloat16), held.data_ptr(), ld, 0, 0, 1,
             *place)
     native.matmul_rows(
-        held.data_ptr(), ld, m, b.values.data_ptr(), b.values.stride(0),
-        b.scales.data_ptr(), b.scales.stride(0), n, k,
+        held.data_ptr(), ld, m, values.data_ptr(), values.stride(0),
+        scales.data_ptr(), scales.stride(0), n, k,
         0 if col_scale is None else col_scale.data_ptr(), out.data_ptr(),
-        int(out_dtype == torch.bfloat16), *place)
+        int(out_dtype == torch.bfloat16),
+        0 if turned is None else turned.data_ptr(), *place)
     return out

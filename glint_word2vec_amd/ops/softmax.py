@@ -23,9 +23,9 @@ from typing import Optional, Tuple
 import torch
 
 # Pieces of the vocabulary are as wide as keeps their coefficients within
-# this.
+# this, and packed copies of unaligned tables within that.
 _COEF_BYTES = 512 << 20
-_TILE = 128
+_PACKED_BYTES = 256 << 20
 _PARTS = 4096
 
 
@@ -88,6 +88,13 @@ def _check(h, w, targets) -> None:
                            f"{h.device}, {w.device}, {targets.device}")
 
 
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether the kernels read rows as they lie: they start at multiples of
+    16 bytes, less than 2^23 bytes apart."""
+    step = t.stride(0) * t.element_size()
+    return t.data_ptr() % 16 == 0 and step % 16 == 0 and step < 1 << 23
+
+
 def _parts(tiles: int, slots: int, most: int) -> int:
     """Parts of a product's long axis for `tiles` results on `slots` places:
     the fewest that fill nine tenths of what any number up to `most` fills."""
@@ -109,17 +116,29 @@ def _forward(h, w, targets, ignore_index, reduce: int):
     lse = torch.empty_like(loss)
     reduced = torch.empty(2, dtype=torch.float32, device=h.device) \
         if reduce else None
-    # a maximum and a sum of every row for each part of the vocabulary: parts
-    # for enough workgroups, of 128 or more words
-    parts = min(_ceil(v, 64), max(1, _PARTS // max(1, _ceil(n, 128))))
+    size, dp = h.element_size(), _ceil(d, 64) * 64
+    packed_h = packed_w = None
+    piece = v
+    if not (n <= 16 and d * size <= 4096):    # the streaming kernel takes any
+        if not _aligned(h):
+            packed_h = torch.empty(n * dp, dtype=h.dtype, device=h.device)
+        if not _aligned(w):
+            piece = max(256, _PACKED_BYTES // (dp * size) // 256 * 256)
+            packed_w = torch.empty(min(piece, v) * dp, dtype=w.dtype,
+                                   device=w.device)
+    # a maximum and a sum of every row for each part of the vocabulary
+    parts = max(_ceil(v, piece), min(_ceil(v, 64),
+                                     _PARTS // max(1, _ceil(n, 128))))
     part = torch.empty(parts * n * 2, dtype=torch.float32, device=h.device)
     _native().softmax_loss(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
         int(h.dtype == torch.bfloat16), targets.data_ptr(),
         int(targets.dtype == torch.int64), int(ignore_index),
-        part.data_ptr(), parts * n, loss.data_ptr(), lse.data_ptr(), reduce,
-        0 if reduced is None else reduced.data_ptr(),
-        *_place(h.device))
+        part.data_ptr(), parts * n,
+        0 if packed_h is None else packed_h.data_ptr(),
+        0 if packed_w is None else packed_w.data_ptr(), piece,
+        loss.data_ptr(), lse.data_ptr(), reduce,
+        0 if reduced is None else reduced.data_ptr(), *_place(h.device))
     return loss, lse, reduced
 
 
@@ -142,17 +161,14 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
     pieces = _ceil(v, max(256, _COEF_BYTES // (rows * size)))
     width = _ceil(_ceil(v, pieces), 256) * 256
     coef = torch.empty(rows * width, dtype=h.dtype, device=h.device)
-    aligned = w.data_ptr() % 16 == 0 and w.stride(0) * size % 16 == 0 \
-        and w.stride(0) * size < 1 << 25
-    packed_w = None if size == 4 or aligned else \
+    packed_w = None if _aligned(w) else \
         torch.empty(width * _ceil(d, 64) * 64, dtype=w.dtype, device=w.device)
     ldp = _ceil(d, 4) * 4
-    # tiles of the products' results, and workgroups that the card holds
-    edge, cols, slots = (256, 320, 256) if size == 2 else (128, 128, 512)
-    splits = _parts(_ceil(n, edge) * _ceil(d, cols), slots,
-                    _ceil(width, 256)) if need_h else 1
-    splits_w = _parts(_ceil(min(v, width), edge) * _ceil(d, cols), slots,
-                      _ceil(n, 256)) if need_w else 1
+    # parts of the long axis where a product's result has few tiles
+    splits = _parts(_ceil(n, 256) * _ceil(d, 320), 256,
+                    _ceil(width, 64)) if need_h else 1
+    splits_w = _parts(_ceil(min(v, width), 256) * _ceil(d, 320), 256,
+                      _ceil(n, 64)) if need_w else 1
     part = torch.empty(splits * n * ldp if need_h else 0,
                        dtype=torch.float32, device=h.device)
     part_w = torch.empty(splits_w * width * ldp if splits_w > 1 else 0,
