@@ -17,11 +17,13 @@
 
 #include <hip/hip_runtime.h>
 #include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 namespace py = pybind11;
 
@@ -439,6 +441,16 @@ __device__ __forceinline__ void part_of(int tiles, int split, int splits, int& t
   t1 = t0 + each + (split < more);
 }
 
+// Where chunk c of 16 bytes of row r lies in LDS, for rows of `pitch` bytes: a
+// read of 16 bytes a lane, in which lanes 0-15 have chunk c of 16 rows, 16-31
+// chunk c + 1 and so on, is served 16 lanes at a time, and not in order (0-3,
+// 12-15, 20-27 first): these take all 64 banks.
+__device__ __forceinline__ constexpr int row_chunk(int pitch, int r, int c) {
+  const int q = (r >> 2) & 3;
+  return pitch % 256 == 0 ? c ^ (r & 15) : pitch % 128 == 0 ? c ^ (r & 7)
+                                         : c ^ (q & 1) << 1 ^ (q >> 1) * 3;
+}
+
 // The factor of table row v in stored scores.
 __device__ __forceinline__ float col_scale_of(const ScoreArgs& a, int v) {
   return a.col_scale && v < a.v_end ? a.col_scale[v] : 1.f;
@@ -508,17 +520,12 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   const int64_t n0 = (int64_t)tn * (16 * NS * WN);
   const int64_t n = n0 + wn * (16 * NS) + r16;
 
-  // Chunk c of LDS row r lies at swizzle(r, c): 8 lanes that read one chunk
-  // of 8 rows touch different banks.
-  auto swizzle = [](int r, int c) {
-    return kChunks % 8 == 0 ? c ^ (r & 7) : c ^ ((r >> 2) & 3);
-  };
-  // of which a lane reads chunks g + 4 k of row r16 and of rows 16, 32, .. on:
-  // with groups of 8 chunks, at two places that alternate with k
-  const uint32_t at0 = r16 * kPitch + swizzle(r16, g) * 16;
-  const uint32_t at1 = kChunks % 8 == 0 ? at0 ^ 64 : at0 + 64;
+  // a lane reads chunks g + 4 k of row r16 and of rows 16, 32, .. on
+  const uint32_t at0 = r16 * kPitch + row_chunk(kPitch, r16, g) * 16;
+  constexpr int kGroup = kPitch % 256 == 0 ? 4 : kPitch % 128 == 0 ? 2 : 1;
   auto chunk = [&](const char* rows, int k) {
-    return *reinterpret_cast<const u32x4*>(rows + (k & 1 ? at1 : at0) + (k >> 1) * 128);
+    return *reinterpret_cast<const u32x4*>(rows + (at0 ^ (k % kGroup * 64)) +
+                                           k / kGroup * (kGroup * 64));
   };
   // the order of k within 64 columns: 8-bit fragments are 16 columns wide
   u32x4 fb[KS][NS];
@@ -557,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     for (int i = 0; i < kLoads; ++i) {
       const int p = lane + 64 * i;
       const int r = wave * (kRows / 4) + p / kChunks;
-      const int c = swizzle(r, p % kChunks);
+      const int c = row_chunk(kPitch, r, p % kChunks);
       if (c < last_chunk)
         load_lds16(base, (uint32_t)(min(r, last) * (int)a.w.ld + c * 16), to + i * 1024);
     }
@@ -699,12 +706,12 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
       if (q * 1024 < kBytesW) {
         const int p = q * 64 + lane;
         const int r = TW == kFP8 ? p >> 1 : p >> 2;
-        const int c = TW == kFP8 ? p & 1 : (p & 3) ^ ((r >> 2) & 3);
+        const int c = TW == kFP8 ? p & 1 : row_chunk(64, r, p & 3);
         load_lds16(bw, (uint32_t)(min(r, last_w) * (int)a.w.ld + min(c * 16, end_w)),
                    lds_address(&lds[buf][q * 1024]));
       } else if (q < kInstr) {
         const int p = (q - kBytesW / 1024) * 64 + lane;
-        const int r = p >> 2, c = (p & 3) ^ ((r >> 2) & 3);
+        const int r = p >> 2, c = row_chunk(64, r, p & 3);
         load_lds16(bh, (uint32_t)(min(r, last_h) * (int)a.h.ld + min(c * 16, end_h)),
                    lds_address(&lds[buf][q * 1024]));
       }
@@ -743,7 +750,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
     }
     const char* buf = lds[s & kAhead];
     const char* lh = buf + kBytesW + wn * (16 * NS) * kWideH;
-    const int at = r16 * 64 + ((g ^ (r16 >> 2)) << 4);
+    const int at = r16 * 64 + row_chunk(64, r16, g) * 16;
     u32x4 fa[MR], fb[NS];
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
@@ -1006,25 +1013,29 @@ __global__ __launch_bounds__(256) void pack_kernel(
   }
 }
 
-// 256 rows r and 32 ND columns d per workgroup of eight waves, 64 x 16 ND per
-// wave, so that narrow tables are read once and the coefficients, the larger
-// part, as often as there are tiles of d.  Steps of 64 bytes of k (32 of bf16,
-// 16 of float32) go straight into LDS, three steps ahead of the one at work.
-template <int T, int ND, bool DW>
+// Eight waves: WR times 16 J rows r, 8 / WR times 16 ND columns d.  With 256
+// rows and 32 ND columns narrow tables are read once and the coefficients, the
+// larger part, as often as there are tiles of d; fewer samples than that take
+// the forms with fewer rows.  Steps of 64 bytes of k (32 of bf16, 16 of
+// float32) go straight into LDS, kAhead steps ahead of the one at work: three,
+// or one where k is short and several workgroups a CU do more.
+template <int T, bool DW, int ND, int WR, int J, int kAhead>
 __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
-  constexpr int ES = Elem<T>::size;
-  constexpr int kRowsR = 256, kStep = 64 / ES, kAhead = 3;
-  constexpr int kPitchX = 32 * ND * ES, kPitchB = kRowsR * ES;   // bytes of a row k
+  constexpr int ES = Elem<T>::size, WD = 8 / WR;
+  constexpr int kRowsR = 16 * J * WR, kCols = 16 * ND * WD, kStep = 64 / ES;
+  constexpr int kPitchX = kCols * ES, kPitchB = kRowsR * ES;     // bytes of a row k
   constexpr int kChunksX = kPitchX / 16, kChunksB = kPitchB / 16;
   constexpr int kBytesX = kStep * kPitchX, kBytesB = kStep * kPitchB;
-  constexpr int kInstrX = kBytesX / 1024;            // loads of a whole wave
-  constexpr int kMoreX = kInstrX % 8;                // waves with one more
+  constexpr int kInstr = (kBytesX + kBytesB) / 1024;             // loads of a whole wave
+  constexpr int kEach = kInstr / 8, kMore = kInstr % 8;          // kMore waves have one more
   constexpr int kBlock = 256 * ES;                   // bytes of 16 x 16 coefficients
   constexpr int kLine = 16 * ES;                     // of which one sample's
+  static_assert(kBytesX % 1024 == 0 && kBytesB % 1024 == 0, "");
+  static_assert(!DW || (WR == 4 && J == 4), "");
   __shared__ __align__(16) char lds[kAhead + 1][kBytesX + kBytesB];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wd = wave & 1, wr = wave >> 1;
+  const int wd = wave % WD, wr = wave / WD;
   const int r16 = lane & 15, g = lane >> 4;
   // the parts of k go round the XCDs: the tiles of r that share rows of x are
   // in one XCD at a time
@@ -1037,7 +1048,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   int s0, s1;
   part_of((int)((a.k + kStep - 1) / kStep), split, a.splits, s0, s1);
   const int64_t r0 = (int64_t)tr * kRowsR;
-  const int d0 = td * 32 * ND;
+  const int d0 = td * kCols;
 
   // Blocks of 16 columns (of kLine bytes) of row k lie at block ^ key(k): the
   // rows that one transposing read touches spread over the banks.
@@ -1055,52 +1066,49 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   const int have_b = (int)min((int64_t)(DW ? kChunksB : kRowsR),
                               DW ? ((a.r - r0) * ES + 15) / 16 : a.r - r0);
   auto fetch = [&](int s) {
-    char* buf = lds[(s - s0) & kAhead];
+    char* buf = lds[(s - s0) % (kAhead + 1)];
     const int64_t k0 = (int64_t)s * kStep;
     const char* xb = a.x.p + k0 * a.x.ld + d0 * ES;
     const int last = (int)min((int64_t)kStep - 1, a.x.rows - 1 - k0);
 #pragma unroll
-    for (int i = 0; i < (kInstrX + 7) / 8; ++i) {
+    for (int i = 0; i < kEach + (kMore > 0); ++i) {
       const int q = wave + 8 * i;
-      if (q < kInstrX) {
+      if (q * 1024 < kBytesX) {
         const int p = q * 64 + lane;
         const int k = p / kChunksX, pos = p % kChunksX;
         const int c = ((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer;
         load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + min(c, have_x - 1) * 16),
                    lds_address(buf + q * 1024));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = wave + 8 * i;
-      const int p = q * 64 + lane;
-      if constexpr (DW) {
-        // samples k, chunk c of 256 table rows
-        const int k = p / kChunksB, pos = p % kChunksB;
-        const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
-        const int in = min(c, have_b - 1);
-        load_lds16(a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock,
-                   (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * kLine +
-                       in / kPer * kBlock + in % kPer * 16,
-                   lds_address(buf + kBytesX + q * 1024));
-      } else {
-        // 64 bytes of samples r: chunk c at c ^ ((r >> 2) & 3)
-        const int r = p >> 2;
-        const int c = (p & 3) ^ ((r >> 2) & 3);
-        const int in = min(r, have_b - 1);
-        load_lds16(a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock,
-                   (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * kLine +
-                       c / kPer * kBlock + c % kPer * 16,
-                   lds_address(buf + kBytesX + q * 1024));
+      } else if (q < kInstr) {
+        const int p = (q - kBytesX / 1024) * 64 + lane;
+        const char* from;
+        uint32_t offset;
+        if constexpr (DW) {
+          // samples k, chunk c of the table rows
+          const int k = p / kChunksB, pos = p % kChunksB;
+          const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
+          const int in = min(c, have_b - 1);
+          from = a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock;
+          offset = (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * kLine +
+                   in / kPer * kBlock + in % kPer * 16;
+        } else {
+          // 64 bytes of samples r
+          const int r = p >> 2, c = row_chunk(64, r, p & 3);
+          const int in = min(r, have_b - 1);
+          from = a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock;
+          offset = (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * kLine +
+                   c / kPer * kBlock + c % kPer * 16;
+        }
+        load_lds16(from, offset, lds_address(buf + q * 1024));
       }
     }
   };
 
-  f32x4 acc[ND][4];
+  f32x4 acc[ND][J];
 #pragma unroll
   for (int i = 0; i < ND; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < J; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
     if (s0 + i < s1) fetch(s0 + i);
@@ -1123,25 +1131,25 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
     }
   };
   for (int s = s0; s < s1; ++s) {
-    // step s has arrived, two more may be on their way
+    // step s has arrived, kAhead - 1 more may be on their way
     if (s + kAhead - 1 < s1) {
-      if (wave < kMoreX) wait_loads_but<(kAhead - 1) * (kInstrX / 8 + 1 + 2)>();
-      else wait_loads_but<(kAhead - 1) * (kInstrX / 8 + 2)>();
+      if (wave < kMore) wait_loads_but<(kAhead - 1) * (kEach + 1)>();
+      else wait_loads_but<(kAhead - 1) * kEach>();
     } else {
       wait_loads();
     }
     __syncthreads();
     if (s + kAhead < s1) fetch(s + kAhead);
-    const char* x = lds[(s - s0) & kAhead];
+    const char* x = lds[(s - s0) % (kAhead + 1)];
     const char* b = x + kBytesX;
-    u32x4 fb[4];
+    u32x4 fb[J];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < J; ++j) {
       if constexpr (DW) {
-        fb[j] = columns(b, kPitchB, wr * 4 + j);
+        fb[j] = columns(b, kPitchB, wr * J + j);
       } else {
-        const int r = wr * 64 + j * 16 + r16;
-        fb[j] = *reinterpret_cast<const u32x4*>(b + r * 64 + ((g ^ ((r >> 2) & 3)) << 4));
+        const int r = (wr * J + j) * 16 + r16;
+        fb[j] = *reinterpret_cast<const u32x4*>(b + r * 64 + row_chunk(64, r, g) * 16);
       }
     }
 #pragma unroll
@@ -1151,8 +1159,8 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t r = r0 + wr * 64 + j * 16 + r16;
+  for (int j = 0; j < J; ++j) {
+    const int64_t r = r0 + (wr * J + j) * 16 + r16;
     if (r >= a.r) continue;
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
@@ -1186,16 +1194,27 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   }
 }
 
-// dh from its parts.
-template <int T>
+// A result from its parts: G lanes of a workgroup share a result, so that many
+// parts of few results are added at the same time, in a fixed order.
+template <int T, int G>
 __global__ __launch_bounds__(256) void sum_parts_kernel(
     const float* part, int splits, int64_t rows, int64_t ldp, int d, char* out) {
+  constexpr int kEach = 256 / G;
+  __shared__ float sums[G][kEach];
+  const int at = threadIdx.x % kEach, group = threadIdx.x / kEach;
   const int64_t total = rows * d;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
+  const int64_t i = (int64_t)blockIdx.x * kEach + at;
+  float s = 0.f;
+  if (i < total) {
     const int64_t r = i / d, c = i - r * d;
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += part[((int64_t)p * rows + r) * ldp + c];
+#pragma unroll 4
+    for (int p = group; p < splits; p += G) s += part[((int64_t)p * rows + r) * ldp + c];
+  }
+  sums[group][at] = s;
+  __syncthreads();
+  if (group == 0 && i < total) {
+#pragma unroll
+    for (int k = 1; k < G; ++k) s += sums[k][at];
     if constexpr (T == kF32) reinterpret_cast<float*>(out)[i] = s;
     else reinterpret_cast<__bf16*>(out)[i] = (__bf16)s;
   }
@@ -1469,11 +1488,12 @@ static void launch_tile(ScoreArgs& a, hipStream_t stream) {
     if (r->align != 16 || r->ld >= (1 << 23)) throw std::runtime_error("rows not aligned");
   const int64_t rows = a.v_end - a.v_begin;
   if (a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
-  // 256 x 256 needs 256 of them to fill the card
+  // 128 x 128 fills the card more evenly; bf16 is bound by LDS there, and takes
+  // 256 x 256 where there are enough of them
   if constexpr (TW != kFP8)
-    if (((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
+    if (TC == kF32 || ((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
       return launch_tile_k<TW, TC, USE, 2, 2, 4>(a, stream);
-  launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
+  if constexpr (TC != kF32) launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
 }
 
 // LDS that the samples of the streaming kernel take; 4 KB at least, for the
@@ -1579,29 +1599,97 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
 
 static void launch_sum_parts(const float* part, int splits, int64_t rows, int64_t ldp, int64_t d,
                              int is_bf16, char* out, hipStream_t stream) {
-  const int blocks = (int)std::min<int64_t>((rows * d + 255) / 256, 4096);
-  if (is_bf16) sum_parts_kernel<kBF16><<<blocks, 256, 0, stream>>>(part, splits, rows, ldp, (int)d, out);
-  else sum_parts_kernel<kF32><<<blocks, 256, 0, stream>>>(part, splits, rows, ldp, (int)d, out);
+  auto go = [&](auto kernel, int each) {
+    kernel<<<grid_of((rows * d + each - 1) / each), 256, 0, stream>>>(part, splits, rows, ldp,
+                                                                     (int)d, out);
+  };
+  if (splits >= 16)
+    is_bf16 ? go(sum_parts_kernel<kBF16, 16>, 16) : go(sum_parts_kernel<kF32, 16>, 16);
+  else
+    is_bf16 ? go(sum_parts_kernel<kBF16, 4>, 64) : go(sum_parts_kernel<kF32, 4>, 64);
 }
 
-// Tiles of 32 ND columns that cover d with the fewest wasted.
-static void wide_tiles(int d, int& nd, int& tiles) {
-  tiles = (d + 319) / 320;
-  nd = ((d + tiles - 1) / tiles + 63) / 64 * 2;
+// The form of grad_kernel for a result of r x d with k terms.
+struct GradForm {
+  int rows;       // of a workgroup; 0: the form for a short k, of 256 rows
+  int nd;         // 16 columns times this per wave
+  int tiles_d;
+  int slots;      // workgroups that the card holds at a time
+};
+
+static GradForm grad_form(bool bf16, bool dw, int64_t r, int64_t k, int d) {
+  GradForm f{256, 0, 0, 256};
+  int wd = 2, most = 10, step = 2;    // waves along d, blocks of 16 columns a wave
+  if (!dw && r <= 32) f.rows = 32, wd = 8, most = 3, step = 1, f.slots = 512;
+  else if (!dw && r <= 128) f.rows = 128, wd = 4, most = 5, step = 1, f.slots = 512;
+  else if (dw && k <= 128) f.rows = 0, most = 4, f.slots = 768;
+  if (f.rows == 0 || (f.rows == 256 && bf16)) {
+    // bound by LDS or by what is written: the fewest tiles
+    f.tiles_d = (d + 16 * wd * most - 1) / (16 * wd * most);
+    f.nd = ((d + f.tiles_d - 1) / f.tiles_d + 63) / 64 * 2;
+    if (f.rows == 0 && f.nd > 2) f.nd = 4;
+    return f;
+  }
+  // the fewest columns past d, and of those the most tiles, which fill the
+  // card more evenly; but no narrow ones where wide ones do
+  int least = INT32_MAX;
+  for (int n = most; n >= step; n -= step) {
+    const int t = (d + 16 * n * wd - 1) / (16 * n * wd);
+    if (t * n < least || (t * n == least && n > 2)) least = t * n, f.nd = n, f.tiles_d = t;
+  }
+  return f;
+}
+
+// Parts of k for `tiles` results on `slots` places: the fewest that fill nine
+// tenths of what any number up to `most` fills.
+static int grad_parts(int64_t tiles, int slots, int64_t most) {
+  if (tiles >= 2 * slots) return 1;
+  most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 512),
+                                                (2 * slots + tiles - 1) / tiles));
+  auto full = [&](int64_t s) {
+    return (double)(tiles * s) / (double)((tiles * s + slots - 1) / slots * slots);
+  };
+  double best = 0;
+  for (int64_t s = 1; s <= most; ++s) best = std::max(best, full(s));
+  int64_t s = 1;
+  while (full(s) < 0.9 * best) ++s;
+  return (int)s;
+}
+
+// (parts of the vocabulary's pieces for dh, parts of the samples for dw)
+static std::pair<int, int> softmax_plan(int64_t n, int64_t chunk, int64_t d, int is_bf16) {
+  const GradForm h = grad_form(is_bf16, false, n, chunk, (int)d);
+  const GradForm w = grad_form(is_bf16, true, chunk, n, (int)d);
+  const int rows_w = w.rows ? w.rows : 256;
+  return {grad_parts((n + h.rows - 1) / h.rows * h.tiles_d, h.slots, (chunk + 63) / 64),
+          grad_parts((chunk + rows_w - 1) / rows_w * w.tiles_d, w.slots, (n + 127) / 128)};
+}
+
+template <int T, bool DW, int ND, int WR, int J, int kAhead>
+static void launch_grad_k(GradArgs& b, hipStream_t stream) {
+  b.tiles_r = grid_of((b.r + 16 * J * WR - 1) / (16 * J * WR));
+  const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
+  const int blocks = grid_of(b.splits >= 8 ? tiles * ((b.splits + 7) / 8) * 8 : tiles * b.splits);
+  grad_kernel<T, DW, ND, WR, J, kAhead><<<blocks, 512, 0, stream>>>(b);
 }
 
 template <int T, bool DW>
 static void launch_grad(GradArgs b, hipStream_t stream) {
-  int nd;
-  wide_tiles(b.d, nd, b.tiles_d);
-  b.tiles_r = grid_of((b.r + 255) / 256);
-  const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
-  const int blocks = grid_of(b.splits >= 8 ? tiles * ((b.splits + 7) / 8) * 8 : tiles * b.splits);
-  if (nd == 2) grad_kernel<T, 2, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 4) grad_kernel<T, 4, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 6) grad_kernel<T, 6, DW><<<blocks, 512, 0, stream>>>(b);
-  else if (nd == 8) grad_kernel<T, 8, DW><<<blocks, 512, 0, stream>>>(b);
-  else grad_kernel<T, 10, DW><<<blocks, 512, 0, stream>>>(b);
+  const GradForm f = grad_form(T == kBF16, DW, b.r, b.k, b.d);
+  b.tiles_d = f.tiles_d;
+#define CASE_ND(R, N, WR, J, A) \
+  if (f.rows == R && f.nd == N) return launch_grad_k<T, DW, N, WR, J, A>(b, stream);
+  if constexpr (DW) {
+    CASE_ND(0, 2, 4, 4, 1) CASE_ND(0, 4, 4, 4, 1)
+  } else {
+    CASE_ND(32, 1, 1, 2, 3) CASE_ND(32, 2, 1, 2, 3) CASE_ND(32, 3, 1, 2, 3)
+    CASE_ND(128, 1, 2, 4, 3) CASE_ND(128, 2, 2, 4, 3) CASE_ND(128, 3, 2, 4, 3)
+    CASE_ND(128, 4, 2, 4, 3) CASE_ND(128, 5, 2, 4, 3)
+  }
+  CASE_ND(256, 2, 4, 4, 3) CASE_ND(256, 4, 4, 4, 3) CASE_ND(256, 6, 4, 4, 3)
+  CASE_ND(256, 8, 4, 4, 3) CASE_ND(256, 10, 4, 4, 3)
+#undef CASE_ND
+  throw std::runtime_error("no kernel for these columns");
 }
 
 // packed: [np][dp] elements with np = n rounded up to 32, dp = d rounded up to
@@ -1778,6 +1866,7 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
 PYBIND11_MODULE(_vocab_native, m) {
   m.doc() = "MI355X (gfx950) kernels over the whole vocabulary";
   m.def("softmax_loss", &softmax_loss);
+  m.def("softmax_plan", &softmax_plan);
   m.def("softmax_grad", &softmax_grad);
   m.def("quantize_rows", &quantize_rows);
   m.def("dequantize_rows", &dequantize_rows);

@@ -95,17 +95,6 @@ def _aligned(t: torch.Tensor) -> bool:
     return t.data_ptr() % 16 == 0 and step % 16 == 0 and step < 1 << 23
 
 
-def _parts(tiles: int, slots: int, most: int) -> int:
-    """Parts of a product's long axis for `tiles` results on `slots` places:
-    the fewest that fill nine tenths of what any number up to `most` fills."""
-    if tiles >= 2 * slots:
-        return 1
-    most = max(1, min(most, _ceil(2 * slots, tiles), 64))
-    full = [tiles * s / (_ceil(tiles * s, slots) * slots)
-            for s in range(1, most + 1)]
-    return next(i for i, f in enumerate(full, 1) if f >= 0.9 * max(full))
-
-
 def _forward(h, w, targets, ignore_index, reduce: int):
     """(loss [N], lse [N], [reduced loss, factor] or None)."""
     _check(h, w, targets)
@@ -165,10 +154,9 @@ def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
         torch.empty(width * _ceil(d, 64) * 64, dtype=w.dtype, device=w.device)
     ldp = _ceil(d, 4) * 4
     # parts of the long axis where a product's result has few tiles
-    splits = _parts(_ceil(n, 256) * _ceil(d, 320), 256,
-                    _ceil(width, 64)) if need_h else 1
-    splits_w = _parts(_ceil(min(v, width), 256) * _ceil(d, 320), 256,
-                      _ceil(n, 64)) if need_w else 1
+    splits, splits_w = _native().softmax_plan(n, min(v, width), d,
+                                              int(size == 2))
+    splits_w = splits_w if need_w else 1
     part = torch.empty(splits * n * ldp if need_h else 0,
                        dtype=torch.float32, device=h.device)
     part_w = torch.empty(splits_w * width * ldp if splits_w > 1 else 0,
