@@ -226,6 +226,7 @@ __device__ __forceinline__ int64_t target_of(const void* t, int is64, int64_t n)
 template <int USE, int TC, int NS>
 struct Sink {
   float top[NS], sum[NS];                      // kLoss
+  bool far;                                    // of the wave: past kFar
   float lse2[NS], gg[NS];                      // kCoef; lse in powers of two
   int yy[NS];                                  // -1: no loss
 
@@ -233,6 +234,7 @@ struct Sink {
     if constexpr (USE == kLoss) {
 #pragma unroll
       for (int j = 0; j < NS; ++j) top[j] = -INFINITY, sum[j] = 0.f;
+      far = false;
     }
     if constexpr (USE == kCoef) {
       const float wt = a.weight ? *a.weight : 1.f;
@@ -249,79 +251,120 @@ struct Sink {
           }
         }
       }
+      bool f = false;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) f |= fabsf(lse2[j]) > kFar;
+      far = __any(f);
     }
   }
 
+  // kCoef: whether the wave has targets among `rows` table rows from v on.
+  __device__ __forceinline__ bool meets(int v, int rows) const {
+    bool m = false;
+    if constexpr (USE == kCoef) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) m |= (unsigned)(yy[j] - v) < (unsigned)rows;
+      m = __any(m);
+    }
+    return m;
+  }
+
+  // `cut`: some of the rows may lie past the last one; `met`: what meets()
+  // says; both are the same for all lanes.
   template <int MR>
   __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                       int64_t n, const f32x4 (&scale)[MR]) {
-    if constexpr (USE == kLoss) take_loss(a, acc, v);
-    if constexpr (USE == kCoef) take_coef(a, acc, v, n);
+                                       int64_t n, bool cut, bool met, const f32x4 (&scale)[MR]) {
+    if constexpr (USE == kLoss) take_loss(a, acc, v, cut);
+    if constexpr (USE == kCoef) take_coef(a, acc, v, n, cut, met);
     if constexpr (USE == kStore) take_store(a, acc, v, n, scale);
   }
 
   template <int MR>
-  __device__ __forceinline__ void take_loss(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v) {
-    if (__any(v + 16 * (MR - 1) + 4 > a.v_end)) {
+  __device__ __forceinline__ void take_loss(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
+                                            bool cut) {
+    if (cut) {
 #pragma unroll
       for (int i = 0; i < MR; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (v + i * 16 + e >= a.v_end) {
 #pragma unroll
-            for (int j = 0; j < NS; ++j) acc[i][j][e] = -INFINITY;
-          }
+          for (int j = 0; j < NS; ++j)
+            acc[i][j][e] = v + i * 16 + e < a.v_end ? acc[i][j][e] : -INFINITY;
     }
+    float most[NS];
+    bool above = false;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      float most = acc[0][j][0];
+      most[j] = acc[0][j][0];
 #pragma unroll
       for (int i = 0; i < MR; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = fmaxf(most, acc[i][j][e]);
-      // The reference moves only when a score is above it, which gets rare.
-      if (__any(most > top[j])) {
-        const float next = fmaxf(top[j], most);
+        for (int e = 0; e < 4; ++e) most[j] = fmaxf(most[j], acc[i][j][e]);
+      above |= most[j] > top[j];
+    }
+    // The reference moves only when a score is above it, which gets rare.
+    if (__any(above)) {
+      bool f = false;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const float next = fmaxf(top[j], most[j]);
         sum[j] *= top[j] == -INFINITY ? 0.f : exp_of(top[j] - next);
         top[j] = next;
+        f |= fabsf(next) > kFar && next != -INFINITY;
       }
-      // nothing but -inf so far: any finite reference will do
-      const float at0 = top[j] == -INFINITY ? 0.f : top[j];
-      // the new terms are added to each other first: one rounding of the long
-      // sum for all of them
-      float s = 0.f;
-      if (__any(fabsf(at0) > kFar)) {
+      far = __any(f);
+    }
+    // the new terms are added to each other first: one rounding of the long
+    // sum for all of them
+    if (far) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const float at0 = top[j] == -INFINITY ? 0.f : top[j];
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < MR; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s += exp_of(acc[i][j][e] - at0);
-      } else {
-        const float ref = at0 * kLog2e;
+        sum[j] += s;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        // nothing but -inf so far: any finite reference will do
+        const float ref = top[j] == -INFINITY ? 0.f : top[j] * kLog2e;
+        float s = 0.f;
 #pragma unroll
         for (int i = 0; i < MR; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -ref));
+        sum[j] += s;
       }
-      sum[j] += s;
     }
   }
 
   template <int MR>
   __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                            int64_t n0) {
+                                            int64_t n0, bool cut, bool met) {
     // the first of the wave's samples and rows, the same in all lanes
     const int64_t n1 = __builtin_amdgcn_readfirstlane((int)(n0 - (threadIdx.x & 15)));
     const int v1 = __builtin_amdgcn_readfirstlane(v - a.v_begin);
     const int lane = threadIdx.x & 63;
+    // 16 samples x 16 table rows are 512 bytes (1 KB) in one piece, as a wave
+    // writes them and with every 16 bytes of one sample, as the products read
+    // them
+    constexpr int es = TC == kF32 ? 4 : 2;
+    const int in_block = (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
+    auto put = [&](int i, int j, f32x4 c) {
+      char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es) + in_block;
+      if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
+      else *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+    };
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      const int64_t n = n0 + j * 16;
-      if (n >= a.coef_rows) continue;
-      const bool far = __any(fabsf(lse2[j]) > kFar);
+      if (n1 + j * 16 >= a.coef_rows) break;
 #pragma unroll
       for (int i = 0; i < MR; ++i) {
-        const int vi = v + i * 16;
         f32x4 c = acc[i][j];
         if (far) {
           // the logarithm's own rounding may pass 0 here
@@ -333,26 +376,19 @@ struct Sink {
           for (int e = 0; e < 4; ++e)
             c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], kLog2e, -lse2[j]));
         }
-        const int right = yy[j] - vi;
-        if (__any((unsigned)right < 4u)) {
+        const int first = v + i * 16;
+        if (met) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] -= right == e ? 1.f : 0.f;
+          for (int e = 0; e < 4; ++e) c[e] -= first + e == yy[j] ? 1.f : 0.f;
         }
-        c *= gg[j];      // 0 without a loss: the row of h is zeros then
-        if (__any(vi + 4 > a.v_end)) {
+        c *= gg[j];      // 0 without a loss: h is zeros there
+        if (cut) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (vi + e >= a.v_end) c[e] = 0.f;
+          for (int e = 0; e < 4; ++e) c[e] = first + e < a.v_end ? c[e] : 0.f;
         }
-        // 16 samples x 16 table rows are 512 bytes (1 KB) in one piece, as a
-        // wave writes them and with every 16 bytes of one sample, as the
-        // products read them
-        constexpr int es = TC == kF32 ? 4 : 2;
-        char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es) +
-                   (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
-        if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
-        else
-          *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
+        put(i, j, c);
+        // one after the other: side by side they would not fit the registers
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -486,8 +522,8 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 
-// Rows of up to 32 KS columns of bf16 (or of 8 bits, on the table's side)
-// that start at multiples of 16 bytes.  A wave holds its 16 NS samples in
+// Rows of up to 32 KS columns of bf16 (or of 8 bits, on the table's side),
+// which on both sides start at multiples of 16 bytes.  A wave holds its 16 NS samples in
 // registers for the whole launch, so that LDS is read for the table alone:
 // one fragment of 16 table rows feeds NS instructions.  Table tiles of kRows
 // rows are loaded straight into LDS, one ahead of the tile at work; two
@@ -530,11 +566,19 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   // the order of k within 64 columns: 8-bit fragments are 16 columns wide
   u32x4 fb[KS][NS];
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+  for (int j = 0; j < NS; ++j) {
+    const char* row = a.h.p + min(n + j * 16, a.h.rows - 1) * a.h.ld;
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
-      fb[k][j] = load16<2>(a.h, n + j * 16,
-                           FP8 ? (k >> 1) * 128 + g * 32 + (k & 1) * 16 : k * 64 + g * 16);
+    for (int k = 0; k < KS; ++k) {
+      const int o = FP8 ? (k >> 1) * 128 + g * 32 + (k & 1) * 16 : k * 64 + g * 16;
+      fb[k][j] = *reinterpret_cast<const u32x4*>(row + min(o, (a.h.kb - 1) & ~15));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int have = a.h.kb - o - 4 * q;
+        fb[k][j][q] &= have >= 4 ? 0xffffffffu : have <= 0 ? 0u : 0xffffu;
+      }
+    }
+  }
   // what lies behind the last column of a table row is cut off here
   u32x4 keep[2];
   if constexpr (!FP8) {
@@ -560,9 +604,13 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     const char* base = a.w.p + v0 * a.w.ld;
     const int last = min(kRows - 1, (int)a.w.rows - 1 - v0);
     const uint32_t to = lds_address(&lds[buf][wave * (kRows / 4) * kPitch]);
+    // the places are worked out anew for every tile: kept, they would take the
+    // registers that the samples need
+    int from = lane;
+    asm volatile("" : "+v"(from));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int p = lane + 64 * i;
+      const int p = from + 64 * i;
       const int r = wave * (kRows / 4) + p / kChunks;
       const int c = row_chunk(kPitch, r, p % kChunks);
       if (c < last_chunk)
@@ -608,49 +656,60 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     else wait_loads();
     __syncthreads();
     if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
-    const int v0 = a.v_begin + tile * kRows + 4 * g;
+    const int v0 = a.v_begin + tile * kRows;
+    const bool cut = v0 + kRows > a.v_end, met = sink.meets(v0, kRows);
+    // Fragments are read kLead steps before they are used, those of the next
+    // rows' first steps before these rows' scores are.
+    constexpr int kReads = FP8 ? KS / 2 : KS, kLead = kReads < 4 ? kReads : 4;
+    constexpr int kGroups = kRows / (16 * MR * WV);
+    u32x4 fa[kLead][MR];
+    auto read = [&](int m, int k) {
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+        fa[k % kLead][i] = chunk(&lds[buf][((m * WV + wv) * MR + i) * 16 * kPitch], k);
+    };
+#pragma unroll
+    for (int k = 0; k < kLead; ++k) read(0, k);
 #pragma unroll 1
-    for (int m = 0; m < kRows / (16 * MR * WV); ++m) {
+    for (int m = 0; m < kGroups; ++m) {
       const int row0 = (m * WV + wv) * 16 * MR;
       f32x4 acc[MR][NS];
 #pragma unroll
       for (int i = 0; i < MR; ++i)
 #pragma unroll
         for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (!FP8) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          u32x4 fa[MR];
+      for (int k = 0; k < kReads; ++k) {
+        u32x4 (&f)[MR] = fa[k % kLead];
+        if constexpr (!FP8) {
+          if (k >= KS - 2)
 #pragma unroll
-          for (int i = 0; i < MR; ++i) {
-            fa[i] = chunk(&lds[buf][(row0 + i * 16) * kPitch], k);
-            if (k >= KS - 2) fa[i] &= keep[k - (KS - 2)];
-          }
-          mma_all<kBF16>(fa, fb[k], acc);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < KS; k += 2) {
+            for (int i = 0; i < MR; ++i) f[i] &= keep[k - (KS - 2)];
+          mma_all<kBF16>(f, fb[k], acc);
+        } else {
 #pragma unroll
           for (int i = 0; i < MR; ++i) {
-            const int r = row0 + i * 16 + r16;
-            u32x4 q = chunk(&lds[buf][(row0 + i * 16) * kPitch], k / 2);
-            if (k >= KS - 2) q &= keep[0];
-            const float s = scales[buf][r * kBlocks + k / 4];
+            if (k == kReads - 1) f[i] &= keep[0];
+            const float s = scales[buf][(row0 + i * 16 + r16) * kBlocks + k / 2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const u32x4 fa = fp8x8_to_bf16(q[2 * half], q[2 * half + 1], s);
-              mma_row<kBF16>(fa, fb[k + half], acc[i]);
-            }
+            for (int half = 0; half < 2; ++half)
+              mma_row<kBF16>(fp8x8_to_bf16(f[i][2 * half], f[i][2 * half + 1], s),
+                             fb[2 * k + half], acc[i]);
           }
         }
+        if (k + kLead < kReads) read(m, k + kLead);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      if (m + 1 < kGroups)
+#pragma unroll
+        for (int k = 0; k < kLead; ++k) read(m + 1, k);
+      __builtin_amdgcn_sched_barrier(0);
       f32x4 cs[MR] = {};
       if constexpr (USE == kStore)
 #pragma unroll
         for (int i = 0; i < MR; ++i)
           cs[i] = *reinterpret_cast<const f32x4*>(&col[buf][row0 + i * 16 + 4 * g]);
-      sink.template take<MR>(a, acc, v0 + row0, n, cs);
+      sink.template take<MR>(a, acc, v0 + row0 + 4 * g, n, cut, met, cs);
     }
     put_scales(buf ^ 1);
   }
@@ -787,7 +846,8 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
         for (int i = 0; i < MR; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) cs[i][e] = col_scale_of(a, v + i * 16 + e);
-      sink.template take<MR>(a, acc, v, n, cs);
+      const int v0 = a.v_begin + tile * kV + wv * 64;
+      sink.template take<MR>(a, acc, v, n, v0 + 64 > a.v_end, sink.meets(v0, 64), cs);
       step = 0;
       ++tile;
     }
@@ -897,7 +957,7 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
         }
       }
     }
-    sink.template take<1>(a, acc, v, n, cs);
+    sink.template take<1>(a, acc, v, n, v_first + group * 64 + 16 > a.v_end, false, cs);
   }
   if constexpr (USE == kLoss) sink.template finish_loss<4>(a, samples, split, n0);
 }
@@ -1445,7 +1505,7 @@ constexpr int kMostResident = 10;
 // Whether the kernel with resident samples takes these rows.  Its offsets
 // within a tile have 32 bits.
 static bool is_resident(const ScoreArgs& a, int64_t cols) {
-  return cols <= 32 * kMostResident && a.w.align == 16 && a.w.ld < (1 << 23);
+  return cols <= 32 * kMostResident && a.w.align == 16 && a.h.align == 16 && a.w.ld < (1 << 23);
 }
 
 template <int KS, int NS, int WN, int USE, bool FP8>

@@ -24,7 +24,7 @@ import torch
 
 # Pieces of the vocabulary are as wide as keeps their coefficients within
 # this, and packed copies of unaligned tables within that.
-_COEF_BYTES = 512 << 20
+_COEF_BYTES = 1 << 30
 _PACKED_BYTES = 256 << 20
 _PARTS = 4096
 
@@ -108,13 +108,13 @@ def _forward(h, w, targets, ignore_index, reduce: int):
     size, dp = h.element_size(), _ceil(d, 64) * 64
     packed_h = packed_w = None
     piece = v
-    if not (n <= 16 and d * size <= 4096):    # the streaming kernel takes any
-        if not _aligned(h):
-            packed_h = torch.empty(n * dp, dtype=h.dtype, device=h.device)
-        if not _aligned(w):
-            piece = max(256, _PACKED_BYTES // (dp * size) // 256 * 256)
-            packed_w = torch.empty(min(piece, v) * dp, dtype=w.dtype,
-                                   device=w.device)
+    if not _aligned(h):
+        packed_h = torch.empty(n * dp, dtype=h.dtype, device=h.device)
+    # (the kernel for few rows streams any table)
+    if not _aligned(w) and not (n <= 16 and d * size <= 4096):
+        piece = max(256, _PACKED_BYTES // (dp * size) // 256 * 256)
+        packed_w = torch.empty(min(piece, v) * dp, dtype=w.dtype,
+                               device=w.device)
     # a maximum and a sum of every row for each part of the vocabulary
     parts = max(_ceil(v, piece), min(_ceil(v, 64),
                                      _PARTS // max(1, _ceil(n, 128))))
