@@ -530,20 +530,34 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // workgroups fit a CU, and one's exponentials run beside the other's
 // products.  WN of the four waves have different samples, the others share
 // them and take different rows of the tile.
+constexpr int resident_rows(int ks, int use, int wn, bool fp8) {
+  // with stores, tiles of at most 20 KB: four of them fit, so that the stores
+  // of several tiles, which are waited for in order with the loads, may be on
+  // their way; without, larger tiles have fewer barriers
+  const int most = use == kLoss ? 40960 : 20480, pitch = ks * (fp8 ? 32 : 64);
+  const int rows = 128 * pitch <= most ? 128 : 64 * pitch <= most ? 64 : 32;
+  return rows < 64 && wn == 1 ? 64 : rows;
+}
+
 template <int KS, int NS, int WN, int USE, bool FP8>
 __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   constexpr int WV = 4 / WN;
-  constexpr int kRows = KS <= 4 ? 128 : KS <= 10 ? 64 : 32;
+  constexpr int kRows = resident_rows(KS, USE, WN, FP8);
   constexpr int kPitch = KS * (FP8 ? 32 : 64);       // bytes of a row in LDS
   constexpr int kChunks = kPitch / 16;
+  // two workgroups share 160 KB
+  constexpr int kEach = kRows * kPitch + (FP8 ? 256 : 0) + (USE == kStore ? kRows * 4 : 0);
+  constexpr int kBufs = kEach * 4 + 64 <= 81920 + (USE == kStore ? 0 : 64) ? 4 : kEach * 3 <= 81920 ? 3 : 2;
+  constexpr int kAhead = kBufs - 1;
   constexpr int kLoads = kRows / 4 * kChunks / 64;   // per lane and tile
   constexpr int MR = kRows / WV >= 32 && KS * NS <= 24 ? 2 : 1;
   constexpr int kBlocks = (KS + 3) / 4;              // scales of a row
   constexpr int kScales = kRows * kBlocks;
   static_assert(kRows / 4 * kChunks % 64 == 0 && kRows % (16 * MR * WV) == 0, "");
-  __shared__ __align__(16) char lds[2][kRows * kPitch];
-  __shared__ float scales[FP8 ? 2 : 1][FP8 ? kScales : 1];
-  __shared__ __align__(16) float col[2][USE == kStore ? kRows : 4];
+  __shared__ __align__(16) char lds[kBufs][kRows * kPitch];
+  __shared__ __align__(16) uint8_t scales[FP8 ? kBufs : 1][256];
+  __shared__ __align__(16) float col[USE == kStore ? kBufs : 1][kRows];
+  static_assert(!FP8 || kScales <= 256, "");
   // stores of a wave for one whole tile
   constexpr int kStores = USE == kLoss ? 0 : kRows / (16 * WV) * NS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -597,65 +611,58 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     }
   }
 
-  const int last_chunk = (a.w.kb + 15) / 16;
-  float next_scale[(kScales + 255) / 256], next_col = 1.f;
-  auto fetch = [&](int tile, int buf) {
-    const int v0 = a.v_begin + tile * kRows;
+  // What lies outside is replaced by what is inside, and no lane sits out: the
+  // waits below count the loads of each wave.
+  const int last_chunk = (a.w.kb - 1) / 16;
+  auto fetch = [&](int tile) {
+    const int v0 = a.v_begin + tile * kRows, buf = (tile - t0) % kBufs;
     const char* base = a.w.p + v0 * a.w.ld;
     const int last = min(kRows - 1, (int)a.w.rows - 1 - v0);
-    const uint32_t to = lds_address(&lds[buf][wave * (kRows / 4) * kPitch]);
     // the places are worked out anew for every tile: kept, they would take the
     // registers that the samples need
     int from = lane;
     asm volatile("" : "+v"(from));
+    // all waves load the same few scales: not counted, as the rows come after
+    if constexpr (FP8)
+      load_lds4((const char*)a.w.scales + (int64_t)v0 * kBlocks,
+                (uint32_t)min(from * 4, ((last + 1) * kBlocks - 1) & ~3),
+                lds_address(scales[buf]));
+    if constexpr (USE == kStore)
+      if (a.col_scale)
+#pragma unroll
+        for (int i = 0; i < kRows; i += 64)
+          if (kRows >= 64)
+            load_lds4((const char*)(a.col_scale + v0), (uint32_t)min(from + i, last) * 4,
+                      lds_address(&col[buf][i]));
+    const uint32_t to = lds_address(&lds[buf][wave * (kRows / 4) * kPitch]);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int p = from + 64 * i;
       const int r = wave * (kRows / 4) + p / kChunks;
       const int c = row_chunk(kPitch, r, p % kChunks);
-      if (c < last_chunk)
-        load_lds16(base, (uint32_t)(min(r, last) * (int)a.w.ld + c * 16), to + i * 1024);
-    }
-    if constexpr (USE == kStore)
-      if (threadIdx.x < kRows) next_col = col_scale_of(a, v0 + (int)threadIdx.x);
-    if constexpr (FP8) {
-#pragma unroll
-      for (int i = 0; i < (kScales + 255) / 256; ++i) {
-        const int p = threadIdx.x + 256 * i;
-        next_scale[i] = 0.f;
-        const int r = p / kBlocks, b = p % kBlocks;
-        if (p < kScales && v0 + r < a.w.rows && b * 128 < a.w.kb)
-          next_scale[i] = scale_of(a.w.scales[(v0 + r) * a.w.lds + b]);
-      }
+      load_lds16(base, (uint32_t)(min(r, last) * (int)a.w.ld + min(c, last_chunk) * 16),
+                 to + i * 1024);
     }
   };
-  auto put_scales = [&](int buf) {
-    if constexpr (USE == kStore)
-      if (threadIdx.x < kRows) col[buf][threadIdx.x] = next_col;
-    if constexpr (FP8) {
-#pragma unroll
-      for (int i = 0; i < (kScales + 255) / 256; ++i)
-        if (threadIdx.x + 256 * i < kScales) scales[buf][threadIdx.x + 256 * i] = next_scale[i];
-    }
-  };
+  static_assert(USE != kStore || kRows >= 64, "");
 
   Sink<USE, kBF16, NS> sink;
   sink.start(a, n);
-  if (t0 < t1) {
-    fetch(t0, 0);
-    put_scales(0);
-  }
-  // Whether the wave makes all of kStores: then the last tile's stores, which
-  // come after this tile's loads, need not be waited for.
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (t0 + i < t1) fetch(t0 + i);
+  // Whether the wave makes all of kStores for every tile but the last: then
+  // those made since this tile's loads need not be waited for.
   const bool whole = n0 + (wn + 1) * (16 * NS) <= a.n && (USE != kStore || (a.ldo & 3) == 0);
+  constexpr int kLater = (kAhead - 1) * kLoads, kMost = kLater + kAhead * kStores;
   for (int tile = t0; tile < t1; ++tile) {
-    const int buf = (tile - t0) & 1;
-    // the tile has arrived for all waves, and all are done with the other one
-    // (only the last tile of all may be cut short)
-    if (kStores > 0 && kStores < 64 && whole && tile > t0) wait_loads_but<kStores & 63>();
-    else wait_loads();
+    const int buf = (tile - t0) % kBufs;
+    // the tile has arrived for all waves, and all are done with the one before
+    if (tile + kAhead - 1 >= t1) wait_loads();
+    else if (kStores > 0 && whole && tile >= t0 + kAhead) wait_loads_but<(kMost < 63 ? kMost : 63)>();
+    else wait_loads_but<kLater>();
     __syncthreads();
-    if (tile + 1 < t1) fetch(tile + 1, buf ^ 1);
+    if (tile + kAhead < t1) fetch(tile + kAhead);
     const int v0 = a.v_begin + tile * kRows;
     const bool cut = v0 + kRows > a.v_end, met = sink.meets(v0, kRows);
     // Fragments are read kLead steps before they are used, those of the next
@@ -690,7 +697,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 #pragma unroll
           for (int i = 0; i < MR; ++i) {
             if (k == kReads - 1) f[i] &= keep[0];
-            const float s = scales[buf][(row0 + i * 16 + r16) * kBlocks + k / 2];
+            const float s = scale_of(scales[buf][(row0 + i * 16 + r16) * kBlocks + k / 2]);
 #pragma unroll
             for (int half = 0; half < 2; ++half)
               mma_row<kBF16>(fp8x8_to_bf16(f[i][2 * half], f[i][2 * half + 1], s),
@@ -704,14 +711,14 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 #pragma unroll
         for (int k = 0; k < kLead; ++k) read(m + 1, k);
       __builtin_amdgcn_sched_barrier(0);
-      f32x4 cs[MR] = {};
-      if constexpr (USE == kStore)
+      f32x4 cs[MR];
 #pragma unroll
-        for (int i = 0; i < MR; ++i)
-          cs[i] = *reinterpret_cast<const f32x4*>(&col[buf][row0 + i * 16 + 4 * g]);
+      for (int i = 0; i < MR; ++i)
+        cs[i] = USE == kStore && a.col_scale
+                    ? *reinterpret_cast<const f32x4*>(&col[buf][(row0 + i * 16 + 4 * g) % kRows])
+                    : f32x4{1.f, 1.f, 1.f, 1.f};
       sink.template take<MR>(a, acc, v0 + row0 + 4 * g, n, cut, met, cs);
     }
-    put_scales(buf ^ 1);
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV>(a, lds[0], split, n0);
 }
@@ -1513,7 +1520,7 @@ static void launch_resident_k(ScoreArgs& a, hipStream_t stream) {
   constexpr auto kernel = resident_kernel<KS, NS, WN, USE, FP8>;
   static const int slots = slots_of(kernel, 256, 0);
   a.tiles_n = grid_of((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
-  cut(a, KS <= 4 ? 128 : 64, slots);
+  cut(a, resident_rows(KS, USE, WN, FP8), slots);
   kernel<<<score_grid(a), 256, 0, stream>>>(a);
 }
 
@@ -1721,8 +1728,11 @@ static std::pair<int, int> softmax_plan(int64_t n, int64_t chunk, int64_t d, int
   const GradForm h = grad_form(is_bf16, false, n, chunk, (int)d);
   const GradForm w = grad_form(is_bf16, true, chunk, n, (int)d);
   const int rows_w = w.rows ? w.rows : 256;
-  return {grad_parts((n + h.rows - 1) / h.rows * h.tiles_d, h.slots, (chunk + 63) / 64),
-          grad_parts((chunk + rows_w - 1) / rows_w * w.tiles_d, w.slots, (n + 127) / 128)};
+  const int64_t tiles_h = (n + h.rows - 1) / h.rows * h.tiles_d;
+  const int64_t tiles_w = (chunk + rows_w - 1) / rows_w * w.tiles_d;
+  // parts of dw are as large as dw: only where half of the card would idle
+  return {grad_parts(tiles_h, h.slots, (chunk + 63) / 64),
+          2 * tiles_w <= w.slots ? grad_parts(tiles_w, w.slots, (n + 255) / 256) : 1};
 }
 
 template <int T, bool DW, int ND, int WR, int J, int kAhead>

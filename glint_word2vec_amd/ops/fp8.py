@@ -154,7 +154,9 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
                                f"{b.device}")
         col_scale = col_scale.detach().contiguous()
     out = torch.empty((m, n), dtype=out_dtype, device=b.device)
-    values, scales = b
+    values, scales = b.values, b.scales.contiguous()
+    if scales.data_ptr() % 4:
+        scales = scales.clone()
     if not _aligned(values):
         values = torch.empty((n, _ceil(k, 16) * 16), dtype=torch.uint8,
                              device=b.device)
