@@ -44,6 +44,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -269,20 +271,22 @@ struct Sink {
     return m;
   }
 
-  // `cut`: some of the rows may lie past the last one; `met`: what meets()
-  // says; both are the same for all lanes.
+  // Scores of the table rows from v1 and the samples from n1 on.  `cut`: some
+  // of the rows may lie past the last one; `met`: what meets() says.  These
+  // four are the same for all lanes.
   template <int MR>
-  __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                       int64_t n, bool cut, bool met, const f32x4 (&scale)[MR]) {
-    if constexpr (USE == kLoss) take_loss(a, acc, v, cut);
-    if constexpr (USE == kCoef) take_coef(a, acc, v, n, cut, met);
-    if constexpr (USE == kStore) take_store(a, acc, v, n, scale);
+  __device__ __forceinline__ void take(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1, int n1,
+                                       bool cut, bool met) {
+    if constexpr (USE == kLoss) take_loss(a, acc, v1, cut);
+    if constexpr (USE == kCoef) take_coef(a, acc, v1 - a.v_begin, n1, cut, met);
+    if constexpr (USE == kStore) take_store(a, acc, v1, n1, cut);
   }
 
   template <int MR>
-  __device__ __forceinline__ void take_loss(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
+  __device__ __forceinline__ void take_loss(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1,
                                             bool cut) {
     if (cut) {
+      const int v = v1 + (threadIdx.x >> 4 & 3) * 4;
 #pragma unroll
       for (int i = 0; i < MR; ++i)
 #pragma unroll
@@ -344,11 +348,8 @@ struct Sink {
   }
 
   template <int MR>
-  __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                            int64_t n0, bool cut, bool met) {
-    // the first of the wave's samples and rows, the same in all lanes
-    const int64_t n1 = __builtin_amdgcn_readfirstlane((int)(n0 - (threadIdx.x & 15)));
-    const int v1 = __builtin_amdgcn_readfirstlane(v - a.v_begin);
+  __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1,
+                                            int n1, bool cut, bool met) {
     const int lane = threadIdx.x & 63;
     // 16 samples x 16 table rows are 512 bytes (1 KB) in one piece, as a wave
     // writes them and with every 16 bytes of one sample, as the products read
@@ -356,7 +357,8 @@ struct Sink {
     constexpr int es = TC == kF32 ? 4 : 2;
     const int in_block = (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
     auto put = [&](int i, int j, f32x4 c) {
-      char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es) + in_block;
+      char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es);
+      to += in_block;
       if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
       else *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
     };
@@ -376,7 +378,7 @@ struct Sink {
           for (int e = 0; e < 4; ++e)
             c[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], kLog2e, -lse2[j]));
         }
-        const int first = v + i * 16;
+        const int first = a.v_begin + v1 + (lane >> 4) * 4 + i * 16;
         if (met) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[e] -= first + e == yy[j] ? 1.f : 0.f;
@@ -393,38 +395,72 @@ struct Sink {
     }
   }
 
-  // `scale`: the column scales of the lane's rows
+  // 4 scores of neighbouring table rows; rows of the output start anywhere.
+  __device__ __forceinline__ static void put_scores(char* o, f32x4 s, bool bf16) {
+    if (bf16)
+      *reinterpret_cast<u32x2a2*>(o) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+    else
+      *reinterpret_cast<f32x4a4*>(o) = s;
+  }
+
+  // An instruction that writes 16 rows of the output, 64 bytes each, is slow: half of the lanes swap one
+  // of two blocks with the other half, so that it writes 8 rows, 128 bytes
+  // each (4096 x 200k float32 scores: 1.08 ms without, 0.78 ms with).
   template <int MR>
-  __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v,
-                                             int64_t n0, const f32x4 (&scale)[MR]) {
-    const int es = a.out_bf16 ? 2 : 4;
-    const bool vec = (a.ldo & 3) == 0;
+  __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1,
+                                             int n1, bool cut) {
+    const bool bf16 = a.out_bf16;
+    const int es = bf16 ? 2 : 4;
+    const int r16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+    const int left = (int)a.n - n1;          // samples from n1 on
+    char* first = a.out + ((int64_t)n1 * a.ldo + v1) * es;
+    if (cut) {
 #pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      const int vi = v + i * 16;
+      for (int i = 0; i < MR; ++i)
 #pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const int64_t n = n0 + j * 16;
-        if (n >= a.n) continue;
-        char* o = a.out + (n * a.ldo + vi) * es;
-        const f32x4 s = acc[i][j] * scale[i];
-        if (vec && vi + 3 < a.v_end) {
-          if (a.out_bf16)
-            *reinterpret_cast<u32x2*>(o) =
-                u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
-          else
-            *reinterpret_cast<f32x4*>(o) = s;
-        } else {
+        for (int j = 0; j < NS; ++j) {
+          if (r16 + j * 16 >= left) continue;
+          char* o = first + ((r16 + j * 16) * a.ldo + 4 * g + i * 16) * es;
+          const f32x4 s = acc[i][j];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (vi + e < a.v_end) {
-              if (a.out_bf16)
-                reinterpret_cast<__bf16*>(o)[e] = (__bf16)s[e];
-              else
-                reinterpret_cast<float*>(o)[e] = s[e];
+            if (v1 + 4 * g + i * 16 + e < a.v_end) {
+              if (bf16) reinterpret_cast<__bf16*>(o)[e] = (__bf16)s[e];
+              else reinterpret_cast<float*>(o)[e] = s[e];
             }
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
+      return;
+    }
+    if constexpr (MR % 2 == 0) {
+      const bool high = r16 & 8;
+      const int64_t in = ((r16 & 7) * a.ldo + 4 * g + (high ? 16 : 0)) * es;
+#pragma unroll
+      for (int i = 0; i < MR; i += 2)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const f32x4 x = acc[i][j], y = acc[i + 1][j];
+          f32x4 low, up;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float other = __int_as_float(__builtin_amdgcn_mov_dpp(
+                __float_as_int(high ? x[e] : y[e]), 0x128, 0xf, 0xf, false));   // row_ror:8
+            low[e] = high ? other : x[e];
+            up[e] = high ? y[e] : other;
+          }
+          char* o = first + (j * 16 * a.ldo + i * 16) * es;
+          if ((r16 & 7) + j * 16 < left) put_scores(o + in, low, bf16);
+          if ((r16 & 7) + j * 16 + 8 < left) put_scores(o + 8 * a.ldo * es + in, up, bf16);
+          __builtin_amdgcn_sched_barrier(0);      // or the registers do not do
+        }
+    } else {
+      const int64_t in = (r16 * a.ldo + 4 * g) * es;
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+          if (r16 + j * 16 < left)
+            put_scores(first + (j * 16 * a.ldo + i * 16) * es + in, acc[i][j], bf16);
     }
   }
 
@@ -550,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   constexpr int kBufs = kEach * 4 + 64 <= 81920 + (USE == kStore ? 0 : 64) ? 4 : kEach * 3 <= 81920 ? 3 : 2;
   constexpr int kAhead = kBufs - 1;
   constexpr int kLoads = kRows / 4 * kChunks / 64;   // per lane and tile
-  constexpr int MR = kRows / WV >= 32 && KS * NS <= 24 ? 2 : 1;
+  constexpr int MR = kRows / WV >= 32 && (KS * NS <= 24 || USE == kStore) ? 2 : 1;
   constexpr int kBlocks = (KS + 3) / 4;              // scales of a row
   constexpr int kScales = kRows * kBlocks;
   static_assert(kRows / 4 * kChunks % 64 == 0 && kRows % (16 * MR * WV) == 0, "");
@@ -560,7 +596,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   static_assert(!FP8 || kScales <= 256, "");
   // stores of a wave for one whole tile
   constexpr int kStores = USE == kLoss ? 0 : kRows / (16 * WV) * NS;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = wave % WV, wn = wave / WV;
   const int r16 = lane & 15, g = lane >> 4;
   int tn, split;
@@ -653,7 +690,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     if (t0 + i < t1) fetch(t0 + i);
   // Whether the wave makes all of kStores for every tile but the last: then
   // those made since this tile's loads need not be waited for.
-  const bool whole = n0 + (wn + 1) * (16 * NS) <= a.n && (USE != kStore || (a.ldo & 3) == 0);
+  const bool whole = n0 + (wn + 1) * (16 * NS) <= a.n;
   constexpr int kLater = (kAhead - 1) * kLoads, kMost = kLater + kAhead * kStores;
   for (int tile = t0; tile < t1; ++tile) {
     const int buf = (tile - t0) % kBufs;
@@ -667,7 +704,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
     const bool cut = v0 + kRows > a.v_end, met = sink.meets(v0, kRows);
     // Fragments are read kLead steps before they are used, those of the next
     // rows' first steps before these rows' scores are.
-    constexpr int kReads = FP8 ? KS / 2 : KS, kLead = kReads < 4 ? kReads : 4;
+    constexpr int kReads = FP8 ? KS / 2 : KS;
+    constexpr int kWant = MR == 2 && KS * NS > 24 ? 2 : 4, kLead = kReads < kWant ? kReads : kWant;
     constexpr int kGroups = kRows / (16 * MR * WV);
     u32x4 fa[kLead][MR];
     auto read = [&](int m, int k) {
@@ -711,13 +749,14 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 #pragma unroll
         for (int k = 0; k < kLead; ++k) read(m + 1, k);
       __builtin_amdgcn_sched_barrier(0);
-      f32x4 cs[MR];
+      if (USE == kStore && a.col_scale)
 #pragma unroll
-      for (int i = 0; i < MR; ++i)
-        cs[i] = USE == kStore && a.col_scale
-                    ? *reinterpret_cast<const f32x4*>(&col[buf][(row0 + i * 16 + 4 * g) % kRows])
-                    : f32x4{1.f, 1.f, 1.f, 1.f};
-      sink.template take<MR>(a, acc, v0 + row0 + 4 * g, n, cut, met, cs);
+        for (int i = 0; i < MR; ++i) {
+          const f32x4 cs = *reinterpret_cast<const f32x4*>(&col[buf][(row0 + i * 16 + 4 * g) % kRows]);
+#pragma unroll
+          for (int j = 0; j < NS; ++j) acc[i][j] *= cs;
+        }
+      sink.template take<MR>(a, acc, v0 + row0, (int)n0 + wn * (16 * NS), cut, met);
     }
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV>(a, lds[0], split, n0);
@@ -847,14 +886,18 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
     mma_all<TC>(fa, fb, acc);
     if (++step == steps) {
       const int v = a.v_begin + tile * kV + wv * 64 + 4 * g;
-      f32x4 cs[MR] = {};
-      if constexpr (USE == kStore)
+      if (USE == kStore && a.col_scale)
 #pragma unroll
-        for (int i = 0; i < MR; ++i)
+        for (int i = 0; i < MR; ++i) {
+          f32x4 cs;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) cs[i][e] = col_scale_of(a, v + i * 16 + e);
+          for (int e = 0; e < 4; ++e) cs[e] = col_scale_of(a, v + i * 16 + e);
+#pragma unroll
+          for (int j = 0; j < NS; ++j) acc[i][j] *= cs;
+        }
       const int v0 = a.v_begin + tile * kV + wv * 64;
-      sink.template take<MR>(a, acc, v, n, v0 + 64 > a.v_end, sink.meets(v0, 64), cs);
+      sink.template take<MR>(a, acc, v0, (int)n0 + wn * (16 * NS), v0 + 64 > a.v_end,
+                             sink.meets(v0, 64));
       step = 0;
       ++tile;
     }
@@ -872,7 +915,8 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
   constexpr int kAhead = 8;
   constexpr int kSteps = TW == kFP8 ? 2 : 1;         // instructions for 16 bytes of a row
   extern __shared__ __align__(16) char samples[];    // [step][NS][64 lanes][16 bytes]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   int tn, split;
   if (!place(a, tn, split)) return;
@@ -926,7 +970,7 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
 #pragma unroll
     for (int j = 0; j < NS; ++j) acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int v = v_first + group * 64 + 4 * g;
-    f32x4 cs[1] = {};
+    f32x4 cs = {1.f, 1.f, 1.f, 1.f};
     for (int k0 = 0; k0 < chunks; k0 += kAhead) {
       u32x4 now[kAhead];
       float scale[TW == kFP8 ? kAhead : 1];
@@ -940,7 +984,7 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
       if constexpr (USE == kStore)
         if (k0 + kAhead >= chunks)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) cs[0][e] = col_scale_of(a, v + e);
+          for (int e = 0; e < 4; ++e) cs[e] = col_scale_of(a, v + e);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (k0 + i >= chunks) break;
@@ -964,7 +1008,10 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
         }
       }
     }
-    sink.template take<1>(a, acc, v, n, v_first + group * 64 + 16 > a.v_end, false, cs);
+    if constexpr (USE == kStore)
+#pragma unroll
+      for (int j = 0; j < NS; ++j) acc[0][j] *= cs;
+    sink.template take<1>(a, acc, v - 4 * g, (int)n0, v_first + group * 64 + 16 > a.v_end, false);
   }
   if constexpr (USE == kLoss) sink.template finish_loss<4>(a, samples, split, n0);
 }
@@ -1554,13 +1601,13 @@ static void launch_tile(ScoreArgs& a, hipStream_t stream) {
   for (const Rows* r : {&a.w, &a.h})
     if (r->align != 16 || r->ld >= (1 << 23)) throw std::runtime_error("rows not aligned");
   const int64_t rows = a.v_end - a.v_begin;
-  if (a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
+  if (TW == kFP8 || a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
   // 128 x 128 fills the card more evenly; bf16 is bound by LDS there, and takes
   // 256 x 256 where there are enough of them
   if constexpr (TW != kFP8)
     if (TC == kF32 || ((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
       return launch_tile_k<TW, TC, USE, 2, 2, 4>(a, stream);
-  if constexpr (TC != kF32) launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
+  if constexpr (TW == kBF16) launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
 }
 
 // LDS that the samples of the streaming kernel take; 4 KB at least, for the
@@ -1898,13 +1945,16 @@ __global__ __launch_bounds__(256) void turn_scales_kernel(
     out[b * ldo + r] = scales[min(r, rows - 1) * lds + b];
 }
 
-// a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n]; turned: a byte for
-// every block of 128 columns and row, rows rounded up to 256, or null where
-// k <= 320, or m <= 16 and k <= 2048
+// a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n].  Where k > 320:
+//   m <= 128, but not with m <= 16 and k <= 2048: turned, a byte for every
+//   block of 128 columns and row, rows rounded up to 256
+//   m > 128: wide, bf16 [piece][k rounded up to 64].  Converting 8-bit rows in
+//   the product costs each workgroup registers that the product wants (1023 x
+//   150001 x 1024: 0.73 ms; converted first, a piece at a time, 0.50 ms)
 static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,
                         uintptr_t scales, int64_t lds, int64_t n, int64_t k, uintptr_t col_scale,
-                        uintptr_t out, int out_bf16, uintptr_t turned, int device,
-                        uintptr_t stream_ptr) {
+                        uintptr_t out, int out_bf16, uintptr_t turned, uintptr_t wide,
+                        int64_t piece, int device, uintptr_t stream_ptr) {
   const OnDevice on(device);
   if (m == 0 || n == 0) return;
   hipStream_t stream = (hipStream_t)stream_ptr;
@@ -1920,7 +1970,25 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
   a.out = (char*)out;
   a.ldo = n;
   a.out_bf16 = out_bf16;
-  if (turned) {
+  if (wide) {
+    const int64_t dp = (k + 63) / 64 * 64;
+    const Rows table = a.w;
+    for (int64_t v0 = 0; v0 < n; v0 += piece) {
+      const int64_t rows = std::min(piece, n - v0);
+      Rows part = table;
+      part.p += v0 * part.ld;
+      part.scales += v0 * part.lds;
+      part.rows = rows;
+      dequantize_kernel<kBF16><<<grid_of((rows * ((k + 7) / 8) + 1023) / 1024), 256, 0, stream>>>(
+          part, (int)k, (char*)wide, dp);
+      a.w = make_rows(wide, dp, rows, k, 2);
+      a.v_end = (int)rows;
+      a.splits = 1 << 20;
+      a.col_scale = col_scale ? (const float*)col_scale + v0 : nullptr;
+      a.out = (char*)out + v0 * (out_bf16 ? 2 : 4);
+      launch_tile<kBF16, kBF16, kStore>(a, stream);
+    }
+  } else if (turned) {
     const int64_t ldo = (n + 255) / 256 * 256;
     turn_scales_kernel<<<grid_of(ldo / 256), 256, 0, stream>>>(
         a.w.scales, a.w.lds, n, (int)((k + 127) / 128), (uint8_t*)turned, ldo);

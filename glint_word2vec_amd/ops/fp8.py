@@ -161,10 +161,16 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
         values = torch.empty((n, _ceil(k, 16) * 16), dtype=torch.uint8,
                              device=b.device)
         values[:, :k] = b.values.view(torch.uint8)
-    # the scales by block of columns, for the kernel that takes wide rows
-    turned = None if k <= 320 or (m <= 16 and k <= 2048) else \
-        torch.empty(_ceil(k, BLOCK) * _ceil(n, 256) * 256, dtype=torch.uint8,
-                    device=b.device)
+    # for wide rows: the scales by block of columns, or a piece of the table
+    turned = wide = None
+    piece = n
+    if k > 320 and m > 128:
+        piece = max(256, (64 << 20) // (_ceil(k, 64) * 128) // 256 * 256)
+        wide = torch.empty(min(piece, n) * _ceil(k, 64) * 64,
+                           dtype=torch.bfloat16, device=b.device)
+    elif k > 320 and not (m <= 16 and k <= 2048):
+        turned = torch.empty(_ceil(k, BLOCK) * _ceil(n, 256) * 256,
+                             dtype=torch.uint8, device=b.device)
     ld = _ceil(k, 8) * 8
     held = torch.empty((m, ld), dtype=torch.bfloat16, device=b.device)
     native, place = _native(), _place(b.device)
@@ -183,5 +189,6 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
         scales.data_ptr(), scales.stride(0), n, k,
         0 if col_scale is None else col_scale.data_ptr(), out.data_ptr(),
         int(out_dtype == torch.bfloat16),
-        0 if turned is None else turned.data_ptr(), *place)
+        0 if turned is None else turned.data_ptr(),
+        0 if wide is None else wide.data_ptr(), piece, *place)
     return out
