@@ -1946,9 +1946,9 @@ __global__ __launch_bounds__(256) void turn_scales_kernel(
 }
 
 // a: bf16 rows [m][k]; b: 8-bit rows [n][k]; out [m][n].  Where k > 320:
-//   m <= 128, but not with m <= 16 and k <= 2048: turned, a byte for every
+//   m <= 160, but not with m <= 16 and k <= 2048: turned, a byte for every
 //   block of 128 columns and row, rows rounded up to 256
-//   m > 128: wide, bf16 [piece][k rounded up to 64].  Converting 8-bit rows in
+//   m > 160: wide, bf16 [piece][k rounded up to 64].  Converting 8-bit rows in
 //   the product costs each workgroup registers that the product wants (1023 x
 //   150001 x 1024: 0.73 ms; converted first, a piece at a time, 0.50 ms)
 static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,

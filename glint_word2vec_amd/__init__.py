@@ -12,10 +12,11 @@ from .estimator import GlintWord2Vec, GlintWord2VecModel, LocalWord2VecModel
 from .vocab import Vocabulary, build_vocab
 
 
-def load_sharded(path, device="auto", dtype="auto"):
+def load_sharded(path, device="auto", dtype="auto", scores=None):
     """Convenience: GlintWord2VecModel.load_sharded (streaming,
     device-resident serving model)."""
-    return GlintWord2VecModel.load_sharded(path, device=device, dtype=dtype)
+    return GlintWord2VecModel.load_sharded(path, device=device, dtype=dtype,
+                                           scores=scores)
 
 __version__ = "0.1.0"
 __all__ = [

@@ -298,6 +298,8 @@ class GlintWord2VecModel:
         self.output_col = output_col
         self._norms: Optional[np.ndarray] = None
         self._gpu = None          # GpuSgns when to_gpu() was called
+        self._gpu_syn1 = False    # whether syn1 was uploaded too
+        self._fp8 = None          # (8-bit table, norms) for scores="fp8"
 
     # --- helpers ----------------------------------------------------------
     @property
@@ -321,17 +323,55 @@ class GlintWord2VecModel:
         return self._norms
 
     # --- GPU-resident serving (the PS-serving analog; inverse of toLocal) --
-    def to_gpu(self, device: str = "cuda", dtype: str = "float32"
-               ) -> "GlintWord2VecModel":
+    def to_gpu(self, device: str = "cuda", dtype: str = "float32",
+               scores: Optional[str] = None) -> "GlintWord2VecModel":
         """Upload syn0 to a GPU; findSynonyms (rocBLAS GEMV + norms kernel)
         and sentence-average transform (pull_average kernel) then run
-        device-side — the reference's server-side model ops."""
+        device-side — the reference's server-side model ops.
+        ``scores="fp8"``: findSynonyms scores an 8-bit copy of the table with
+        8-bit queries (ops/fp8.py; a value is off by 2^-4 at most)."""
         from .ops.gpu import GpuSgns
+        if scores not in (None, "fp8"):
+            raise ValueError(f"scores must be None or 'fp8', got {scores!r}")
         self._gpu = GpuSgns(self.num_words, self.vector_size, dtype=dtype,
                             device=device, syn0_host=self._f32())
         self._norms = None
         self._norms_t = None
+        self._gpu_syn1 = False
+        self._fp8 = None
+        if scores == "fp8":
+            self._fp8 = (self._gpu.quantize_table(), self._gpu.norms())
         return self
+
+    def softmax_loss(self, sentences, batch: int = 8192) -> float:
+        """Mean -log probability of every context word within the window
+        around every known word of ``sentences``, by the softmax over the
+        whole vocabulary: how well the model predicts held-out text.  Needs
+        to_gpu() and a model with syn1."""
+        if self._gpu is None:
+            raise RuntimeError("call to_gpu() first")
+        if self.syn1 is None:
+            raise ValueError("the model has no syn1: it was saved without")
+        import torch
+        if not self._gpu_syn1:
+            self._gpu.load_host(self._f32(), self.syn1)
+            self._gpu_syn1 = True
+        pairs = []
+        for sent in sentences:
+            ids = np.asarray([self.vocab[w] for w in sent if w in self.vocab],
+                             dtype=np.int32)
+            for o in range(1, min(self.config.window, len(ids) - 1) + 1):
+                pairs.append(np.stack([ids[:-o], ids[o:]]))
+                pairs.append(np.stack([ids[o:], ids[:-o]]))
+        if not pairs:
+            return float("nan")
+        both = torch.from_numpy(np.concatenate(pairs, axis=1)) \
+            .to(self._gpu.device)
+        total = torch.zeros((), dtype=torch.float64, device=both.device)
+        for i in range(0, both.shape[1], batch):
+            c, t = both[:, i:i + batch].unbind(0)
+            total += self._gpu.softmax_loss(c, t).double().sum()
+        return float(total) / both.shape[1]
 
     def transform_sentences_gpu(self, sentences) -> np.ndarray:
         """Batched sentence-average transform on the GPU (ml:443-456)."""
@@ -395,10 +435,14 @@ class GlintWord2VecModel:
             # hipGraph replay once multiply() became a hand-written
             # kernel (2.9k vs 2.4k q/s — the graph re-runs the query
             # staging copies; synonyms_query remains available)
-            if getattr(self, "_norms_t", None) is None:
-                self._norms_t = self._gpu.norms().clamp_min(1e-12)
-            cos_t = self._gpu.multiply(torch.from_numpy(vec),
-                                       norms=self._norms_t)
+            if self._fp8 is not None:
+                cos_t = self._gpu.multiply_fp8(torch.from_numpy(vec)[None],
+                                               *self._fp8)[0]
+            else:
+                if getattr(self, "_norms_t", None) is None:
+                    self._norms_t = self._gpu.norms().clamp_min(1e-12)
+                cos_t = self._gpu.multiply(torch.from_numpy(vec),
+                                           norms=self._norms_t)
             k = min(num + 1, self.num_words)
             val, idx = torch.topk(cos_t, k)
             val = val.cpu().numpy()
@@ -458,12 +502,16 @@ class GlintWord2VecModel:
         np.divide(vecs, qn, out=vecs, where=qn > 0)
         if self._gpu is not None:
             import torch
-            scores = self._gpu.multiply_batch(torch.from_numpy(vecs))
-            norms = (self._gpu.norms() if self._norms is None
-                     else torch.from_numpy(self._norms)
-                     .to(self._gpu.device))
-            cos = torch.where(norms[None, :] > 0, scores / norms[None, :],
-                              torch.zeros((), device=scores.device))
+            if self._fp8 is not None:
+                cos = self._gpu.multiply_fp8(torch.from_numpy(vecs),
+                                             *self._fp8)
+            else:
+                scores = self._gpu.multiply_batch(torch.from_numpy(vecs))
+                norms = (self._gpu.norms() if self._norms is None
+                         else torch.from_numpy(self._norms)
+                         .to(self._gpu.device))
+                cos = torch.where(norms[None, :] > 0, scores / norms[None, :],
+                                  torch.zeros((), device=scores.device))
             k = min(num + 1, cos.shape[1])
             val, idx = torch.topk(cos, k, dim=1)
             val = val.cpu().numpy()
@@ -540,7 +588,7 @@ class GlintWord2VecModel:
 
     @classmethod
     def load_sharded(cls, path: str, device: str = "auto",
-                     dtype: str = "auto"):
+                     dtype: str = "auto", scores: Optional[str] = None):
         """Load WITHOUT host materialisation: rows stream from the shard
         files straight to each rank's device and serving ops (findSynonyms
         / transform / getVector) run sharded — the reference's PS-side
@@ -548,7 +596,8 @@ class GlintWord2VecModel:
         under torchrun (one rank per GPU); returns a
         serving.ShardedWord2VecModel."""
         from .serving import ShardedWord2VecModel
-        return ShardedWord2VecModel.load(path, device=device, dtype=dtype)
+        return ShardedWord2VecModel.load(path, device=device, dtype=dtype,
+                                         scores=scores)
 
     def stop(self, terminate_other_clients: bool = False) -> None:
         """Release training resources (reference: stops PS cluster,

@@ -24,7 +24,8 @@ BLOCK = 128
 class Fp8Rows(NamedTuple):
     """``values`` float8_e4m3fn [R, K] and ``scales`` float8_e8m0fnu
     [R, ceil(K / 128)]: element (r, k) stands for
-    values[r, k] * scales[r, k // 128]."""
+    values[r, k] * scales[r, k // 128].  Scales are from 2^-126 to 2^127;
+    beyond that they are taken as the nearest of those."""
     values: torch.Tensor
     scales: torch.Tensor
 
@@ -50,8 +51,8 @@ def _check_float(name: str, x) -> None:
                          f"column, got {list(x.shape)}")
     if x.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"unsupported dtype {x.dtype}: float32 or bfloat16")
-    if x.shape[0] >= 2 ** 31 or x.shape[1] > 1 << 24:
-        raise ValueError("at most 2^31 - 1 rows of 2^24 columns")
+    if x.shape[0] > 2 ** 31 - 1024 or x.shape[1] > 1 << 24:
+        raise ValueError("at most 2^31 - 1024 rows of 2^24 columns")
     if not x.is_cuda:
         raise RuntimeError(f"the 8-bit kernels run on the GPU: move {name} "
                            "there")
@@ -72,8 +73,8 @@ def _check_rows(name: str, q) -> Fp8Rows:
         raise ValueError(f"{name}: {list(values.shape)} values need one scale "
                          f"for every {BLOCK} columns, got "
                          f"{list(scales.shape)}")
-    if values.shape[0] >= 2 ** 31 or values.shape[1] > 1 << 24:
-        raise ValueError("at most 2^31 - 1 rows of 2^24 columns")
+    if values.shape[0] > 2 ** 31 - 1024 or values.shape[1] > 1 << 24:
+        raise ValueError("at most 2^31 - 1024 rows of 2^24 columns")
     if not (values.is_cuda and scales.is_cuda):
         raise RuntimeError(f"the 8-bit kernels run on the GPU: move {name} "
                            "there")
@@ -164,7 +165,7 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
     # for wide rows: the scales by block of columns, or a piece of the table
     turned = wide = None
     piece = n
-    if k > 320 and m > 128:
+    if k > 320 and m > 160:
         piece = max(256, (64 << 20) // (_ceil(k, 64) * 128) // 256 * 256)
         wide = torch.empty(min(piece, n) * _ceil(k, 64) * 64,
                            dtype=torch.bfloat16, device=b.device)

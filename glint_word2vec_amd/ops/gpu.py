@@ -278,3 +278,49 @@ class GpuSgns:
                         device=self.device)
         q[:, :self.dim] = vecs.to(self.syn0.dtype).to(self.device)
         return (q @ self.syn0.T).float()
+
+    # --- the whole vocabulary at once (ops/softmax.py, ops/fp8.py) ----------
+    def softmax_loss(self, centers: torch.Tensor, targets: torch.Tensor
+                     ) -> torch.Tensor:
+        """-log of the softmax probability that center word's vector (syn0)
+        gives its target among all words (syn1): float32 [N], the exact form
+        of what negative sampling approximates.  Targets of -1 count 0."""
+        from .softmax import softmax_loss_forward
+        h = self.syn0[centers.to(self.device)]
+        return softmax_loss_forward(h[:, :self.dim], self.syn1[:, :self.dim],
+                                    targets.to(self.device))[0]
+
+    def train_softmax(self, centers: torch.Tensor, targets: torch.Tensor,
+                      alpha: float) -> torch.Tensor:
+        """One SGD step on the sum of softmax_loss over the pairs, from the
+        tables as they are before it; returns the losses [N].  Exact where
+        train_batch samples: every word's output row moves.  Repeated centers
+        add up, in a fixed order."""
+        from .softmax import softmax_loss_backward, softmax_loss_forward
+        centers = centers.to(self.device, torch.long)
+        targets = targets.to(self.device)
+        h = self.syn0[centers][:, :self.dim]
+        w = self.syn1[:, :self.dim]
+        loss, lse = softmax_loss_forward(h, w, targets)
+        step = torch.full((), -float(alpha), device=self.device)
+        dh, dw = softmax_loss_backward(h, w, targets, lse, step)
+        w.add_(dw)
+        self.syn0[:, :self.dim].index_put_((centers,), dh, accumulate=True)
+        return loss
+
+    def quantize_table(self):
+        """syn0 in 8-bit floats as it is now: an ``fp8.Fp8Rows`` of half the
+        bytes of bfloat16, for multiply_fp8."""
+        from .fp8 import quantize_rows
+        return quantize_rows(self.syn0[:, :self.dim])
+
+    def multiply_fp8(self, vecs: torch.Tensor, table,
+                     norms: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Scores [Q, vocab] of queries against an 8-bit table from
+        quantize_table, the queries in 8 bits too.  ``norms`` fuses the cosine
+        divide; a norm of 0 gives scores of 0."""
+        from .fp8 import matmul_rows
+        scale = None if norms is None else \
+            torch.where(norms > 0, 1.0 / norms, torch.zeros_like(norms))
+        return matmul_rows(vecs.float().to(self.device), table,
+                           col_scale=scale)

@@ -78,8 +78,8 @@ def _check(h, w, targets) -> None:
         raise TypeError(f"h is {h.dtype} but w is {w.dtype}")
     if targets.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
-    if max(h.shape[0], w.shape[0]) >= 2 ** 31:
-        raise ValueError("at most 2^31 - 1 rows")
+    if max(h.shape[0], w.shape[0]) > 2 ** 31 - 1024 or w.shape[1] > 1 << 24:
+        raise ValueError("at most 2^31 - 1024 rows of 2^24 columns")
     if not (h.is_cuda and w.is_cuda and targets.is_cuda):
         raise RuntimeError("the softmax kernels run on the GPU: move h, w and "
                            "targets there")

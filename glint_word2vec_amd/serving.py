@@ -107,13 +107,19 @@ class ShardedWord2VecModel:
         self.device = shard.device
         self.is_cuda = shard.device.type == "cuda"
         self._norms: Optional[torch.Tensor] = None   # local shard norms
+        self._fp8 = None              # the shard in 8 bits, for scores
 
     # ------------------------------------------------------------------
     @classmethod
     def load(cls, path: str, device: str = "auto", dtype: str = "auto",
-             block_rows: int = 1 << 20) -> "ShardedWord2VecModel":
+             block_rows: int = 1 << 20,
+             scores: Optional[str] = None) -> "ShardedWord2VecModel":
         """Streaming sharded load (the PS-side load, mllib:717-722).
-        Host RSS stays O(block_rows*dim) + the word index (~24 B/word)."""
+        Host RSS stays O(block_rows*dim) + the word index (~24 B/word).
+        ``scores="fp8"``: findSynonyms scores an 8-bit copy of the shard with
+        8-bit queries (ops/fp8.py; GPU only)."""
+        if scores not in (None, "fp8"):
+            raise ValueError(f"scores must be None or 'fp8', got {scores!r}")
         rank, world = comm.init_from_env()
         if device == "auto":
             device = "cuda" if torch.cuda.is_available() else "cpu"
@@ -162,6 +168,9 @@ class ShardedWord2VecModel:
             raise ValueError(f"words file has {vocab.num_words} entries, "
                              f"index says {V}")
         m = cls(config, vocab, shard, rank, world, D)
+        if scores == "fp8":
+            from .ops.fp8 import quantize_rows
+            m._fp8 = quantize_rows(shard)
         log.info("sharded load: rank %d/%d holds %d of %d rows (%s, %s)",
                  rank, world, shard_size, V, device, tdtype)
         return m
@@ -297,11 +306,18 @@ class ShardedWord2VecModel:
             skip_words.append(w)
             n = np.linalg.norm(v)
             vecs[qi] = v / n if n > 0 else v
-        qs = torch.from_numpy(vecs).to(self.shard.dtype).to(self.device)
-        scores = (qs @ self.shard.T).float()            # [Q, shard]
         norms = self._local_norms()
-        cos = torch.where(norms[None, :] > 0, scores / norms[None, :],
-                          torch.zeros((), device=self.device))
+        if self._fp8 is not None:
+            from .ops.fp8 import matmul_rows
+            cos = matmul_rows(
+                torch.from_numpy(vecs).to(self.device), self._fp8,
+                col_scale=torch.where(norms > 0, 1.0 / norms,
+                                      torch.zeros_like(norms)))
+        else:
+            qs = torch.from_numpy(vecs).to(self.shard.dtype).to(self.device)
+            scores = (qs @ self.shard.T).float()        # [Q, shard]
+            cos = torch.where(norms[None, :] > 0, scores / norms[None, :],
+                              torch.zeros((), device=self.device))
         k = min(num + 1, cos.shape[1])
         val, loc = torch.topk(cos, k, dim=1)            # [Q, k]
         val = val.T.contiguous()                        # [k, Q] for gather

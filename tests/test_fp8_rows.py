@@ -132,7 +132,11 @@ def _product(a, b, b64, col_scale=None, out=torch.float32, given=False):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off"
 
 
-PRODUCTS = [(1, 1, 1), (1, 5, 16), (1, 300, 300), (2, 129, 128), (16, 1000, 100),
+# (queries at which another kernel takes over, narrow and wide rows)
+PRODUCTS = [(16, 700, 20), (17, 700, 321), (16, 300, 2049), (32, 1025, 330),
+            (40, 600, 64), (160, 300, 400), (161, 515, 400), (200, 900, 321),
+            (300, 601, 200), (2, 150_000, 40), (70, 70_001, 300),
+            (18, 150_000, 330), (1, 1, 1), (1, 5, 16), (1, 300, 300), (2, 129, 128), (16, 1000, 100),
             (17, 257, 301), (33, 64, 1024), (64, 500, 257), (65, 128, 640),
             (128, 3613, 100), (129, 130, 131), (300, 700, 2048)]
 
@@ -149,6 +153,33 @@ def test_product(m, n, k, out):
     _product(a, q, b64, cs, out)
     _product(a.bfloat16(), q, b64, cs, out)
     _product(a, q, b64, cs, out, given=True)
+
+
+@gpu
+def test_product_in_many_pieces(monkeypatch):
+    """More table rows than one piece of the converted table holds."""
+    b = _rows(9000, 4000, torch.bfloat16, seed=3)
+    q, b64 = fp8.quantize_rows(b), _held(b)[0]
+    cs = torch.rand(9000, generator=torch.Generator().manual_seed(5)).cuda()
+    _product(_rows(170, 4000, torch.float32), q, b64, cs, torch.bfloat16)
+
+
+@gpu
+def test_scales_that_start_anywhere():
+    b = _rows(200, 300, torch.float32)
+    q, b64 = fp8.quantize_rows(b), _held(b)[0]
+    for before in (1, 2, 3):
+        flat = torch.zeros(200 * 3 + before, dtype=torch.uint8, device="cuda")
+        flat[before:] = q.scales.view(torch.uint8).flatten()
+        moved = fp8.Fp8Rows(q.values, flat[before:].view(200, 3)
+                            .view(torch.float8_e8m0fnu))
+        for m in (1, 20, 80):
+            _product(_rows(m, 300, torch.float32, m), moved, b64)
+    wide = torch.zeros(200, 5, dtype=torch.uint8, device="cuda")
+    wide[:, 1:4] = q.scales.view(torch.uint8)
+    moved = fp8.Fp8Rows(q.values, wide.view(torch.float8_e8m0fnu)[:, 1:4])
+    _product(_rows(20, 300, torch.float32), moved, b64)
+    assert torch.equal(fp8.dequantize_rows(moved).double().cpu(), b64)
 
 
 @gpu

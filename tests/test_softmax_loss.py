@@ -96,11 +96,41 @@ def test_matches_float64(n, v, d, dtype):
     _check(*_inputs(n, v, d, dtype, seed=n + v + d))
 
 
+# samples around the sizes at which another kernel takes over, narrow and wide
+# rows
+FORMS = [(16, 700, 20), (17, 700, 321), (32, 1025, 330), (33, 600, 400),
+         (64, 900, 640), (65, 513, 321), (100, 1300, 512), (128, 1000, 40),
+         (130, 1000, 700), (256, 2600, 200), (300, 515, 1030), (31, 257, 2049),
+         (700, 300, 33)]
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_many_pieces_of_the_vocabulary(dtype, monkeypatch):
+@pytest.mark.parametrize("n,v,d", FORMS)
+def test_forms(n, v, d, dtype):
+    _check(*_inputs(n, v, d, dtype, seed=n + v + d))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v,d", [(2, 150_000, 24), (40, 150_001, 300),
+                                   (40, 140_000, 330), (260, 70_000, 40)])
+def test_many_tiles_for_each_workgroup(n, v, d, dtype):
+    _check(*_inputs(n, v, d, dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [5, 70])
+def test_many_pieces_of_the_vocabulary(n, dtype, monkeypatch):
     monkeypatch.setattr(S, "_COEF_BYTES", 1 << 16)
-    _check(*_inputs(70, 1500, 96, dtype))
+    monkeypatch.setattr(S, "_PACKED_BYTES", 1 << 16)
+    h, w, y = _inputs(n, 1500, 97, dtype)
+    _check(h, w, y)
+    # unaligned, so that the pieces are packed
+    big = torch.zeros(1502, 103, dtype=dtype, device="cuda")
+    big[1:-1, 5:102] = w
+    _check(h, big[1:-1, 5:102], y)
 
 
 @gpu
@@ -328,6 +358,39 @@ def test_captured_step():
         for graph, out in graphs:
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [88, 350])
+def test_captured_without_a_call_before(d, dtype):
+    h, w, y = _inputs(45, 333, d, dtype)
+    one = torch.ones((), device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, lse = S.softmax_loss_forward(h, w, y)
+        dh, dw = S.softmax_loss_backward(h, w, y, lse, one)
+    graph.replay()
+    loss2, lse2 = S.softmax_loss_forward(h, w, y)
+    dh2, dw2 = S.softmax_loss_backward(h, w, y, lse2, one)
+    torch.cuda.synchronize()
+    for a, b in ((loss, loss2), (lse, lse2), (dh, dh2), (dw, dw2)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_two_steps_before_the_first_is_read():
+    """Calls that are queued behind each other do not share workspaces."""
+    first = _inputs(300, 4000, 64, torch.bfloat16, seed=1)
+    second = _inputs(200, 3000, 200, torch.float32, seed=2)
+    one = torch.ones((), device="cuda")
+    out = []
+    for h, w, y in (first, second, first):
+        loss, lse = S.softmax_loss_forward(h, w, y)
+        out.append((loss, *S.softmax_loss_backward(h, w, y, lse, one)))
+    for a, b in zip(out[0], out[2]):
+        assert torch.equal(a, b)
+    _check(*second)
 
 
 @gpu
