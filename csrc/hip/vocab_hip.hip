@@ -204,9 +204,7 @@ struct ScoreArgs {
   int targets64;
   int64_t ignore, vocab;
   const float* lse;
-  const float* grad;
-  int grad_step;
-  const float* weight;      // one factor for all samples, or null
+  const float* grad;        // of every sample's loss, or null for ones
   // [coef_rows][ldc] in blocks of 16 x 16, column 0 = table row v_begin,
   // zeros in rows from N on
   char* coef;
@@ -217,6 +215,11 @@ struct ScoreArgs {
   int64_t ldo;
   int out_bf16;
 };
+
+// The product of up to two numbers in memory.
+__device__ __forceinline__ float scale_by(const float* a, const float* b) {
+  return (a ? *a : 1.f) * (b ? *b : 1.f);
+}
 
 __device__ __forceinline__ int64_t target_of(const void* t, int is64, int64_t n) {
   return is64 ? reinterpret_cast<const int64_t*>(t)[n]
@@ -239,7 +242,6 @@ struct Sink {
       far = false;
     }
     if constexpr (USE == kCoef) {
-      const float wt = a.weight ? *a.weight : 1.f;
 #pragma unroll
       for (int j = 0; j < NS; ++j) {
         const int64_t m = n + j * 16;
@@ -249,7 +251,7 @@ struct Sink {
           if (y != a.ignore && y >= 0 && y < a.vocab) {
             yy[j] = (int)y;
             lse2[j] = a.lse[m] * kLog2e;
-            gg[j] = a.grad[m * a.grad_step] * wt;
+            gg[j] = a.grad ? a.grad[m] : 1.f;
           }
         }
       }
@@ -769,7 +771,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 // they are read from LDS, and their scales lie by block of columns, then row.
 template <int TW, int TC, int USE, int WV, int WN, int NS>
 __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
-  constexpr int kWaves = WV * WN, kAhead = 3, MR = 4;
+  // float32 steps are long: two ahead do, and three workgroups fit a CU
+  constexpr int kWaves = WV * WN, kAhead = TC == kF32 ? 2 : 3, MR = 4;
   constexpr int kV = 64 * WV, kN = 16 * NS * WN;
   constexpr int kWideW = TW == kFP8 ? 32 : 64, kWideH = 64;   // bytes per step
   constexpr int kBytesW = kV * kWideW, kBytesH = kN * kWideH;
@@ -836,7 +839,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
     if (i < all) fetch(i);
-  int tile = t0, step = 0;
+  int tile = t0, step = 0, at_buf = 0;
   for (int64_t s = 0; s < all; ++s) {
     // step s has arrived, two more may be on their way
     if (s + kAhead - 1 < all) {
@@ -846,14 +849,15 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
       wait_loads();
     }
     __syncthreads();
-    if (s + kAhead < all) fetch((int)(s + kAhead) & kAhead);
+    if (s + kAhead < all) fetch(at_buf == 0 ? kAhead : at_buf - 1);
     if (step == 0) {
 #pragma unroll
       for (int i = 0; i < MR; ++i)
 #pragma unroll
         for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const char* buf = lds[s & kAhead];
+    const char* buf = lds[at_buf];
+    at_buf = at_buf == kAhead ? 0 : at_buf + 1;
     const char* lh = buf + kBytesW + wn * (16 * NS) * kWideH;
     const int at = r16 * 64 + row_chunk(64, r16, g) * 16;
     u32x4 fa[MR], fb[NS];
@@ -1100,6 +1104,7 @@ struct GradArgs {
   float* part;   // [splits][R][ldp], added to where `add`; or null, and
   int64_t ldp;
   int add;
+  const float* scale[2];   // factors of all results, or null
   char* out;     // [R][D], of the rows' type
   int64_t ldo;
 };
@@ -1132,7 +1137,8 @@ __global__ __launch_bounds__(256) void pack_kernel(
 // larger part, as often as there are tiles of d; fewer samples than that take
 // the forms with fewer rows.  Steps of 64 bytes of k (32 of bf16, 16 of
 // float32) go straight into LDS, kAhead steps ahead of the one at work: three,
-// or one where k is short and several workgroups a CU do more.
+// two for float32, whose steps are long, or one where k is short: there several
+// workgroups a CU do more.
 template <int T, bool DW, int ND, int WR, int J, int kAhead>
 __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   constexpr int ES = Elem<T>::size, WD = 8 / WR;
@@ -1272,6 +1278,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
       mma_row<T>(fa, fb, acc[i]);
     }
   }
+  const float scale = a.part ? 1.f : scale_by(a.scale[0], a.scale[1]);
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int64_t r = r0 + (wr * J + j) * 16 + r16;
@@ -1280,6 +1287,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
     for (int i = 0; i < ND; ++i) {
       const int d = d0 + (wd * ND + i) * 16 + 4 * g;
       if (d >= a.d) continue;
+      acc[i][j] *= scale;
       if (a.part) {
         f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
         *o = a.add ? *o + acc[i][j] : acc[i][j];
@@ -1312,7 +1320,8 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
 // parts of few results are added at the same time, in a fixed order.
 template <int T, int G>
 __global__ __launch_bounds__(256) void sum_parts_kernel(
-    const float* part, int splits, int64_t rows, int64_t ldp, int d, char* out) {
+    const float* part, int splits, int64_t rows, int64_t ldp, int d, const float* scale0,
+    const float* scale1, char* out) {
   constexpr int kEach = 256 / G;
   __shared__ float sums[G][kEach];
   const int at = threadIdx.x % kEach, group = threadIdx.x / kEach;
@@ -1329,6 +1338,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
   if (group == 0 && i < total) {
 #pragma unroll
     for (int k = 1; k < G; ++k) s += sums[k][at];
+    s *= scale_by(scale0, scale1);
     if constexpr (T == kF32) reinterpret_cast<float*>(out)[i] = s;
     else reinterpret_cast<__bf16*>(out)[i] = (__bf16)s;
   }
@@ -1712,10 +1722,11 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
 }
 
 static void launch_sum_parts(const float* part, int splits, int64_t rows, int64_t ldp, int64_t d,
-                             int is_bf16, char* out, hipStream_t stream) {
+                             const float* const (&scale)[2], int is_bf16, char* out,
+                             hipStream_t stream) {
   auto go = [&](auto kernel, int each) {
     kernel<<<grid_of((rows * d + each - 1) / each), 256, 0, stream>>>(part, splits, rows, ldp,
-                                                                     (int)d, out);
+                                                                     (int)d, scale[0], scale[1], out);
   };
   if (splits >= 16)
     is_bf16 ? go(sum_parts_kernel<kBF16, 16>, 16) : go(sum_parts_kernel<kF32, 16>, 16);
@@ -1751,6 +1762,7 @@ static GradForm grad_form(bool bf16, bool dw, int64_t r, int64_t k, int d) {
     const int t = (d + 16 * n * wd - 1) / (16 * n * wd);
     if (t * n < least || (t * n == least && n > 2)) least = t * n, f.nd = n, f.tiles_d = t;
   }
+  if (f.rows == 256 && f.nd <= 4) f.slots = 512;
   return f;
 }
 
@@ -1803,8 +1815,9 @@ static void launch_grad(GradArgs b, hipStream_t stream) {
     CASE_ND(128, 1, 2, 4, 3) CASE_ND(128, 2, 2, 4, 3) CASE_ND(128, 3, 2, 4, 3)
     CASE_ND(128, 4, 2, 4, 3) CASE_ND(128, 5, 2, 4, 3)
   }
-  CASE_ND(256, 2, 4, 4, 3) CASE_ND(256, 4, 4, 4, 3) CASE_ND(256, 6, 4, 4, 3)
-  CASE_ND(256, 8, 4, 4, 3) CASE_ND(256, 10, 4, 4, 3)
+  constexpr int kAhead = T == kF32 ? 2 : 3;
+  CASE_ND(256, 2, 4, 4, kAhead) CASE_ND(256, 4, 4, 4, kAhead) CASE_ND(256, 6, 4, 4, kAhead)
+  CASE_ND(256, 8, 4, 4, kAhead) CASE_ND(256, 10, 4, 4, kAhead)
 #undef CASE_ND
   throw std::runtime_error("no kernel for these columns");
 }
@@ -1831,6 +1844,10 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
   const Rows rh = pack(make_rows(h, ldh, n, d, es), is_bf16, (const void*)targets, targets64,
                        ignore, v, packed, np, dp, stream);
   const bool pack_w = packed_w != 0;
+  // One gradient for all samples stays out of the coefficients: in bf16 it
+  // would round all of them by the same 2^-9 or less.
+  const float* const scale[2] = {grad_step ? nullptr : (const float*)grad,
+                                 (const float*)weight};
   for (int64_t v0 = 0; v0 < v; v0 += chunk) {
     const int64_t v1 = std::min(v, v0 + chunk);
     // the table's rows from v0 on; v_begin and the targets count from row 0
@@ -1851,9 +1868,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.targets64 = targets64;
     a.ignore = ignore;
     a.lse = (const float*)lse;
-    a.grad = (const float*)grad;
-    a.grad_step = grad_step;
-    a.weight = (const float*)weight;
+    a.grad = grad_step ? (const float*)grad : nullptr;
     a.coef = (char*)coef;
     a.coef_rows = np;
     a.ldc = chunk;
@@ -1864,6 +1879,8 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     b.ldc = chunk;
     b.d = (int)d;
     b.ldp = ldp;
+    b.scale[0] = scale[0];
+    b.scale[1] = scale[1];
     if (dh) {
       b.x = piece;
       b.r = n;
@@ -1886,11 +1903,11 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       if (is_bf16) launch_grad<kBF16, true>(b, stream);
       else launch_grad<kF32, true>(b, stream);
       if (splits_w > 1)
-        launch_sum_parts(b.part, splits_w, v1 - v0, ldp, d, is_bf16, b.out, stream);
+        launch_sum_parts(b.part, splits_w, v1 - v0, ldp, d, scale, is_bf16, b.out, stream);
     }
   }
   if (dh)
-    launch_sum_parts((const float*)part, splits, n, ldp, d, is_bf16, (char*)dh, stream);
+    launch_sum_parts((const float*)part, splits, n, ldp, d, scale, is_bf16, (char*)dh, stream);
   HIP_CHECK(hipGetLastError());
 }
 
