@@ -499,13 +499,14 @@ struct Sink {
 };
 
 // The workgroup's tile of samples and part of the table.  Workgroups go round
-// the 8 XCDs; those of one XCD take all sample tiles of one part of the table
-// before the next part, so that its L2 gets each table row from memory once.
-__device__ __forceinline__ bool place(const ScoreArgs& a, int& tn, int& split) {
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+// the 8 XCDs.  Where there are parts for all XCDs, those of one XCD take all
+// sample tiles of one part before the next part, so that its L2 gets each
+// table row from memory once.
+__device__ __forceinline__ void place(const ScoreArgs& a, int& tn, int& split) {
+  const int of = a.splits % 8 == 0 ? 8 : 1;
+  const int at = blockIdx.x / of;
   tn = at % a.tiles_n;
-  split = (at / a.tiles_n) * 8 + xcd;
-  return split < a.splits;
+  split = at / a.tiles_n * of + (of == 8 ? blockIdx.x & 7 : 0);
 }
 
 // [t0, t1): part `split` of `splits` of the tiles.
@@ -603,7 +604,7 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
   const int wv = wave % WV, wn = wave / WV;
   const int r16 = lane & 15, g = lane >> 4;
   int tn, split;
-  if (!place(a, tn, split)) return;
+  place(a, tn, split);
   int t0, t1;
   part_of((a.v_end - a.v_begin + kRows - 1) / kRows, split, a.splits, t0, t1);
   const int64_t n0 = (int64_t)tn * (16 * NS * WN);
@@ -789,7 +790,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   const int wv = wave % WV, wn = wave / WV;
   const int r16 = lane & 15, g = lane >> 4;
   int tn, split;
-  if (!place(a, tn, split)) return;
+  place(a, tn, split);
   int t0, t1;
   part_of((a.v_end - a.v_begin + kV - 1) / kV, split, a.splits, t0, t1);
   const int64_t n0 = (int64_t)tn * kN;
@@ -923,7 +924,7 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   int tn, split;
-  if (!place(a, tn, split)) return;
+  place(a, tn, split);
   const int64_t n0 = (int64_t)tn * (16 * NS);
   const int64_t n = n0 + r16;
   const int chunks = (a.w.kb + 63) / 64;             // per lane and row
@@ -1160,10 +1161,9 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   // the parts of k go round the XCDs: the tiles of r that share rows of x are
   // in one XCD at a time
   const int tiles = a.tiles_d * a.tiles_r;
-  const int split = a.splits >= 8 ? (int)(blockIdx.x & 7) + 8 * (int)((blockIdx.x >> 3) / tiles)
-                                  : (int)blockIdx.x / tiles;
-  const int at = a.splits >= 8 ? (int)(blockIdx.x >> 3) % tiles : (int)blockIdx.x % tiles;
-  if (split >= a.splits) return;
+  const int of = a.splits % 8 == 0 ? 8 : 1;
+  const int split = (int)(blockIdx.x / of) / tiles * of + (of == 8 ? blockIdx.x & 7 : 0);
+  const int at = (int)(blockIdx.x / of) % tiles;
   const int td = at % a.tiles_d, tr = at / a.tiles_d;
   int s0, s1;
   part_of((int)((a.k + kStep - 1) / kStep), split, a.splits, s0, s1);
@@ -1533,7 +1533,7 @@ static int grid_of(int64_t blocks) {
 }
 
 static int score_grid(const ScoreArgs& a) {
-  return grid_of((int64_t)8 * a.tiles_n * ((a.splits + 7) / 8));
+  return grid_of((int64_t)a.tiles_n * a.splits);
 }
 
 // How many workgroups of a kernel the card holds at a time.
@@ -1549,13 +1549,15 @@ static int slots_of(K kernel, int threads, int lds) {
 // Cuts the table into at most a.splits parts of whole tiles of `rows` rows.
 // With `slots` workgroups at a time, R rounds of them leave room for
 // R slots / tiles_n parts; of one to four rounds the one is taken in which the
-// longest workgroups end first.  A workgroup's start counts as one tile.
+// longest workgroups end first.  A workgroup's start counts as one tile.  Parts
+// of several tiles are a multiple of 8, so that all XCDs have as many.
 static void cut(ScoreArgs& a, int64_t rows, int slots) {
   const int64_t tiles = (a.v_end - a.v_begin + rows - 1) / rows;
   int64_t best = 1, least = INT64_MAX;
   for (int64_t rounds = 1; rounds <= 4; ++rounds) {
     int64_t parts = std::max<int64_t>(1, rounds * slots / a.tiles_n);
     parts = std::min(std::min<int64_t>(parts, a.splits), tiles);
+    if (parts > 8 && parts < tiles) parts &= ~7;
     const int64_t each = (tiles + parts - 1) / parts;
     const int64_t time = (parts * a.tiles_n + slots - 1) / slots * (each + 1);
     if (time < least) least = time, best = parts;
@@ -1798,7 +1800,7 @@ template <int T, bool DW, int ND, int WR, int J, int kAhead>
 static void launch_grad_k(GradArgs& b, hipStream_t stream) {
   b.tiles_r = grid_of((b.r + 16 * J * WR - 1) / (16 * J * WR));
   const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
-  const int blocks = grid_of(b.splits >= 8 ? tiles * ((b.splits + 7) / 8) * 8 : tiles * b.splits);
+  const int blocks = grid_of(tiles * b.splits);
   grad_kernel<T, DW, ND, WR, J, kAhead><<<blocks, 512, 0, stream>>>(b);
 }
 
