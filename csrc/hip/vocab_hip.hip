@@ -1066,10 +1066,10 @@ __global__ __launch_bounds__(256) void loss_join_kernel(
 }
 
 // Sum or mean over the samples that count, in 64 bits and a fixed order.
-// out[0] = the sum times out[1]; out[1] = 1 / count for the mean, 1 for the sum.
+// factor = 1 / count for the mean, 1 for the sum; result = the sum times it.
 __global__ __launch_bounds__(1024) void loss_reduce_kernel(
     const float* loss, const void* targets, int targets64, int64_t ignore,
-    int64_t n, int mean, float* out) {
+    int64_t n, int mean, float* result, float* factor) {
   __shared__ double sums[16];
   __shared__ long long counts[16];
   double s = 0;
@@ -1083,8 +1083,8 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i];
     const double f = mean ? 1.0 / (double)c : 1.0;
-    out[0] = (float)(s * f);
-    out[1] = (float)f;
+    *result = (float)(s * f);
+    *factor = (float)f;
   }
 }
 
@@ -1678,7 +1678,8 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
                          int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t packed_h,
                          uintptr_t packed_w, int64_t piece, uintptr_t loss, uintptr_t lse,
-                         int reduce, uintptr_t reduced, int device, uintptr_t stream_ptr) {
+                         int reduce, uintptr_t result, uintptr_t factor, int device,
+                         uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
   const int es = is_bf16 ? 2 : 4;
@@ -1719,7 +1720,8 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
   }
   if (reduce)      // 1: sum, 2: mean
     loss_reduce_kernel<<<1, 1024, 0, stream>>>((const float*)loss, (const void*)targets,
-                                               targets64, ignore, n, reduce == 2, (float*)reduced);
+                                               targets64, ignore, n, reduce == 2, (float*)result,
+                                               (float*)factor);
   HIP_CHECK(hipGetLastError());
 }
 

@@ -280,25 +280,39 @@ class GpuSgns:
         return (q @ self.syn0.T).float()
 
     # --- the whole vocabulary at once (ops/softmax.py, ops/fp8.py) ----------
+    def _pairs(self, centers: torch.Tensor, targets: torch.Tensor):
+        """Centers and targets on the device; a pair whose center is no row
+        gets row 0 and, unless it is ignored, a target that is no row."""
+        centers = centers.to(self.device, torch.long)
+        targets = targets.to(self.device)
+        if centers.shape != targets.shape:
+            raise ValueError(f"{list(centers.shape)} centers but "
+                             f"{list(targets.shape)} targets")
+        bad = (centers < 0) | (centers >= self.vocab_size)
+        return centers.masked_fill(bad, 0), targets.masked_fill(
+            bad & (targets != -1), self.vocab_size)
+
     def softmax_loss(self, centers: torch.Tensor, targets: torch.Tensor
                      ) -> torch.Tensor:
         """-log of the softmax probability that center word's vector (syn0)
         gives its target among all words (syn1): float32 [N], the exact form
-        of what negative sampling approximates.  Targets of -1 count 0."""
+        of what negative sampling approximates.  Targets of -1 count 0; a
+        center or another target that is no word gives NaN."""
         from .softmax import softmax_loss_forward
-        h = self.syn0[centers.to(self.device)]
+        centers, targets = self._pairs(centers, targets)
+        h = self.syn0[centers]
         return softmax_loss_forward(h[:, :self.dim], self.syn1[:, :self.dim],
-                                    targets.to(self.device))[0]
+                                    targets)[0]
 
     def train_softmax(self, centers: torch.Tensor, targets: torch.Tensor,
                       alpha: float) -> torch.Tensor:
         """One SGD step on the sum of softmax_loss over the pairs, from the
         tables as they are before it; returns the losses [N].  Exact where
         train_batch samples: every word's output row moves.  Repeated centers
-        add up, in a fixed order."""
+        add up, in a fixed order.  Pairs that are no words, as in
+        softmax_loss, move nothing."""
         from .softmax import softmax_loss_backward, softmax_loss_forward
-        centers = centers.to(self.device, torch.long)
-        targets = targets.to(self.device)
+        centers, targets = self._pairs(centers, targets)
         h = self.syn0[centers][:, :self.dim]
         w = self.syn1[:, :self.dim]
         loss, lse = softmax_loss_forward(h, w, targets)

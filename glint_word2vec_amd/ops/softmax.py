@@ -95,103 +95,117 @@ def _aligned(t: torch.Tensor) -> bool:
     return t.data_ptr() % 16 == 0 and step % 16 == 0 and step < 1 << 23
 
 
+def _workspace(device, *sizes: int) -> Tuple[torch.Tensor, list]:
+    """One allocation for parts of these many bytes, and where they start
+    (0 for a part of none); hold the tensor until the launches are made."""
+    starts, total = [], 0
+    for size in sizes:
+        starts.append(total)
+        total += _ceil(size, 256) * 256
+    held = torch.empty(total, dtype=torch.uint8, device=device)
+    base = held.data_ptr()
+    return held, [base + at if size else 0
+                  for at, size in zip(starts, sizes)]
+
+
 def _forward(h, w, targets, ignore_index, reduce: int):
-    """(loss [N], lse [N], [reduced loss, factor] or None)."""
+    """(loss [N], lse [N], reduced loss or None, its factor or None)."""
     _check(h, w, targets)
-    h, w, targets = _rows(h.detach()), _rows(w.detach()), targets.contiguous()
-    n, d = h.shape
-    v = w.shape[0]
-    loss = torch.empty(n, dtype=torch.float32, device=h.device)
+    h, w, targets = _rows(h), _rows(w), targets.contiguous()
+    (n, d), v, device = h.shape, w.shape[0], h.device
+    loss = torch.empty(n, dtype=torch.float32, device=device)
     lse = torch.empty_like(loss)
-    reduced = torch.empty(2, dtype=torch.float32, device=h.device) \
-        if reduce else None
-    size, dp = h.element_size(), _ceil(d, 64) * 64
-    packed_h = packed_w = None
+    result = factor = None
+    if reduce:      # two tensors: the result may be changed in place
+        result = torch.empty((), dtype=torch.float32, device=device)
+        factor = torch.empty_like(result)
+    size = h.element_size()
+    row = _ceil(d, 64) * 64 * size            # bytes of a packed row
     piece = v
-    if not _aligned(h):
-        packed_h = torch.empty(n * dp, dtype=h.dtype, device=h.device)
     # (the kernel for few rows streams any table)
-    if not _aligned(w) and not (n <= 16 and d * size <= 4096):
-        piece = max(256, _PACKED_BYTES // (dp * size) // 256 * 256)
-        packed_w = torch.empty(min(piece, v) * dp, dtype=w.dtype,
-                               device=w.device)
+    pack_w = not _aligned(w) and not (n <= 16 and d * size <= 4096)
+    if pack_w:
+        piece = max(256, _PACKED_BYTES // row // 256 * 256)
     # a maximum and a sum of every row for each part of the vocabulary
     parts = max(_ceil(v, piece), min(_ceil(v, 64),
                                      _PARTS // max(1, _ceil(n, 128))))
-    part = torch.empty(parts * n * 2, dtype=torch.float32, device=h.device)
+    held, (part, packed_h, packed_w) = _workspace(
+        device, parts * n * 8, 0 if _aligned(h) else n * row,
+        min(piece, v) * row if pack_w else 0)
     _native().softmax_loss(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-        int(h.dtype == torch.bfloat16), targets.data_ptr(),
-        int(targets.dtype == torch.int64), int(ignore_index),
-        part.data_ptr(), parts * n,
-        0 if packed_h is None else packed_h.data_ptr(),
-        0 if packed_w is None else packed_w.data_ptr(), piece,
-        loss.data_ptr(), lse.data_ptr(), reduce,
-        0 if reduced is None else reduced.data_ptr(), *_place(h.device))
-    return loss, lse, reduced
+        int(size == 2), targets.data_ptr(),
+        int(targets.dtype == torch.int64), ignore_index, part, parts * n,
+        packed_h, packed_w, piece, loss.data_ptr(), lse.data_ptr(), reduce,
+        0 if result is None else result.data_ptr(),
+        0 if factor is None else factor.data_ptr(), *_place(device))
+    return loss, lse, result, factor
 
 
-def _backward(h, w, targets, lse, grad, weight, ignore_index, need_h, need_w):
-    h, w, targets = _rows(h.detach()), _rows(w.detach()), targets.contiguous()
-    n, d = h.shape
-    v = w.shape[0]
-    dh = torch.empty((n, d), dtype=h.dtype, device=h.device) \
+def _backward(h, w, targets, lse, grad, factor, ignore_index, need_h, need_w):
+    h, w, targets = _rows(h), _rows(w), targets.contiguous()
+    (n, d), v, device = h.shape, w.shape[0], h.device
+    dh = torch.empty((n, d), dtype=h.dtype, device=device) \
         if need_h else None
     if n == 0 or not (need_h or need_w):
-        return dh, (torch.zeros((v, d), dtype=w.dtype, device=w.device)
+        return dh, (torch.zeros((v, d), dtype=w.dtype, device=device)
                     if need_w else None)
-    dw = torch.empty((v, d), dtype=w.dtype, device=w.device) \
+    dw = torch.empty((v, d), dtype=w.dtype, device=device) \
         if need_w else None
+    native = _native()
     size = h.element_size()
-    rows = _ceil(n, 32) * 32
-    packed = torch.empty(rows * _ceil(d, 64) * 64, dtype=h.dtype,
-                         device=h.device)
+    rows, row = _ceil(n, 32) * 32, _ceil(d, 64) * 64 * size
     # equal pieces of the vocabulary, in whole tiles
     pieces = _ceil(v, max(256, _COEF_BYTES // (rows * size)))
     width = _ceil(_ceil(v, pieces), 256) * 256
-    coef = torch.empty(rows * width, dtype=h.dtype, device=h.device)
-    packed_w = None if _aligned(w) else \
-        torch.empty(width * _ceil(d, 64) * 64, dtype=w.dtype, device=w.device)
-    ldp = _ceil(d, 4) * 4
     # parts of the long axis where a product's result has few tiles
-    splits, splits_w = _native().softmax_plan(n, min(v, width), d,
-                                              int(size == 2))
-    splits_w = splits_w if need_w else 1
-    part = torch.empty(splits * n * ldp if need_h else 0,
-                       dtype=torch.float32, device=h.device)
-    part_w = torch.empty(splits_w * width * ldp if splits_w > 1 else 0,
-                         dtype=torch.float32, device=h.device)
-    _native().softmax_grad(
+    splits, splits_w = native.softmax_plan(n, min(v, width), d, int(size == 2))
+    ldp = _ceil(d, 4) * 4
+    held, (packed, packed_w, coef, part, part_w) = _workspace(
+        device, rows * row, 0 if _aligned(w) else width * row,
+        rows * width * size, splits * n * ldp * 4 if need_h else 0,
+        splits_w * width * ldp * 4 if need_w and splits_w > 1 else 0)
+    native.softmax_grad(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-        int(h.dtype == torch.bfloat16), targets.data_ptr(),
-        int(targets.dtype == torch.int64), int(ignore_index), lse.data_ptr(),
+        int(size == 2), targets.data_ptr(),
+        int(targets.dtype == torch.int64), ignore_index, lse.data_ptr(),
         grad.data_ptr(), int(grad.dim() > 0),
-        0 if weight is None else weight.data_ptr(), packed.data_ptr(),
-        0 if packed_w is None else packed_w.data_ptr(), width,
-        coef.data_ptr(), splits, part.data_ptr() if need_h else 0, splits_w,
-        part_w.data_ptr() if splits_w > 1 else 0, ldp,
+        0 if factor is None else factor.data_ptr(), packed, packed_w, width,
+        coef, splits, part, splits_w, part_w, ldp,
         0 if dh is None else dh.data_ptr(),
-        0 if dw is None else dw.data_ptr(), *_place(h.device))
+        0 if dw is None else dw.data_ptr(), *_place(device))
     return dh, dw
+
+
+def _refuse_capture() -> None:
+    # Leaves keep one gradient node per eager graph that lives, bound to that
+    # graph's stream; a captured backward that meets one ends the process.
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            "softmax_loss with gradients cannot be captured: capture "
+            "softmax_loss_forward and softmax_loss_backward")
 
 
 class _SoftmaxLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, targets, reduce, ignore_index):
-        loss, lse, reduced = _forward(h, w, targets, ignore_index, reduce)
-        ctx.save_for_backward(h, w, targets, lse,
-                              None if reduced is None else reduced[1])
+        loss, lse, result, factor = _forward(h, w, targets, ignore_index,
+                                             reduce)
         ctx.ignore_index = ignore_index
-        return loss if reduced is None else reduced[0]
+        ctx.save_for_backward(h, w, targets, lse,
+                              *(() if factor is None else (factor,)))
+        return loss if result is None else result
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        h, w, targets, lse, weight = ctx.saved_tensors
-        dh, dw = _backward(h, w, targets, lse,
-                           grad.to(torch.float32).contiguous(), weight,
-                           ctx.ignore_index, *ctx.needs_input_grad[:2])
-        return dh, dw, None, None, None
+        _refuse_capture()
+        h, w, targets, lse, *factor = ctx.saved_tensors
+        if grad.dtype != torch.float32 or not grad.is_contiguous():
+            grad = grad.to(torch.float32).contiguous()
+        return (*_backward(h, w, targets, lse, grad,
+                           factor[0] if factor else None, ctx.ignore_index,
+                           *ctx.needs_input_grad[:2]), None, None, None)
 
 
 _REDUCE = {"none": 0, "sum": 1, "mean": 2}
@@ -209,10 +223,14 @@ def softmax_loss(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
     count nothing and give no gradient (the mean of none is NaN).  Any other
     target outside [0, V) cannot be refused without waiting for the GPU: its
     loss is NaN, and it gives no gradient.  Rows whose scores are not finite
-    give NaN."""
+    give NaN.  A call that needs gradients is refused while a graph is being
+    captured: softmax_loss_forward and softmax_loss_backward can be."""
     if reduction not in _REDUCE:
         raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got "
                          f"{reduction!r}")
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False)
+                                       for t in (h, w)):
+        _refuse_capture()
     return _SoftmaxLoss.apply(h, w, targets, _REDUCE[reduction],
                               int(ignore_index))
 
@@ -223,7 +241,8 @@ def softmax_loss_forward(h: torch.Tensor, w: torch.Tensor,
     """The loss and the log of the softmax's sum, both float32 [N], without
     autograd (evaluation, or a captured step together with
     softmax_loss_backward).  Targets as for softmax_loss."""
-    return _forward(h, w, targets, ignore_index, 0)[:2]
+    with torch.no_grad():
+        return _forward(h, w, targets, int(ignore_index), 0)[:2]
 
 
 def softmax_loss_backward(h: torch.Tensor, w: torch.Tensor,
@@ -246,6 +265,6 @@ def softmax_loss_backward(h: torch.Tensor, w: torch.Tensor,
                              f"{list(t.shape)}")
         if t.device != h.device:
             raise RuntimeError(f"{name} is on {t.device}, h on {h.device}")
-    return _backward(h, w, targets, lse.detach().contiguous(),
-                     grad.detach().contiguous(), None, ignore_index, need_h,
-                     need_w)
+    with torch.no_grad():
+        return _backward(h, w, targets, lse.contiguous(), grad.contiguous(),
+                         None, int(ignore_index), need_h, need_w)

@@ -456,3 +456,42 @@ def test_refusals_of_the_backward():
         S.softmax_loss_backward(h, w, y, lse.cpu(), one)
     with pytest.raises(RuntimeError):
         S.softmax_loss(h, w.cpu(), y)
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_loss_may_be_changed_in_place(reduction):
+    """loss /= 4 before backward(), as when gradients are accumulated: a power
+    of two, so that the gradients are a quarter to the last bit."""
+    h, w, y = _inputs(50, 400, 24, torch.float32)
+    grads = []
+    for change in (False, True):
+        a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = S.softmax_loss(a, b, y, reduction=reduction)
+        if change:
+            loss /= 4
+        loss.sum().backward()
+        grads.append((a.grad, b.grad))
+    for one, quarter in zip(*grads):
+        assert torch.equal(one / 4, quarter)
+
+
+@gpu
+def test_gradients_are_not_captured(monkeypatch):
+    h, w, y = _inputs(20, 100, 24, torch.float32)
+    a = h.clone().requires_grad_()
+    loss = S.softmax_loss(a, w, y)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            S.softmax_loss(a, w, y)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            loss.backward(retain_graph=True)
+        assert torch.equal(S.softmax_loss(h, w, y), loss.detach())
+    loss.backward()
+    assert a.grad is not None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        out = S.softmax_loss(a, w, y)
+    graph.replay()
+    assert torch.equal(out, loss.detach())

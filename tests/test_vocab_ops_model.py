@@ -96,6 +96,30 @@ def test_softmax_step_is_the_same_on_every_run():
 
 
 @gpu
+def test_pairs_that_are_no_words():
+    """They move nothing, and the other pairs as if they were not there."""
+    a, b = _tables("float32"), _tables("float32")
+    c = torch.tensor([3, -1, 300, 7, 2 ** 40, -1, 3, 9])
+    t = torch.tensor([5, 6, 7, 300, 8, -1, -1, 11])
+    want = a.softmax_loss(c[[0, 7]], t[[0, 7]])
+    for gs in (a, b):
+        got = gs.softmax_loss(c, t) if gs is a else \
+            gs.train_softmax(c, t, 0.1)
+        assert got[[1, 2, 3, 4]].isnan().all()
+        assert (got[[5, 6]] == 0).all()
+        assert torch.equal(got[[0, 7]], want)
+    good = _tables("float32")
+    good.train_softmax(c[[0, 7]], t[[0, 7]], 0.1)
+    # sums over eight pairs and over two may be cut differently: within the
+    # rounding of two products of one step
+    for x, y in ((b.syn0, good.syn0), (b.syn1, good.syn1)):
+        assert (x - y).abs().max() <= 64 * U * float(y.abs().max())
+    assert torch.equal(b.syn0[4:9:4], _tables("float32").syn0[4:9:4])
+    with pytest.raises(ValueError, match="centers"):
+        a.softmax_loss(c, t[:3])
+
+
+@gpu
 def test_step_then_loss_then_8_bit_scores():
     """The operators one after the other, as a program trains on the whole
     softmax and answers from 8 bits: each against the tables as they are."""
