@@ -55,15 +55,22 @@ constexpr float kLn2 = 0.6931471805599453f;
 // is (s - m) log2e instead: one instruction more, but it cannot overflow.
 constexpr float kFar = 1e6f;
 
-enum Type { kF32 = 0, kBF16 = 1, kFP8 = 2 };
+// kSplit is float32 in three parts of bf16, x = hi + mid + lo exactly: each
+// part is the nearest bf16 to what the ones before leave, so that mid and lo
+// are at most 2^-9 and 2^-18 of x.  Of the nine products of two such numbers
+// the six from 2^-18 up are taken; the others are 2^-26 of the product at
+// most, a quarter of float32's rounding.  Six bf16 instructions take 3/8 of
+// the time of the float32 ones for the same columns.
+enum Type { kF32 = 0, kBF16 = 1, kFP8 = 2, kSplit = 3 };
 
-// Storage of one element, and of one element as the matrix instruction takes
-// it: 8-bit rows are brought to bf16, which holds e4m3 times a power of two
-// exactly.
+// Bytes of one element (of kSplit, of one of its parts).  8-bit rows are
+// brought to bf16 for the matrix instruction, which holds e4m3 times a power of
+// two exactly.
 template <int T> struct Elem;
-template <> struct Elem<kF32> { using S = float; static constexpr int size = 4; };
-template <> struct Elem<kBF16> { using S = uint16_t; static constexpr int size = 2; };
-template <> struct Elem<kFP8> { using S = uint8_t; static constexpr int size = 1; };
+template <> struct Elem<kF32> { static constexpr int size = 4, parts = 1; };
+template <> struct Elem<kBF16> { static constexpr int size = 2, parts = 1; };
+template <> struct Elem<kFP8> { static constexpr int size = 1, parts = 1; };
+template <> struct Elem<kSplit> { static constexpr int size = 2, parts = 3; };
 
 // Rows of a matrix in global memory, all of which start at multiples of
 // `align` bytes: 16, 4 or less.
@@ -95,6 +102,29 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   v[0] = (__bf16)a;
   v[1] = (__bf16)b;
   return __builtin_bit_cast(uint32_t, v);
+}
+
+// The three parts of x.  What is not finite is all in the first.
+__device__ __forceinline__ void split(float x, float& hi, float& mid, float& lo) {
+  const uint32_t u = __float_as_uint(x);
+  const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+  hi = (float)(__bf16)x;
+  if (finite && __builtin_isinf(hi)) hi = __uint_as_float(u & 0xffff0000u);
+  const float rest = finite ? x - hi : 0.f;
+  mid = (float)(__bf16)rest;
+  lo = rest - mid;
+}
+__device__ __forceinline__ void split4(const f32x4& x, u32x2 (&to)[3]) {
+  f32x4 t[3];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float hi, mid, lo;
+    split(x[e], hi, mid, lo);
+    t[0][e] = hi, t[1][e] = mid, t[2][e] = lo;
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+    to[p] = u32x2{pack_bf16(t[p][0], t[p][1]), pack_bf16(t[p][2], t[p][3])};
 }
 
 // 16 bytes of a row from byte `o` on; zeros outside of the matrix.
@@ -184,6 +214,18 @@ template <int T, int N>
 __device__ __forceinline__ void mma_row(u32x4 a, const u32x4 (&b)[N], f32x4 (&c)[N]) {
   const u32x4 a1[1] = {a};
   mma_all<T>(a1, b, reinterpret_cast<f32x4(&)[1][N]>(c));
+}
+
+// The six products of two sides in three parts, small ones first.
+template <int M, int N>
+__device__ __forceinline__ void mma_split(const u32x4 (&a)[3][M], const u32x4 (&b)[3][N],
+                                          f32x4 (&c)[M][N]) {
+  mma_all<kBF16>(a[2], b[0], c);
+  mma_all<kBF16>(a[0], b[2], c);
+  mma_all<kBF16>(a[1], b[1], c);
+  mma_all<kBF16>(a[1], b[0], c);
+  mma_all<kBF16>(a[0], b[1], c);
+  mma_all<kBF16>(a[0], b[0], c);
 }
 
 // ---------------------------------------------------------------------------
@@ -353,15 +395,20 @@ struct Sink {
   __device__ __forceinline__ void take_coef(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1,
                                             int n1, bool cut, bool met) {
     const int lane = threadIdx.x & 63;
-    // 16 samples x 16 table rows are 512 bytes (1 KB) in one piece, as a wave
-    // writes them and with every 16 bytes of one sample, as the products read
+    // 16 samples x 16 table rows are 512 bytes (float32: 1 KB, or three times
+    // 512 bytes of its parts) in one piece, as a wave writes them and with every 16 bytes of one sample, as the products read
     // them
-    constexpr int es = TC == kF32 ? 4 : 2;
+    constexpr int es = TC == kF32 ? 4 : 2, parts = Elem<TC>::parts;
     const int in_block = (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
     auto put = [&](int i, int j, f32x4 c) {
-      char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es);
+      char* to = a.coef + (((n1 >> 4) + j) * (a.ldc >> 4) + (v1 >> 4) + i) * (256 * es * parts);
       to += in_block;
-      if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
+      if constexpr (TC == kSplit) {
+        u32x2 t[3];
+        split4(c, t);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(to + p * 512) = t[p];
+      } else if constexpr (TC == kF32) *reinterpret_cast<f32x4*>(to) = c;
       else *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16(c[0], c[1]), pack_bf16(c[2], c[3])};
     };
 #pragma unroll
@@ -671,9 +718,8 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
       if (a.col_scale)
 #pragma unroll
         for (int i = 0; i < kRows; i += 64)
-          if (kRows >= 64)
-            load_lds4((const char*)(a.col_scale + v0), (uint32_t)min(from + i, last) * 4,
-                      lds_address(&col[buf][i]));
+          load_lds4((const char*)(a.col_scale + v0), (uint32_t)min(from + i, last) * 4,
+                    lds_address(&col[buf][i]));
     const uint32_t to = lds_address(&lds[buf][wave * (kRows / 4) * kPitch]);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -771,12 +817,14 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 // rows start at multiples of 16 bytes; 8-bit table rows are converted when
 // they are read from LDS, and their scales lie by block of columns, then row.
 template <int TW, int TC, int USE, int WV, int WN, int NS>
-__global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2) void tile_kernel(ScoreArgs a) {
   // float32 steps are long: two ahead do, and three workgroups fit a CU
-  constexpr int kWaves = WV * WN, kAhead = TC == kF32 ? 2 : 3, MR = 4;
+  constexpr int kWaves = WV * WN, MR = 4, P = Elem<TC>::parts;
+  constexpr int kAhead = TC == kSplit ? 1 : TC == kF32 ? 2 : 3;
   constexpr int kV = 64 * WV, kN = 16 * NS * WN;
-  constexpr int kWideW = TW == kFP8 ? 32 : 64, kWideH = 64;   // bytes per step
-  constexpr int kBytesW = kV * kWideW, kBytesH = kN * kWideH;
+  constexpr int kWideW = TW == kFP8 ? 32 : 64, kWideH = 64;   // bytes per step and part
+  constexpr int kPartW = kV * kWideW, kPartH = kN * kWideH;
+  constexpr int kBytesW = kPartW * P, kBytesH = kPartH * P;
   constexpr int kBytesS = TW == kFP8 ? kV : 0;
   constexpr int kInstr = (kBytesW + kBytesH) / 1024;          // loads of a whole wave
   constexpr int kEach = kInstr / kWaves, kMore = kInstr % kWaves;
@@ -805,7 +853,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   auto fetch = [&](int buf) {
     const int v0 = a.v_begin + fetch_tile * kV;
     const int last_w = min(kV - 1, (int)a.w.rows - 1 - v0);
-    const int ow = fetch_step * kWideW, oh = fetch_step * kWideH;
+    const int ow = fetch_step * (kWideW * P), oh = fetch_step * (kWideH * P);
     const char* bw = a.w.p + v0 * a.w.ld + ow;
     const char* bh = a.h.p + n0 * a.h.ld + oh;
     const int end_w = ((a.w.kb - 1) & ~15) - ow, end_h = ((a.h.kb - 1) & ~15) - oh;
@@ -813,15 +861,18 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
     for (int i = 0; i < kEach + (kMore > 0); ++i) {
       const int q = wave + kWaves * i;
       if (q * 1024 < kBytesW) {
-        const int p = q * 64 + lane;
+        const int part = q / (kPartW / 1024), p = (q - part * (kPartW / 1024)) * 64 + lane;
         const int r = TW == kFP8 ? p >> 1 : p >> 2;
         const int c = TW == kFP8 ? p & 1 : row_chunk(64, r, p & 3);
-        load_lds16(bw, (uint32_t)(min(r, last_w) * (int)a.w.ld + min(c * 16, end_w)),
+        const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, end_w);
+        load_lds16(bw, (uint32_t)(min(r, last_w) * (int)a.w.ld + at),
                    lds_address(&lds[buf][q * 1024]));
       } else if (q < kInstr) {
-        const int p = (q - kBytesW / 1024) * 64 + lane;
+        const int q1 = q - kBytesW / 1024;
+        const int part = q1 / (kPartH / 1024), p = (q1 - part * (kPartH / 1024)) * 64 + lane;
         const int r = p >> 2, c = row_chunk(64, r, p & 3);
-        load_lds16(bh, (uint32_t)(min(r, last_h) * (int)a.h.ld + min(c * 16, end_h)),
+        const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, end_h);
+        load_lds16(bh, (uint32_t)(min(r, last_h) * (int)a.h.ld + at),
                    lds_address(&lds[buf][q * 1024]));
       }
     }
@@ -861,34 +912,48 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
     at_buf = at_buf == kAhead ? 0 : at_buf + 1;
     const char* lh = buf + kBytesW + wn * (16 * NS) * kWideH;
     const int at = r16 * 64 + row_chunk(64, r16, g) * 16;
-    u32x4 fa[MR], fb[NS];
+    if constexpr (P > 1) {
+      u32x4 fa[P][MR], fb[P][NS];
 #pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      if constexpr (TW == kFP8) {
-        const int r = wv * 64 + i * 16 + r16;
-        const u32x2 q = *reinterpret_cast<const u32x2*>(buf + r * 32 + g * 8);
-        const uint8_t e = *reinterpret_cast<const uint8_t*>(buf + kBytesW + kBytesH + r);
-        fa[i] = fp8x8_to_bf16(q[0], q[1], scale_of(e));
-      } else {
-        fa[i] = *reinterpret_cast<const u32x4*>(buf + (wv * 64 + i * 16) * 64 + at);
+      for (int p = P - 1; p >= 0; --p) {
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+          fa[p][i] = *reinterpret_cast<const u32x4*>(buf + p * kPartW + (wv * 64 + i * 16) * 64 + at);
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+          fb[p][j] = *reinterpret_cast<const u32x4*>(lh + p * kPartH + j * 16 * 64 + at);
       }
-    }
+      mma_split(fa, fb, acc);
+    } else {
+      u32x4 fa[MR], fb[NS];
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
-      fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64 + at);
-    if (step + 1 == steps && (a.h.kb & 63) != 0) {
-      // columns past the last one, whatever they hold
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
-        const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
-#pragma unroll
-        for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
+      for (int i = 0; i < MR; ++i) {
+        if constexpr (TW == kFP8) {
+          const int r = wv * 64 + i * 16 + r16;
+          const u32x2 q = *reinterpret_cast<const u32x2*>(buf + r * 32 + g * 8);
+          const uint8_t e = *reinterpret_cast<const uint8_t*>(buf + kBytesW + kBytesH + r);
+          fa[i] = fp8x8_to_bf16(q[0], q[1], scale_of(e));
+        } else {
+          fa[i] = *reinterpret_cast<const u32x4*>(buf + (wv * 64 + i * 16) * 64 + at);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < NS; ++j)
+        fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64 + at);
+      if (step + 1 == steps && (a.h.kb & 63) != 0) {
+        // columns past the last one, whatever they hold
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
+          const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+#pragma unroll
+          for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
+#pragma unroll
+          for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
+        }
+      }
+      mma_all<TC>(fa, fb, acc);
     }
-    mma_all<TC>(fa, fb, acc);
     if (++step == steps) {
       const int v = a.v_begin + tile * kV + wv * 64 + 4 * g;
       if (USE == kStore && a.col_scale)
@@ -1110,6 +1175,34 @@ struct GradArgs {
   int64_t ldo;
 };
 
+// Rows in parts of bf16: for each 32 columns 64 bytes of each part, and zeros
+// as in pack_kernel.  A thread takes 8 columns.
+__global__ __launch_bounds__(256) void split_kernel(
+    Rows h, const void* targets, int targets64, int64_t ignore, int64_t vocab, char* out,
+    int64_t rows, int ldo) {
+  const int chunks = ldo / 8;
+  const int64_t total = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int c = (int)(i - r * chunks);
+    u32x4 v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (r < h.rows) {
+      const int64_t y = targets ? target_of(targets, targets64, r) : 0;
+      if (!targets || (y != ignore && y >= 0 && y < vocab))
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[k] = load16<4>(h, r, c * 32 + 16 * k);
+    }
+    u32x2 t[2][3];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) split4(__builtin_bit_cast(f32x4, v[k]), t[k]);
+    char* to = out + r * ldo * 6 + (c >> 2) * 192 + (c & 3) * 16;
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<u32x4*>(to + p * 64) = u32x4{t[0][p][0], t[0][p][1], t[1][p][0], t[1][p][1]};
+  }
+}
+
 // Rows for the gradient: [rows][ldo] of 16-byte multiples with zeros behind
 // the last column and row, and (with targets) in rows that have no loss,
 // whatever they hold: a coefficient of 0 would not hide a NaN.
@@ -1142,16 +1235,17 @@ __global__ __launch_bounds__(256) void pack_kernel(
 // workgroups a CU do more.
 template <int T, bool DW, int ND, int WR, int J, int kAhead>
 __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
-  constexpr int ES = Elem<T>::size, WD = 8 / WR;
+  constexpr int ES = Elem<T>::size, P = Elem<T>::parts, WD = 8 / WR;
   constexpr int kRowsR = 16 * J * WR, kCols = 16 * ND * WD, kStep = 64 / ES;
   constexpr int kPitchX = kCols * ES, kPitchB = kRowsR * ES;     // bytes of a row k
   constexpr int kChunksX = kPitchX / 16, kChunksB = kPitchB / 16;
-  constexpr int kBytesX = kStep * kPitchX, kBytesB = kStep * kPitchB;
+  constexpr int kPartX = kStep * kPitchX, kPartB = kStep * kPitchB;
+  constexpr int kBytesX = kPartX * P, kBytesB = kPartB * P;
   constexpr int kInstr = (kBytesX + kBytesB) / 1024;             // loads of a whole wave
   constexpr int kEach = kInstr / 8, kMore = kInstr % 8;          // kMore waves have one more
-  constexpr int kBlock = 256 * ES;                   // bytes of 16 x 16 coefficients
+  constexpr int kBlock = 256 * ES * P;               // bytes of 16 x 16 coefficients
   constexpr int kLine = 16 * ES;                     // of which one sample's
-  static_assert(kBytesX % 1024 == 0 && kBytesB % 1024 == 0, "");
+  static_assert(kPartX % 1024 == 0 && kPartB % 1024 == 0, "");
   static_assert(!DW || (WR == 4 && J == 4), "");
   __shared__ __align__(16) char lds[kAhead + 1][kBytesX + kBytesB];
   const int lane = threadIdx.x & 63;
@@ -1182,25 +1276,26 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   // waits below count the loads of each wave.  Columns d and rows r past the
   // end are not stored; past the last k, one side is zeros.
   const int have_x = (a.x.kb - d0 * ES + 15) / 16;   // chunks of x from d0 on
-  const int64_t block_row = a.ldc * kLine;           // 16 samples' coefficients
+  const int64_t block_row = a.ldc * (kLine * P);     // 16 samples' coefficients
   const int have_b = (int)min((int64_t)(DW ? kChunksB : kRowsR),
                               DW ? ((a.r - r0) * ES + 15) / 16 : a.r - r0);
   auto fetch = [&](int s) {
     char* buf = lds[(s - s0) % (kAhead + 1)];
     const int64_t k0 = (int64_t)s * kStep;
-    const char* xb = a.x.p + k0 * a.x.ld + d0 * ES;
+    const char* xb = a.x.p + k0 * a.x.ld + d0 * (ES * P);
     const int last = (int)min((int64_t)kStep - 1, a.x.rows - 1 - k0);
 #pragma unroll
     for (int i = 0; i < kEach + (kMore > 0); ++i) {
       const int q = wave + 8 * i;
       if (q * 1024 < kBytesX) {
-        const int p = q * 64 + lane;
+        const int part = q / (kPartX / 1024), p = (q - part * (kPartX / 1024)) * 64 + lane;
         const int k = p / kChunksX, pos = p % kChunksX;
-        const int c = ((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer;
-        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + min(c, have_x - 1) * 16),
-                   lds_address(buf + q * 1024));
+        const int c = min(((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer, have_x - 1);
+        const int in = P > 1 ? (c >> 2) * 192 + part * 64 + (c & 3) * 16 : c * 16;
+        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + in), lds_address(buf + q * 1024));
       } else if (q < kInstr) {
-        const int p = (q - kBytesX / 1024) * 64 + lane;
+        const int q1 = q - kBytesX / 1024;
+        const int part = q1 / (kPartB / 1024), p = (q1 - part * (kPartB / 1024)) * 64 + lane;
         const char* from;
         uint32_t offset;
         if constexpr (DW) {
@@ -1209,14 +1304,14 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
           const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
           const int in = min(c, have_b - 1);
           from = a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock;
-          offset = (uint32_t)(k >> 4) * (uint32_t)block_row + (k & 15) * kLine +
+          offset = (uint32_t)(k >> 4) * (uint32_t)block_row + part * 512 + (k & 15) * kLine +
                    in / kPer * kBlock + in % kPer * 16;
         } else {
           // 64 bytes of samples r
           const int r = p >> 2, c = row_chunk(64, r, p & 3);
           const int in = min(r, have_b - 1);
           from = a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock;
-          offset = (uint32_t)(in >> 4) * (uint32_t)block_row + (in & 15) * kLine +
+          offset = (uint32_t)(in >> 4) * (uint32_t)block_row + part * 512 + (in & 15) * kLine +
                    c / kPer * kBlock + c % kPer * 16;
         }
         load_lds16(from, offset, lds_address(buf + q * 1024));
@@ -1235,7 +1330,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   // 16 columns x one step of k: for bf16 by transposing reads, in which 16
   // lanes take 4 rows k of one block; for float32 a word at a time
   auto columns = [&](const char* p, int pitch, int block) {
-    if constexpr (T == kBF16) {
+    if constexpr (T != kF32) {
       const int k = 8 * g + (r16 >> 2);
       const char* q = p + k * pitch + ((block ^ key(k, pitch)) << 5) + (r16 & 3) * 8;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
@@ -1262,20 +1357,31 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
     if (s + kAhead < s1) fetch(s + kAhead);
     const char* x = lds[(s - s0) % (kAhead + 1)];
     const char* b = x + kBytesX;
-    u32x4 fb[J];
+    u32x4 fb[P][J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      if constexpr (DW) {
-        fb[j] = columns(b, kPitchB, wr * J + j);
-      } else {
-        const int r = (wr * J + j) * 16 + r16;
-        fb[j] = *reinterpret_cast<const u32x4*>(b + r * 64 + row_chunk(64, r, g) * 16);
+    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if constexpr (DW) {
+          fb[p][j] = columns(b + p * kPartB, kPitchB, wr * J + j);
+        } else {
+          const int r = (wr * J + j) * 16 + r16;
+          fb[p][j] = *reinterpret_cast<const u32x4*>(b + p * kPartB + r * 64 +
+                                                     row_chunk(64, r, g) * 16);
+        }
       }
-    }
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      const u32x4 fa = columns(x, kPitchX, wd * ND + i);
-      mma_row<T>(fa, fb, acc[i]);
+      if constexpr (P > 1) {
+        u32x4 fa[P][1];
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p)
+          fa[p][0] = columns(x + p * kPartX, kPitchX, wd * ND + i);
+        mma_split(fa, fb, reinterpret_cast<f32x4(&)[1][J]>(acc[i]));
+      } else {
+        const u32x4 fa = columns(x, kPitchX, wd * ND + i);
+        mma_row<T>(fa, fb[0], acc[i]);
+      }
     }
   }
   const float scale = a.part ? 1.f : scale_by(a.scale[0], a.scale[1]);
@@ -1291,7 +1397,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
       if (a.part) {
         f32x4* o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.r + r) * a.ldp + d);
         *o = a.add ? *o + acc[i][j] : acc[i][j];
-      } else if constexpr (T == kF32) {
+      } else if constexpr (T != kBF16) {
         float* o = reinterpret_cast<float*>(a.out) + r * a.ldo + d;
         if ((a.ldo & 3) == 0) {       // then d + 3 < ldo as well
           *reinterpret_cast<f32x4*>(o) = acc[i][j];
@@ -1612,14 +1718,20 @@ template <int TW, int TC, int USE>
 static void launch_tile(ScoreArgs& a, hipStream_t stream) {
   for (const Rows* r : {&a.w, &a.h})
     if (r->align != 16 || r->ld >= (1 << 23)) throw std::runtime_error("rows not aligned");
-  const int64_t rows = a.v_end - a.v_begin;
-  if (TW == kFP8 || a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
-  // 128 x 128 fills the card more evenly; bf16 is bound by LDS there, and takes
-  // 256 x 256 where there are enough of them
-  if constexpr (TW != kFP8)
-    if (TC == kF32 || ((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
-      return launch_tile_k<TW, TC, USE, 2, 2, 4>(a, stream);
-  if constexpr (TW == kBF16) launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
+  if constexpr (TW == kSplit) {
+    // eight waves of 64 x 64; four of 64 x 128 read less from LDS, but leave
+    // one a SIMD (20000 x 8000 x 256: 425 us, with four 483)
+    launch_tile_k<TW, TC, USE, 4, 2, 4>(a, stream);
+  } else {
+    if (TW == kFP8 || a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
+    // 128 x 128 fills the card more evenly; bf16 is bound by LDS there, and
+    // takes 256 x 256 where there are enough of them
+    const int64_t rows = a.v_end - a.v_begin;
+    if constexpr (TW != kFP8)
+      if (TC == kF32 || ((rows + 255) / 256) * ((a.n + 255) / 256) < 256)
+        return launch_tile_k<TW, TC, USE, 2, 2, 4>(a, stream);
+    if constexpr (TW == kBF16) launch_tile_k<TW, TC, USE, 4, 2, 8>(a, stream);
+  }
 }
 
 // LDS that the samples of the streaming kernel take; 4 KB at least, for the
@@ -1645,7 +1757,7 @@ static void launch_any(ScoreArgs& a, int64_t cols, hipStream_t stream) {
   constexpr bool fp8 = TW == kFP8;
   if constexpr (TC == kBF16)
     if (is_resident(a, cols)) return launch_resident<USE, fp8>(a, cols, stream);
-  if constexpr (USE != kCoef)
+  if constexpr (USE != kCoef && TC != kSplit)
     if (a.n <= 16 && stream_bytes(a, 1, fp8) <= kMostStream)
       return launch_stream<TW, TC, 1, USE>(a, stream);
   if constexpr (fp8) throw std::runtime_error("no workspace for the scales");
@@ -1653,12 +1765,15 @@ static void launch_any(ScoreArgs& a, int64_t cols, hipStream_t stream) {
 }
 
 // rows [np][dp] at `to`, see pack_kernel
-static Rows pack(const Rows& r, int is_bf16, const void* targets, int targets64, int64_t ignore,
+static Rows pack(const Rows& r, int type, const void* targets, int targets64, int64_t ignore,
                  int64_t vocab, uintptr_t to, int64_t np, int64_t dp, hipStream_t stream) {
-  const int es = is_bf16 ? 2 : 4;
+  const int es = type == kBF16 ? 2 : type == kF32 ? 4 : 6;
   if (to % 16 != 0) throw std::runtime_error("no workspace for rows");
-  const int blocks = (int)std::min<int64_t>((np * dp * es / 16 + 255) / 256, 8192);
-  if (is_bf16) pack_kernel<kBF16><<<blocks, 256, 0, stream>>>(
+  const int each = type == kSplit ? 8 : 16 / es;
+  const int blocks = (int)std::min<int64_t>((np * dp / each + 255) / 256, 8192);
+  if (type == kBF16) pack_kernel<kBF16><<<blocks, 256, 0, stream>>>(
+      r, targets, targets64, ignore, vocab, (char*)to, np, (int)dp);
+  else if (type == kSplit) split_kernel<<<blocks, 256, 0, stream>>>(
       r, targets, targets64, ignore, vocab, (char*)to, np, (int)dp);
   else pack_kernel<kF32><<<blocks, 256, 0, stream>>>(
       r, targets, targets64, ignore, vocab, (char*)to, np, (int)dp);
@@ -1667,6 +1782,7 @@ static Rows pack(const Rows& r, int is_bf16, const void* targets, int targets64,
   packed.ld = dp * es;
   packed.rows = np;
   packed.align = 16;
+  if (type == kSplit) packed.kb = (int)dp * 2;
   return packed;
 }
 
@@ -1675,15 +1791,15 @@ static Rows pack(const Rows& r, int is_bf16, const void* targets, int targets64,
 // rows can be read as they lie: they start at multiples of 16 bytes and less
 // than 2^23 bytes apart, or the streaming kernel takes them.
 static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
-                         int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
+                         int64_t v, int64_t d, int type, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t part, int64_t part_size, uintptr_t packed_h,
                          uintptr_t packed_w, int64_t piece, uintptr_t loss, uintptr_t lse,
                          int reduce, uintptr_t result, uintptr_t factor, int device,
                          uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
-  const int es = is_bf16 ? 2 : 4;
-  const int64_t dp = (d + 63) / 64 * 64;
+  const int es = type == kBF16 ? 2 : 4;
+  const int64_t dp = type == kSplit ? (d + 31) / 32 * 32 : (d + 63) / 64 * 64;
   if (n > 0) {
     const Rows rw = make_rows(w, ldw, v, d, es), rh = make_rows(h, ldh, n, d, es);
     ScoreArgs a{};
@@ -1691,8 +1807,10 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.h = rh;
     a.ldp = n;
     const bool pack_w = packed_w != 0;
+    if (type == kSplit && !(packed_h && packed_w))
+      throw std::runtime_error("no workspace for rows");
     if (packed_h)
-      a.h = pack(rh, is_bf16, nullptr, 0, 0, 0, packed_h, n, dp, stream);
+      a.h = pack(rh, type, nullptr, 0, 0, 0, packed_h, n, dp, stream);
     if (!pack_w) piece = v;
     const int64_t pieces = (v + piece - 1) / piece;
     int parts = 0;
@@ -1700,18 +1818,19 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       const int64_t v1 = std::min(v, v0 + piece);
       a.w = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
       if (pack_w)
-        a.w = pack(a.w, is_bf16, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
+        a.w = pack(a.w, type, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
       a.v_begin = 0;
       a.v_end = (int)(v1 - v0);
       a.part = (float2*)part + parts * n;
       a.splits = (int)std::min<int64_t>(1 << 20, part_size / n / pieces);
       if (a.splits < 1) throw std::runtime_error("workspace too small");
-      if (is_bf16) launch_any<kBF16, kBF16, kLoss>(a, d, stream);
+      if (type == kBF16) launch_any<kBF16, kBF16, kLoss>(a, d, stream);
+      else if (type == kSplit) launch_any<kSplit, kSplit, kLoss>(a, d, stream);
       else launch_any<kF32, kF32, kLoss>(a, d, stream);
       parts += a.splits;
     }
     const int joins = grid_of((n + 3) / 4);
-    if (is_bf16)
+    if (type == kBF16)
       loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(rw, rh, (const float2*)part, parts, n,
           (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
     else
@@ -1746,13 +1865,20 @@ struct GradForm {
   int slots;      // workgroups that the card holds at a time
 };
 
-static GradForm grad_form(bool bf16, bool dw, int64_t r, int64_t k, int d) {
+static GradForm grad_form(int type, bool dw, int64_t r, int64_t k, int d) {
   GradForm f{256, 0, 0, 256};
   int wd = 2, most = 10, step = 2;    // waves along d, blocks of 16 columns a wave
+  if (type == kSplit) {
+    // 256 x 128: two steps of that fit LDS
+    const int columns = (d + 31) / 32;
+    f.tiles_d = (columns + 3) / 4;
+    f.nd = (columns + f.tiles_d - 1) / f.tiles_d <= 2 ? 2 : 4;
+    return f;
+  }
   if (!dw && r <= 32) f.rows = 32, wd = 8, most = 3, step = 1, f.slots = 512;
   else if (!dw && r <= 128) f.rows = 128, wd = 4, most = 5, step = 1, f.slots = 512;
   else if (dw && k <= 128) f.rows = 0, most = 4, f.slots = 768;
-  if (f.rows == 0 || (f.rows == 256 && bf16)) {
+  if (f.rows == 0 || (f.rows == 256 && type == kBF16)) {
     // bound by LDS or by what is written: the fewest tiles
     f.tiles_d = (d + 16 * wd * most - 1) / (16 * wd * most);
     f.nd = ((d + f.tiles_d - 1) / f.tiles_d + 63) / 64 * 2;
@@ -1787,9 +1913,9 @@ static int grad_parts(int64_t tiles, int slots, int64_t most) {
 }
 
 // (parts of the vocabulary's pieces for dh, parts of the samples for dw)
-static std::pair<int, int> softmax_plan(int64_t n, int64_t chunk, int64_t d, int is_bf16) {
-  const GradForm h = grad_form(is_bf16, false, n, chunk, (int)d);
-  const GradForm w = grad_form(is_bf16, true, chunk, n, (int)d);
+static std::pair<int, int> softmax_plan(int64_t n, int64_t chunk, int64_t d, int type) {
+  const GradForm h = grad_form(type, false, n, chunk, (int)d);
+  const GradForm w = grad_form(type, true, chunk, n, (int)d);
   const int rows_w = w.rows ? w.rows : 256;
   const int64_t tiles_h = (n + h.rows - 1) / h.rows * h.tiles_d;
   const int64_t tiles_w = (chunk + rows_w - 1) / rows_w * w.tiles_d;
@@ -1808,20 +1934,24 @@ static void launch_grad_k(GradArgs& b, hipStream_t stream) {
 
 template <int T, bool DW>
 static void launch_grad(GradArgs b, hipStream_t stream) {
-  const GradForm f = grad_form(T == kBF16, DW, b.r, b.k, b.d);
+  const GradForm f = grad_form(T, DW, b.r, b.k, b.d);
   b.tiles_d = f.tiles_d;
 #define CASE_ND(R, N, WR, J, A) \
   if (f.rows == R && f.nd == N) return launch_grad_k<T, DW, N, WR, J, A>(b, stream);
-  if constexpr (DW) {
+  if constexpr (T == kSplit) {
+    CASE_ND(256, 2, 4, 4, 1) CASE_ND(256, 4, 4, 4, 1)
+  } else if constexpr (DW) {
     CASE_ND(0, 2, 4, 4, 1) CASE_ND(0, 4, 4, 4, 1)
   } else {
     CASE_ND(32, 1, 1, 2, 3) CASE_ND(32, 2, 1, 2, 3) CASE_ND(32, 3, 1, 2, 3)
     CASE_ND(128, 1, 2, 4, 3) CASE_ND(128, 2, 2, 4, 3) CASE_ND(128, 3, 2, 4, 3)
     CASE_ND(128, 4, 2, 4, 3) CASE_ND(128, 5, 2, 4, 3)
   }
-  constexpr int kAhead = T == kF32 ? 2 : 3;
-  CASE_ND(256, 2, 4, 4, kAhead) CASE_ND(256, 4, 4, 4, kAhead) CASE_ND(256, 6, 4, 4, kAhead)
-  CASE_ND(256, 8, 4, 4, kAhead) CASE_ND(256, 10, 4, 4, kAhead)
+  if constexpr (T != kSplit) {
+    constexpr int kAhead = T == kF32 ? 2 : 3;
+    CASE_ND(256, 2, 4, 4, kAhead) CASE_ND(256, 4, 4, 4, kAhead) CASE_ND(256, 6, 4, 4, kAhead)
+    CASE_ND(256, 8, 4, 4, kAhead) CASE_ND(256, 10, 4, 4, kAhead)
+  }
 #undef CASE_ND
   throw std::runtime_error("no kernel for these columns");
 }
@@ -1831,7 +1961,7 @@ static void launch_grad(GradArgs b, hipStream_t stream) {
 // bytes and less than 2^23 bytes apart; coef: [np][chunk] elements; part:
 // [splits][n][ldp] floats; part_w: [splits_w][chunk][ldp] where splits_w > 1
 static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64_t ldw,
-                         int64_t v, int64_t d, int is_bf16, uintptr_t targets, int targets64,
+                         int64_t v, int64_t d, int type, uintptr_t targets, int targets64,
                          int64_t ignore, uintptr_t lse, uintptr_t grad, int grad_step,
                          uintptr_t weight, uintptr_t packed, uintptr_t packed_w, int64_t chunk,
                          uintptr_t coef, int splits, uintptr_t part, int splits_w,
@@ -1839,15 +1969,18 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
                          uintptr_t stream_ptr) {
   const OnDevice on(device);
   hipStream_t stream = (hipStream_t)stream_ptr;
+  const bool is_bf16 = type == kBF16;
   const int es = is_bf16 ? 2 : 4;
   if (chunk % 256 != 0 || ldp % 4 != 0 || coef % 16 != 0)
     throw std::runtime_error("bad workspace shape");
   if (n == 0) throw std::runtime_error("no rows");
-  const int64_t np = (n + 31) / 32 * 32, dp = (d + 63) / 64 * 64;
+  const int64_t np = (n + 31) / 32 * 32;
+  const int64_t dp = type == kSplit ? (d + 31) / 32 * 32 : (d + 63) / 64 * 64;
   const Rows rw = make_rows(w, ldw, v, d, es);
-  const Rows rh = pack(make_rows(h, ldh, n, d, es), is_bf16, (const void*)targets, targets64,
+  const Rows rh = pack(make_rows(h, ldh, n, d, es), type, (const void*)targets, targets64,
                        ignore, v, packed, np, dp, stream);
   const bool pack_w = packed_w != 0;
+  if (type == kSplit && !pack_w) throw std::runtime_error("no workspace for rows");
   // One gradient for all samples stays out of the coefficients: in bf16 it
   // would round all of them by the same 2^-9 or less.
   const float* const scale[2] = {grad_step ? nullptr : (const float*)grad,
@@ -1857,7 +1990,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     // the table's rows from v0 on; v_begin and the targets count from row 0
     Rows piece = make_rows(w + v0 * ldw * es, ldw, v1 - v0, d, es);
     if (pack_w)
-      piece = pack(piece, is_bf16, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
+      piece = pack(piece, type, nullptr, 0, 0, 0, packed_w, v1 - v0, dp, stream);
     ScoreArgs a{};
     a.w = piece;
     a.w.p -= v0 * a.w.ld;
@@ -1877,6 +2010,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
     a.coef_rows = np;
     a.ldc = chunk;
     if (is_bf16) launch_any<kBF16, kBF16, kCoef>(a, d, stream);
+    else if (type == kSplit) launch_any<kSplit, kSplit, kCoef>(a, d, stream);
     else launch_any<kF32, kF32, kCoef>(a, d, stream);
     GradArgs b{};
     b.coef = (const char*)coef;
@@ -1893,6 +2027,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.part = (float*)part;
       b.add = v0 > 0;
       if (is_bf16) launch_grad<kBF16, false>(b, stream);
+      else if (type == kSplit) launch_grad<kSplit, false>(b, stream);
       else launch_grad<kF32, false>(b, stream);
     }
     if (dw) {
@@ -1905,6 +2040,7 @@ static void softmax_grad(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       b.out = (char*)dw + v0 * d * es;
       b.ldo = d;
       if (is_bf16) launch_grad<kBF16, true>(b, stream);
+      else if (type == kSplit) launch_grad<kSplit, true>(b, stream);
       else launch_grad<kF32, true>(b, stream);
       if (splits_w > 1)
         launch_sum_parts(b.part, splits_w, v1 - v0, ldp, d, scale, is_bf16, b.out, stream);

@@ -137,6 +137,8 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
     n = b.shape[0]
     if b.shape[1] != k:
         raise ValueError(f"a has {k} columns, b has {b.shape[1]}")
+    if k > 1 << 20:
+        raise ValueError("at most 2^20 columns")
     if a.device != b.device:
         raise RuntimeError(f"a is on {a.device}, b on {b.device}")
     if out_dtype not in (torch.float32, torch.bfloat16):

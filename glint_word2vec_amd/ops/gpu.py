@@ -315,7 +315,7 @@ class GpuSgns:
         centers, targets = self._pairs(centers, targets)
         h = self.syn0[centers][:, :self.dim]
         w = self.syn1[:, :self.dim]
-        loss, lse = softmax_loss_forward(h, w, targets)
+        loss, lse = softmax_loss_forward(h, w, targets, gradient=True)
         step = torch.full((), -float(alpha), device=self.device)
         dh, dw = softmax_loss_backward(h, w, targets, lse, step)
         w.add_(dw)

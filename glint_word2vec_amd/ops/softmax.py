@@ -78,8 +78,8 @@ def _check(h, w, targets) -> None:
         raise TypeError(f"h is {h.dtype} but w is {w.dtype}")
     if targets.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
-    if max(h.shape[0], w.shape[0]) > 2 ** 31 - 1024 or w.shape[1] > 1 << 24:
-        raise ValueError("at most 2^31 - 1024 rows of 2^24 columns")
+    if max(h.shape[0], w.shape[0]) > 2 ** 31 - 1024 or w.shape[1] > 1 << 20:
+        raise ValueError("at most 2^31 - 1024 rows of 2^20 columns")
     if not (h.is_cuda and w.is_cuda and targets.is_cuda):
         raise RuntimeError("the softmax kernels run on the GPU: move h, w and "
                            "targets there")
@@ -95,6 +95,41 @@ def _aligned(t: torch.Tensor) -> bool:
     return t.data_ptr() % 16 == 0 and step % 16 == 0 and step < 1 << 23
 
 
+# How the kernels take the numbers, and bytes of one: float32, bfloat16, and
+# float32 in three parts of bfloat16 (see kSplit in the kernels' source).
+_FLOAT, _BF16, _SPLIT = 0, 1, 3
+_BYTES = {_FLOAT: 4, _BF16: 2, _SPLIT: 6}
+# float32 goes in parts from so many samples and products on; see _kind
+_SPLIT_LOSS = 384, 1 << 31
+_SPLIT_GRAD = 192, 0
+_SPLIT_COEF_BYTES = 256 << 20
+
+
+def _kind(h: torch.Tensor, v: int, grad: bool) -> int:
+    """How this call takes its numbers: with `grad` for a gradient and the lse
+    that it starts from.  A coefficient exp(s - lse) is exact to a part of the
+    score's own error, as its score and those in lse were rounded alike; an lse
+    of the other form costs that (285 x 95 x 588: 1.6e-6 instead of 5e-7 of
+    the gradient).  In parts the products run faster, but
+    the table is written once more and the coefficients take half as much
+    again.  Times in float32 and in parts (us):
+      loss, d = 200: 512 x 30000 71 and 63, 4096 x 30000 438 and 300;
+        256 x 200000 202 and 252, 1024 x 4000 28 and 37
+      gradient, d = 200: 256 x 4000 95 and 81, 1024 x 30000 460 and 292;
+        128 x 200000 402 and 484
+      gradient, d = 64: 1024 x 30000 166 and 153; 512 x 200000 438 and 556,
+        whose coefficients are past the cache"""
+    if h.dtype == torch.bfloat16:
+        return _BF16
+    n, d = h.shape
+    rows, products = _SPLIT_GRAD if grad else _SPLIT_LOSS
+    if n < rows or n * v * d < products:
+        return _FLOAT
+    if grad and d < 96 and n * v * _BYTES[_SPLIT] > _SPLIT_COEF_BYTES:
+        return _FLOAT
+    return _SPLIT
+
+
 def _workspace(device, *sizes: int) -> Tuple[torch.Tensor, list]:
     """One allocation for parts of these many bytes, and where they start
     (0 for a part of none); hold the tensor until the launches are made."""
@@ -108,7 +143,7 @@ def _workspace(device, *sizes: int) -> Tuple[torch.Tensor, list]:
                   for at, size in zip(starts, sizes)]
 
 
-def _forward(h, w, targets, ignore_index, reduce: int):
+def _forward(h, w, targets, ignore_index, reduce: int, grad: bool):
     """(loss [N], lse [N], reduced loss or None, its factor or None)."""
     _check(h, w, targets)
     h, w, targets = _rows(h), _rows(w), targets.contiguous()
@@ -120,21 +155,24 @@ def _forward(h, w, targets, ignore_index, reduce: int):
         result = torch.empty((), dtype=torch.float32, device=device)
         factor = torch.empty_like(result)
     size = h.element_size()
-    row = _ceil(d, 64) * 64 * size            # bytes of a packed row
+    kind = _kind(h, v, grad)
+    row = _ceil(d, 64) * 64 * _BYTES[kind]    # of a packed row
     piece = v
     # (the kernel for few rows streams any table)
-    pack_w = not _aligned(w) and not (n <= 16 and d * size <= 4096)
+    pack_w = kind == _SPLIT or not _aligned(w) and not (
+        n <= 16 and d * size <= 4096)
     if pack_w:
         piece = max(256, _PACKED_BYTES // row // 256 * 256)
     # a maximum and a sum of every row for each part of the vocabulary
     parts = max(_ceil(v, piece), min(_ceil(v, 64),
                                      _PARTS // max(1, _ceil(n, 128))))
     held, (part, packed_h, packed_w) = _workspace(
-        device, parts * n * 8, 0 if _aligned(h) else n * row,
+        device, parts * n * 8,
+        0 if kind != _SPLIT and _aligned(h) else n * row,
         min(piece, v) * row if pack_w else 0)
     _native().softmax_loss(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-        int(size == 2), targets.data_ptr(),
+        kind, targets.data_ptr(),
         int(targets.dtype == torch.int64), ignore_index, part, parts * n,
         packed_h, packed_w, piece, loss.data_ptr(), lse.data_ptr(), reduce,
         0 if result is None else result.data_ptr(),
@@ -153,21 +191,24 @@ def _backward(h, w, targets, lse, grad, factor, ignore_index, need_h, need_w):
     dw = torch.empty((v, d), dtype=w.dtype, device=device) \
         if need_w else None
     native = _native()
-    size = h.element_size()
+    kind = _kind(h, v, True)
+    size = _BYTES[kind]
     rows, row = _ceil(n, 32) * 32, _ceil(d, 64) * 64 * size
     # equal pieces of the vocabulary, in whole tiles
-    pieces = _ceil(v, max(256, _COEF_BYTES // (rows * size)))
+    most = rows * size if kind != _SPLIT else max(rows * size, row)
+    pieces = _ceil(v, max(256, _COEF_BYTES // most))
     width = _ceil(_ceil(v, pieces), 256) * 256
     # parts of the long axis where a product's result has few tiles
-    splits, splits_w = native.softmax_plan(n, min(v, width), d, int(size == 2))
+    splits, splits_w = native.softmax_plan(n, min(v, width), d, kind)
     ldp = _ceil(d, 4) * 4
     held, (packed, packed_w, coef, part, part_w) = _workspace(
-        device, rows * row, 0 if _aligned(w) else width * row,
+        device, rows * row,
+        0 if kind != _SPLIT and _aligned(w) else width * row,
         rows * width * size, splits * n * ldp * 4 if need_h else 0,
         splits_w * width * ldp * 4 if need_w and splits_w > 1 else 0)
     native.softmax_grad(
         h.data_ptr(), h.stride(0), n, w.data_ptr(), w.stride(0), v, d,
-        int(size == 2), targets.data_ptr(),
+        kind, targets.data_ptr(),
         int(targets.dtype == torch.int64), ignore_index, lse.data_ptr(),
         grad.data_ptr(), int(grad.dim() > 0),
         0 if factor is None else factor.data_ptr(), packed, packed_w, width,
@@ -188,9 +229,9 @@ def _refuse_capture() -> None:
 
 class _SoftmaxLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, w, targets, reduce, ignore_index):
+    def forward(ctx, h, w, targets, reduce, ignore_index, grad):
         loss, lse, result, factor = _forward(h, w, targets, ignore_index,
-                                             reduce)
+                                             reduce, grad)
         ctx.ignore_index = ignore_index
         ctx.save_for_backward(h, w, targets, lse,
                               *(() if factor is None else (factor,)))
@@ -205,7 +246,7 @@ class _SoftmaxLoss(torch.autograd.Function):
             grad = grad.to(torch.float32).contiguous()
         return (*_backward(h, w, targets, lse, grad,
                            factor[0] if factor else None, ctx.ignore_index,
-                           *ctx.needs_input_grad[:2]), None, None, None)
+                           *ctx.needs_input_grad[:2]), None, None, None, None)
 
 
 _REDUCE = {"none": 0, "sum": 1, "mean": 2}
@@ -228,21 +269,26 @@ def softmax_loss(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
     if reduction not in _REDUCE:
         raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got "
                          f"{reduction!r}")
-    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False)
-                                       for t in (h, w)):
+    grad = torch.is_grad_enabled() and any(
+        getattr(t, "requires_grad", False) for t in (h, w))
+    if grad:
         _refuse_capture()
     return _SoftmaxLoss.apply(h, w, targets, _REDUCE[reduction],
-                              int(ignore_index))
+                              int(ignore_index), grad)
 
 
 def softmax_loss_forward(h: torch.Tensor, w: torch.Tensor,
-                         targets: torch.Tensor, ignore_index: int = -1
+                         targets: torch.Tensor, ignore_index: int = -1,
+                         gradient: bool = False
                          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """The loss and the log of the softmax's sum, both float32 [N], without
     autograd (evaluation, or a captured step together with
-    softmax_loss_backward).  Targets as for softmax_loss."""
+    softmax_loss_backward).  Targets as for softmax_loss.  With ``gradient``
+    scores are rounded as softmax_loss_backward rounds them: its gradient is
+    then the most exact."""
     with torch.no_grad():
-        return _forward(h, w, targets, int(ignore_index), 0)[:2]
+        return _forward(h, w, targets, int(ignore_index), 0,
+                        bool(gradient))[:2]
 
 
 def softmax_loss_backward(h: torch.Tensor, w: torch.Tensor,

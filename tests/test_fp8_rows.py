@@ -156,6 +156,20 @@ def test_product(m, n, k, out):
 
 
 @gpu
+@pytest.mark.parametrize("m", [1, 20, 161])
+def test_widest_product(m):
+    """2^20 columns; more are refused."""
+    k = 1 << 20
+    b = _rows(70, k, torch.bfloat16)
+    _product(_rows(m, k, torch.bfloat16, seed=1), fp8.quantize_rows(b),
+             _held(b)[0])
+    with pytest.raises(ValueError, match="2\\^20"):
+        fp8.matmul_rows(torch.zeros(1, k + 1, device="cuda"),
+                        fp8.quantize_rows(torch.zeros(1, k + 1,
+                                                      device="cuda")))
+
+
+@gpu
 def test_product_in_many_pieces(monkeypatch):
     """More table rows than one piece of the converted table holds."""
     b = _rows(9000, 4000, torch.bfloat16, seed=3)

@@ -154,6 +154,152 @@ def test_strides_and_offsets(dtype):
     _check(h[:1].expand(n, d), w, y)
 
 
+@pytest.fixture
+def in_parts(monkeypatch):
+    """float32 of any size in parts of bfloat16."""
+    monkeypatch.setattr(S, "_SPLIT_LOSS", (0, 0))
+    monkeypatch.setattr(S, "_SPLIT_GRAD", (0, 0))
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d", SHAPES + FORMS + [(260, 70_000, 40)])
+def test_parts_of_bfloat16(n, v, d, in_parts):
+    """As exact as float32: the same tolerances."""
+    _check(*_inputs(n, v, d, torch.float32, seed=n + v + d))
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d", [(384, 60_000, 100), (192, 2000, 100),
+                                   (191, 2000, 100), (383, 60_000, 100)])
+def test_where_parts_begin(n, v, d):
+    """Sizes at which the form changes, as they are chosen."""
+    _check(*_inputs(n, v, d, torch.float32))
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d", [(285, 95, 588), (192, 2000, 100),
+                                   (600, 3000, 64)])
+def test_gradient_from_scores_rounded_alike(n, v, d):
+    """Confident rows, whose targets score 12 and the other words little.
+    Where a target's score and those in lse are rounded alike, an error e_v of
+    the scores changes p_v by p_v (e_v - sum_k p_k e_k): for the target, whose
+    p is almost 1, by 2 p (1 - p) of the largest.  What is left is lse in
+    float32, its product with log2 e and the exponent's own rounding: (3 |lse|
+    + 3 |s|) U, and with the sum's and the exponentials' roundings twice
+    that and (v / 8 + 64) U (1 - p), 16 U at most."""
+    g = torch.Generator().manual_seed(n)
+    w = torch.randn(v, d, generator=g)
+    y = torch.randint(0, v, (n,), generator=g)
+    h = w[y] * (12.0 / (w[y] ** 2).sum(1, keepdim=True))
+    h = h + 0.3 * torch.randn(n, d, generator=g) / d ** 0.5
+    a, b = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    S.softmax_loss(a, b, y.cuda(), reduction="sum").backward()
+    _, lse = S.softmax_loss_forward(h.cuda(), w.cuda(), y.cuda(),
+                                    gradient=True)
+    pair = S.softmax_loss_backward(h.cuda(), w.cuda(), y.cuda(), lse,
+                                   torch.ones((), device="cuda"))
+    h, w = h.double(), w.double()
+    s = h @ w.T
+    off_s = (2 * (d + 2) * U * (h.abs() @ w.abs().T)).amax(1, keepdim=True)
+    p = torch.softmax(s, 1)
+    lse = torch.logsumexp(s, 1, keepdim=True)
+    c = p.clone()
+    c[torch.arange(n), y] -= 1
+    off_c = p * (2 * (1 - p) * off_s * 1.01 + (1 - p) * (v / 8 + 64) * U
+                 + 6 * U * (lse.abs() + s.abs()) + 16 * U) + 4 * U * c.abs()
+    dh, dw = c @ w, c.T @ h
+    off_dh = (off_c + 2 * (v + 2) * U * c.abs()) @ w.abs() + 2 * U * dh.abs()
+    off_dw = (off_c + 2 * (n + 2) * U * c.abs()).T @ h.abs() \
+        + 2 * U * dw.abs()
+    for x, z in ((a.grad, b.grad), pair):
+        _near(x, dh, off_dh, "dh")
+        _near(z, dw, off_dw, "dw")
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_widest_rows(n, dtype):
+    """2^20 columns; more are refused."""
+    _check(*_inputs(n, 70, 1 << 20, dtype))
+
+
+@gpu
+def test_widest_rows_in_parts(in_parts):
+    _check(*_inputs(5, 70, 1 << 20, torch.float32))
+
+
+@gpu
+def test_parts_of_every_magnitude(in_parts, monkeypatch):
+    """Numbers from 2^-126 up to float32's largest, alone in their rows, so
+    that each score is one product: within two roundings of it, and within a
+    subnormal part of bfloat16 (2^-134) times the other factor."""
+    monkeypatch.setattr(S, "_COEF_BYTES", 1 << 16)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(300, 1, generator=g)
+    x = x / x.abs() * 2.0 ** torch.linspace(-126, 127.99, 300)[:, None]
+    x[-1] = torch.finfo(torch.float32).max
+    h = torch.zeros(300, 40)
+    h[:, 7] = x[:, 0]
+    w = torch.zeros(2, 40)
+    for f in (1.0, 1 + 2.0 ** -8 + 2.0 ** -16 + 2.0 ** -23, 2.0 ** -100,
+              -0.99999994):
+        w[0, 7] = f
+        want = h[:, 7].double() * float(w[0, 7])
+        # a product past float32 is not finite in any form
+        fits = want.abs() <= torch.finfo(torch.float32).max
+        y = torch.ones(300, dtype=torch.long, device="cuda")
+        # the loss of word 1, whose score is 0, is log(1 + exp(score)): the
+        # score itself where that is large
+        loss, lse = S.softmax_loss_forward(h.cuda(), w.cuda(), y)
+        ref = torch.logaddexp(want, torch.zeros_like(want))
+        off = 4 * U * want.abs() + 2.0 ** -134 * abs(float(w[0, 7])) + 8 * U
+        assert ((loss.double().cpu() - ref).abs() <= off)[fits].all()
+        assert fits.sum() >= 299
+    # and as gradients: one sample, whose coefficients are p - 1 = -1/2
+    for rows in x.reshape(-1, 10)[:29]:
+        h = rows[:, None].repeat(1, 40).cuda()
+        dh, dw = S.softmax_loss_backward(
+            h, torch.zeros(2, 40, device="cuda"),
+            torch.zeros(10, dtype=torch.long, device="cuda"),
+            torch.full((10,), math.log(2.0), device="cuda"),
+            torch.ones((), device="cuda"))
+        assert (dh == 0).all()
+        want = -0.5 * rows.double().sum()
+        off = 16 * U * rows.double().abs().sum() + 2.0 ** -133
+        assert ((dw[0].double().cpu() - want).abs() <= off).all()
+
+
+@gpu
+def test_parts_strides_ignored_and_not_finite(in_parts, monkeypatch):
+    monkeypatch.setattr(S, "_COEF_BYTES", 1 << 16)
+    monkeypatch.setattr(S, "_PACKED_BYTES", 1 << 16)
+    h, w, y = _inputs(100, 1500, 97, torch.float32)
+    big_h = torch.full((100, 203), math.nan, device="cuda")
+    big_h[:, 5:199:2] = h
+    big_w = torch.full((1502, 103), math.nan, device="cuda")
+    big_w[1:-1, 5:102] = w
+    y[::9] = -1
+    _check(big_h[:, 5:199:2], big_w[1:-1, 5:102], y)
+    one = torch.ones((), device="cuda")
+    good, lse = S.softmax_loss_forward(h, w, y)
+    dh, dw = S.softmax_loss_backward(h, w, y, lse, one)
+    # rows without a loss may hold anything
+    h[::9] = math.nan
+    h[0], h[9] = math.inf, -math.inf
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    assert torch.equal(loss, good)
+    a, b = S.softmax_loss_backward(h, w, y, lse, one)
+    assert torch.equal(a, dh) and torch.equal(b, dw)
+    # others that are not finite keep to themselves
+    h[[1, 2, 3]] = torch.tensor([math.nan, math.inf, -math.inf],
+                                device="cuda")[:, None]
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    assert loss[1:4].isnan().all() and torch.equal(loss[4:], good[4:])
+    a, _ = S.softmax_loss_backward(h, w, y, lse, one)
+    assert a[1:4].isnan().all() and torch.equal(a[4:], dh[4:])
+
+
 @gpu
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 @pytest.mark.parametrize("ignore", [-1, -100, 0, 5])
@@ -427,6 +573,8 @@ def test_refusals():
             ((h, w, y[:, None]), ValueError),
             ((h, w[:, :7], y), ValueError), ((h[:3], w, y), ValueError),
             ((h, w[:0], y), ValueError), ((h[:, :0], w[:, :0], y), ValueError),
+            ((torch.zeros(4, 2 ** 20 + 1), torch.zeros(1, 2 ** 20 + 1), y),
+             ValueError),
             ((h.half(), w.half(), y), TypeError),
             ((h.double(), w.double(), y), TypeError),
             ((h, w.bfloat16(), y), TypeError),
