@@ -36,6 +36,10 @@ namespace py = pybind11;
                                std::to_string(__LINE__));                   \
   } while (0)
 
+// For lambdas with many calls: one that is not inlined keeps what it captures
+// in memory.
+#define INLINE __attribute__((always_inline))
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -55,7 +59,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 // is (s - m) log2e instead: one instruction more, but it cannot overflow.
 constexpr float kFar = 1e6f;
 
-// kSplit is float32 in three parts of bf16, x = hi + mid + lo exactly: each
+// kSplit is float32 in three parts of bf16, x = hi + mid + lo exactly (down to
+// bf16's smallest subnormal, 2^-133, for numbers under 2^-109): each
 // part is the nearest bf16 to what the ones before leave, so that mid and lo
 // are at most 2^-9 and 2^-18 of x.  Of the nine products of two such numbers
 // the six from 2^-18 up are taken; the others are 2^-26 of the product at
@@ -104,14 +109,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// The three parts of x.  What is not finite is all in the first.
+// The three parts of x.  What is not finite is all in the first.  Where bf16
+// would round x past the largest number, the parts are cut off instead of
+// rounded: all of x's sign, so that no sum of them passes x.
 __device__ __forceinline__ void split(float x, float& hi, float& mid, float& lo) {
   const uint32_t u = __float_as_uint(x);
   const bool finite = (u & 0x7f800000u) != 0x7f800000u;
   hi = (float)(__bf16)x;
-  if (finite && __builtin_isinf(hi)) hi = __uint_as_float(u & 0xffff0000u);
+  const bool cut = finite && __builtin_isinf(hi);
+  if (cut) hi = __uint_as_float(u & 0xffff0000u);
   const float rest = finite ? x - hi : 0.f;
-  mid = (float)(__bf16)rest;
+  mid = cut ? __uint_as_float(__float_as_uint(rest) & 0xffff0000u) : (float)(__bf16)rest;
   lo = rest - mid;
 }
 __device__ __forceinline__ void split4(const f32x4& x, u32x2 (&to)[3]) {
@@ -216,16 +224,16 @@ __device__ __forceinline__ void mma_row(u32x4 a, const u32x4 (&b)[N], f32x4 (&c)
   mma_all<T>(a1, b, reinterpret_cast<f32x4(&)[1][N]>(c));
 }
 
-// The six products of two sides in three parts, small ones first.
+// The six products of two sides in three parts.
 template <int M, int N>
 __device__ __forceinline__ void mma_split(const u32x4 (&a)[3][M], const u32x4 (&b)[3][N],
                                           f32x4 (&c)[M][N]) {
-  mma_all<kBF16>(a[2], b[0], c);
-  mma_all<kBF16>(a[0], b[2], c);
-  mma_all<kBF16>(a[1], b[1], c);
-  mma_all<kBF16>(a[1], b[0], c);
-  mma_all<kBF16>(a[0], b[1], c);
   mma_all<kBF16>(a[0], b[0], c);
+  mma_all<kBF16>(a[1], b[0], c);
+  mma_all<kBF16>(a[2], b[0], c);
+  mma_all<kBF16>(a[0], b[1], c);
+  mma_all<kBF16>(a[1], b[1], c);
+  mma_all<kBF16>(a[0], b[2], c);
 }
 
 // ---------------------------------------------------------------------------
@@ -590,7 +598,11 @@ __device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint3
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
-// The same, 4 bytes a lane.
+// The same, and for all reads of LDS.
+__device__ __forceinline__ void wait_all() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+// load_lds16 with 4 bytes a lane.
 __device__ __forceinline__ void load_lds4(const char* p, uint32_t offset, uint32_t lds) {
   const uint64_t at = (uint64_t)p;
   const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
@@ -832,6 +844,7 @@ __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2)
   constexpr int kScaleWave = TW == kFP8 ? kWaves - 1 : -1;
   static_assert(kBytesW % 1024 == 0 && kBytesH % 1024 == 0 && kMore < kWaves, "");
   static_assert(TW != kFP8 || kV == 256, "");
+  static_assert(P == 1 || (kMore == 0 && kEach >= 2 * MR), "");
   __shared__ __align__(16) char lds[kAhead + 1][kBytesW + kBytesH + kBytesS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -850,39 +863,45 @@ __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2)
   // What lies outside is replaced by what is inside, and no lane sits out: the
   // waits below count the loads of each wave.
   int fetch_tile = t0, fetch_step = 0;
-  auto fetch = [&](int buf) {
+  constexpr int kFetches = kEach + (kMore > 0);
+  // load i of kFetches of the step that is next
+  auto fetch_one = [&](int buf, int i) INLINE {
     const int v0 = a.v_begin + fetch_tile * kV;
-    const int last_w = min(kV - 1, (int)a.w.rows - 1 - v0);
     const int ow = fetch_step * (kWideW * P), oh = fetch_step * (kWideH * P);
-    const char* bw = a.w.p + v0 * a.w.ld + ow;
-    const char* bh = a.h.p + n0 * a.h.ld + oh;
-    const int end_w = ((a.w.kb - 1) & ~15) - ow, end_h = ((a.h.kb - 1) & ~15) - oh;
-#pragma unroll
-    for (int i = 0; i < kEach + (kMore > 0); ++i) {
-      const int q = wave + kWaves * i;
-      if (q * 1024 < kBytesW) {
-        const int part = q / (kPartW / 1024), p = (q - part * (kPartW / 1024)) * 64 + lane;
-        const int r = TW == kFP8 ? p >> 1 : p >> 2;
-        const int c = TW == kFP8 ? p & 1 : row_chunk(64, r, p & 3);
-        const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, end_w);
-        load_lds16(bw, (uint32_t)(min(r, last_w) * (int)a.w.ld + at),
-                   lds_address(&lds[buf][q * 1024]));
-      } else if (q < kInstr) {
-        const int q1 = q - kBytesW / 1024;
-        const int part = q1 / (kPartH / 1024), p = (q1 - part * (kPartH / 1024)) * 64 + lane;
-        const int r = p >> 2, c = row_chunk(64, r, p & 3);
-        const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, end_h);
-        load_lds16(bh, (uint32_t)(min(r, last_h) * (int)a.h.ld + at),
-                   lds_address(&lds[buf][q * 1024]));
-      }
+    const int q = wave + kWaves * i;
+    if (q * 1024 < kBytesW) {
+      const int part = q / (kPartW / 1024), p = (q - part * (kPartW / 1024)) * 64 + lane;
+      const int r = TW == kFP8 ? p >> 1 : p >> 2;
+      const int c = TW == kFP8 ? p & 1 : row_chunk(64, r, p & 3);
+      const int last = min(kV - 1, (int)a.w.rows - 1 - v0);
+      const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, ((a.w.kb - 1) & ~15) - ow);
+      load_lds16(a.w.p + v0 * a.w.ld + ow, (uint32_t)(min(r, last) * (int)a.w.ld + at),
+                 lds_address(&lds[buf][q * 1024]));
+    } else if (q < kInstr) {
+      const int q1 = q - kBytesW / 1024;
+      const int part = q1 / (kPartH / 1024), p = (q1 - part * (kPartH / 1024)) * 64 + lane;
+      const int r = p >> 2, c = row_chunk(64, r, p & 3);
+      const int at = P > 1 ? part * 64 + c * 16 : min(c * 16, ((a.h.kb - 1) & ~15) - oh);
+      load_lds16(a.h.p + n0 * a.h.ld + oh, (uint32_t)(min(r, last_h) * (int)a.h.ld + at),
+                 lds_address(&lds[buf][q * 1024]));
     }
+  };
+  auto fetched = [&]() INLINE {
+    // kSplit loads without a branch: after the last step, that one again
+    if (P > 1 && fetch_tile + 1 == t1 && fetch_step + 1 == steps) return;
+    if (++fetch_step == steps) fetch_step = 0, ++fetch_tile;
+  };
+  auto fetch = [&](int buf) INLINE {
+#pragma unroll
+    for (int i = 0; i < kFetches; ++i) fetch_one(buf, i);
     if constexpr (TW == kFP8) {
       // kV bytes, four to a lane; rows past the end have room
       if (wave == kScaleWave)
-        load_lds4((const char*)a.w.scales + (int64_t)(ow >> 7) * a.w.lds + v0,
+        load_lds4((const char*)a.w.scales + (int64_t)(fetch_step * kWideW >> 7) * a.w.lds +
+                      a.v_begin + fetch_tile * kV,
                   (uint32_t)lane * 4, lds_address(&lds[buf][kBytesW + kBytesH]));
     }
-    if (++fetch_step == steps) fetch_step = 0, ++fetch_tile;
+    fetched();
   };
 
   Sink<USE, TC, NS> sink;
@@ -892,6 +911,106 @@ __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2)
   for (int i = 0; i < kAhead; ++i)
     if (i < all) fetch(i);
   int tile = t0, step = 0, at_buf = 0;
+  auto finish_tile = [&]() INLINE {
+    const int v = a.v_begin + tile * kV + wv * 64 + 4 * g;
+    if (USE == kStore && a.col_scale)
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        f32x4 cs;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cs[e] = col_scale_of(a, v + i * 16 + e);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) acc[i][j] *= cs;
+      }
+    const int v0 = a.v_begin + tile * kV + wv * 64;
+    sink.template take<MR>(a, acc, v0, (int)n0 + wn * (16 * NS), v0 + 64 > a.v_end,
+                           sink.meets(v0, 64));
+    step = 0;
+    ++tile;
+  };
+  const int at = r16 * 64 + row_chunk(64, r16, g) * 16;
+  if constexpr (P > 1) {
+    // The step's fragments are in registers and the next step's tiles in LDS
+    // before the last two products, which run beside the next step's first
+    // reads and the loads of the one after.
+    u32x4 fa[P][MR], fb[P][NS], na[MR], nb[NS];
+    auto read_a = [&](u32x4 (&f)[MR], int buf, int p) INLINE {
+      const char* q = lds[buf] + p * kPartW + wv * 64 * 64 + at;
+#pragma unroll
+      for (int i = 0; i < MR; ++i) f[i] = *reinterpret_cast<const u32x4*>(q + i * 16 * 64);
+    };
+    auto read_b = [&](u32x4 (&f)[NS], int buf, int p) INLINE {
+      const char* q = lds[buf] + kBytesW + p * kPartH + wn * (16 * NS) * 64 + at;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) f[j] = *reinterpret_cast<const u32x4*>(q + j * 16 * 64);
+    };
+    wait_loads();
+    __syncthreads();
+    if (all > 0) fetch(1), read_a(na, 0, 0), read_b(nb, 0, 0);
+    for (int64_t s = 0; s < all; ++s) {
+      if (step == 0) {
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int i = 0; i < MR; ++i) fa[0][i] = na[i];
+#pragma unroll
+      for (int j = 0; j < NS; ++j) fb[0][j] = nb[j];
+      // 4 NS results of one product, and loads or reads among them: in one
+      // block they would keep the matrix unit waiting
+      auto mma = [&](int p, int q, int i) INLINE {
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, fa[p][i]), __builtin_bit_cast(bf16x8, fb[q][j]),
+              acc[i][j], 0, 0, 0);
+      };
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        if (i == 0) read_a(fa[1], at_buf, 1);
+        if (i == 1) read_b(fb[1], at_buf, 1);
+        if (i == 2) read_a(fa[2], at_buf, 2);
+        if (i == 3) read_b(fb[2], at_buf, 2);
+        mma(0, 0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < MR; ++i) mma(1, 0, i);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) mma(0, 1, i);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) mma(2, 0, i);
+      __builtin_amdgcn_sched_barrier(0);
+      const int to = at_buf;
+      wait_all();
+      __syncthreads();
+      at_buf ^= 1;
+      read_a(na, at_buf, 0);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        mma(1, 1, i);
+        if (i == 0) read_b(nb, at_buf, 0);
+        fetch_one(to, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        mma(0, 2, i);
+        fetch_one(to, i + MR);
+        if (i + 1 == MR)
+#pragma unroll
+          for (int k = 2 * MR; k < kFetches; ++k) fetch_one(to, k);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fetched();
+      if (++step == steps) finish_tile();
+    }
+    wait_loads();
+    if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
+    return;
+  }
   for (int64_t s = 0; s < all; ++s) {
     // step s has arrived, two more may be on their way
     if (s + kAhead - 1 < all) {
@@ -911,66 +1030,35 @@ __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2)
     const char* buf = lds[at_buf];
     at_buf = at_buf == kAhead ? 0 : at_buf + 1;
     const char* lh = buf + kBytesW + wn * (16 * NS) * kWideH;
-    const int at = r16 * 64 + row_chunk(64, r16, g) * 16;
-    if constexpr (P > 1) {
-      u32x4 fa[P][MR], fb[P][NS];
+    u32x4 fa[MR], fb[NS];
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p) {
-#pragma unroll
-        for (int i = 0; i < MR; ++i)
-          fa[p][i] = *reinterpret_cast<const u32x4*>(buf + p * kPartW + (wv * 64 + i * 16) * 64 + at);
-#pragma unroll
-        for (int j = 0; j < NS; ++j)
-          fb[p][j] = *reinterpret_cast<const u32x4*>(lh + p * kPartH + j * 16 * 64 + at);
+    for (int i = 0; i < MR; ++i) {
+      if constexpr (TW == kFP8) {
+        const int r = wv * 64 + i * 16 + r16;
+        const u32x2 q = *reinterpret_cast<const u32x2*>(buf + r * 32 + g * 8);
+        const uint8_t e = *reinterpret_cast<const uint8_t*>(buf + kBytesW + kBytesH + r);
+        fa[i] = fp8x8_to_bf16(q[0], q[1], scale_of(e));
+      } else {
+        fa[i] = *reinterpret_cast<const u32x4*>(buf + (wv * 64 + i * 16) * 64 + at);
       }
-      mma_split(fa, fb, acc);
-    } else {
-      u32x4 fa[MR], fb[NS];
-#pragma unroll
-      for (int i = 0; i < MR; ++i) {
-        if constexpr (TW == kFP8) {
-          const int r = wv * 64 + i * 16 + r16;
-          const u32x2 q = *reinterpret_cast<const u32x2*>(buf + r * 32 + g * 8);
-          const uint8_t e = *reinterpret_cast<const uint8_t*>(buf + kBytesW + kBytesH + r);
-          fa[i] = fp8x8_to_bf16(q[0], q[1], scale_of(e));
-        } else {
-          fa[i] = *reinterpret_cast<const u32x4*>(buf + (wv * 64 + i * 16) * 64 + at);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NS; ++j)
-        fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64 + at);
-      if (step + 1 == steps && (a.h.kb & 63) != 0) {
-        // columns past the last one, whatever they hold
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
-          const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
-#pragma unroll
-          for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
-#pragma unroll
-          for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
-        }
-      }
-      mma_all<TC>(fa, fb, acc);
     }
-    if (++step == steps) {
-      const int v = a.v_begin + tile * kV + wv * 64 + 4 * g;
-      if (USE == kStore && a.col_scale)
 #pragma unroll
-        for (int i = 0; i < MR; ++i) {
-          f32x4 cs;
+    for (int j = 0; j < NS; ++j)
+      fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64 + at);
+    if (step + 1 == steps && (a.h.kb & 63) != 0) {
+      // columns past the last one, whatever they hold
 #pragma unroll
-          for (int e = 0; e < 4; ++e) cs[e] = col_scale_of(a, v + i * 16 + e);
+      for (int q = 0; q < 4; ++q) {
+        const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
+        const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
 #pragma unroll
-          for (int j = 0; j < NS; ++j) acc[i][j] *= cs;
-        }
-      const int v0 = a.v_begin + tile * kV + wv * 64;
-      sink.template take<MR>(a, acc, v0, (int)n0 + wn * (16 * NS), v0 + 64 > a.v_end,
-                             sink.meets(v0, 64));
-      step = 0;
-      ++tile;
+        for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
+      }
     }
+    mma_all<TC>(fa, fb, acc);
+    if (++step == steps) finish_tile();
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
 }
@@ -1359,7 +1447,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
     const char* b = x + kBytesX;
     u32x4 fb[P][J];
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p)
+    for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         if constexpr (DW) {
@@ -1375,7 +1463,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
       if constexpr (P > 1) {
         u32x4 fa[P][1];
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p)
+        for (int p = 0; p < P; ++p)
           fa[p][0] = columns(x + p * kPartX, kPitchX, wd * ND + i);
         mma_split(fa, fb, reinterpret_cast<f32x4(&)[1][J]>(acc[i]));
       } else {
