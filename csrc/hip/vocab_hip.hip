@@ -1367,44 +1367,47 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   const int64_t block_row = a.ldc * (kLine * P);     // 16 samples' coefficients
   const int have_b = (int)min((int64_t)(DW ? kChunksB : kRowsR),
                               DW ? ((a.r - r0) * ES + 15) / 16 : a.r - r0);
-  auto fetch = [&](int s) {
+  // load i of kFetches of step s
+  constexpr int kFetches = kEach + (kMore > 0);
+  auto fetch_one = [&](int s, int i) INLINE {
     char* buf = lds[(s - s0) % (kAhead + 1)];
     const int64_t k0 = (int64_t)s * kStep;
     const char* xb = a.x.p + k0 * a.x.ld + d0 * (ES * P);
     const int last = (int)min((int64_t)kStep - 1, a.x.rows - 1 - k0);
-#pragma unroll
-    for (int i = 0; i < kEach + (kMore > 0); ++i) {
-      const int q = wave + 8 * i;
-      if (q * 1024 < kBytesX) {
-        const int part = q / (kPartX / 1024), p = (q - part * (kPartX / 1024)) * 64 + lane;
-        const int k = p / kChunksX, pos = p % kChunksX;
-        const int c = min(((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer, have_x - 1);
-        const int in = P > 1 ? (c >> 2) * 192 + part * 64 + (c & 3) * 16 : c * 16;
-        load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + in), lds_address(buf + q * 1024));
-      } else if (q < kInstr) {
-        const int q1 = q - kBytesX / 1024;
-        const int part = q1 / (kPartB / 1024), p = (q1 - part * (kPartB / 1024)) * 64 + lane;
-        const char* from;
-        uint32_t offset;
-        if constexpr (DW) {
-          // samples k, chunk c of the table rows
-          const int k = p / kChunksB, pos = p % kChunksB;
-          const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
-          const int in = min(c, have_b - 1);
-          from = a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock;
-          offset = (uint32_t)(k >> 4) * (uint32_t)block_row + part * 512 + (k & 15) * kLine +
-                   in / kPer * kBlock + in % kPer * 16;
-        } else {
-          // 64 bytes of samples r
-          const int r = p >> 2, c = row_chunk(64, r, p & 3);
-          const int in = min(r, have_b - 1);
-          from = a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock;
-          offset = (uint32_t)(in >> 4) * (uint32_t)block_row + part * 512 + (in & 15) * kLine +
-                   c / kPer * kBlock + c % kPer * 16;
-        }
-        load_lds16(from, offset, lds_address(buf + q * 1024));
+    const int q = wave + 8 * i;
+    if (q * 1024 < kBytesX) {
+      const int part = q / (kPartX / 1024), p = (q - part * (kPartX / 1024)) * 64 + lane;
+      const int k = p / kChunksX, pos = p % kChunksX;
+      const int c = min(((pos / kPer) ^ key(k, kPitchX)) * kPer + pos % kPer, have_x - 1);
+      const int in = P > 1 ? (c >> 2) * 192 + part * 64 + (c & 3) * 16 : c * 16;
+      load_lds16(xb, (uint32_t)(min(k, last) * (int)a.x.ld + in), lds_address(buf + q * 1024));
+    } else if (q < kInstr) {
+      const int q1 = q - kBytesX / 1024;
+      const int part = q1 / (kPartB / 1024), p = (q1 - part * (kPartB / 1024)) * 64 + lane;
+      const char* from;
+      uint32_t offset;
+      if constexpr (DW) {
+        // samples k, chunk c of the table rows
+        const int k = p / kChunksB, pos = p % kChunksB;
+        const int c = ((pos / kPer) ^ key(k, kPitchB)) * kPer + pos % kPer;
+        const int in = min(c, have_b - 1);
+        from = a.coef + (k0 >> 4) * block_row + (r0 >> 4) * kBlock;
+        offset = (uint32_t)(k >> 4) * (uint32_t)block_row + part * 512 + (k & 15) * kLine +
+                 in / kPer * kBlock + in % kPer * 16;
+      } else {
+        // 64 bytes of samples r
+        const int r = p >> 2, c = row_chunk(64, r, p & 3);
+        const int in = min(r, have_b - 1);
+        from = a.coef + (r0 >> 4) * block_row + (k0 >> 4) * kBlock;
+        offset = (uint32_t)(in >> 4) * (uint32_t)block_row + part * 512 + (in & 15) * kLine +
+                 c / kPer * kBlock + c % kPer * 16;
       }
+      load_lds16(from, offset, lds_address(buf + q * 1024));
     }
+  };
+  auto fetch = [&](int s) INLINE {
+#pragma unroll
+    for (int i = 0; i < kFetches; ++i) fetch_one(s, i);
   };
 
   f32x4 acc[ND][J];
@@ -1442,7 +1445,7 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
       wait_loads();
     }
     __syncthreads();
-    if (s + kAhead < s1) fetch(s + kAhead);
+    const bool more = s + kAhead < s1;
     const char* x = lds[(s - s0) % (kAhead + 1)];
     const char* b = x + kBytesX;
     u32x4 fb[P][J];
@@ -1470,6 +1473,13 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
         const u32x4 fa = columns(x, kPitchX, wd * ND + i);
         mma_row<T>(fa, fb[0], acc[i]);
       }
+      // loads among the products: in one block they would keep the matrix unit
+      // waiting
+      constexpr int kPerRow = (kFetches + ND - 1) / ND;
+      if (more)
+#pragma unroll
+        for (int k = i * kPerRow; k < (i + 1) * kPerRow && k < kFetches; ++k)
+          fetch_one(s + kAhead, k);
     }
   }
   const float scale = a.part ? 1.f : scale_by(a.scale[0], a.scale[1]);
