@@ -830,9 +830,10 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 // they are read from LDS, and their scales lie by block of columns, then row.
 template <int TW, int TC, int USE, int WV, int WN, int NS>
 __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2) void tile_kernel(ScoreArgs a) {
-  // float32 steps are long: two ahead do, and three workgroups fit a CU
+  // float32 steps are long: two ahead do, and three workgroups fit a CU; the
+  // small tile's are short
   constexpr int kWaves = WV * WN, MR = 4, P = Elem<TC>::parts;
-  constexpr int kAhead = TC == kSplit ? 1 : TC == kF32 ? 2 : 3;
+  constexpr int kAhead = TC == kSplit ? 1 : TC == kF32 ? (WV == 1 ? 4 : 2) : 3;
   constexpr int kV = 64 * WV, kN = 16 * NS * WN;
   constexpr int kWideW = TW == kFP8 ? 32 : 64, kWideH = 64;   // bytes per step and part
   constexpr int kPartW = kV * kWideW, kPartH = kN * kWideH;
@@ -1821,6 +1822,12 @@ static void launch_tile(ScoreArgs& a, hipStream_t stream) {
     // one a SIMD (20000 x 8000 x 256: 425 us, with four 483)
     launch_tile_k<TW, TC, USE, 4, 2, 4>(a, stream);
   } else {
+    // few results: 64 x 64, so that more of the card's matrix units work and a
+    // step takes a wave a quarter of the time
+    if constexpr (TC == kF32) {
+      const int64_t tiles = ((a.v_end - a.v_begin + 127) / 128) * ((a.n + 127) / 128);
+      if (tiles <= 128) return launch_tile_k<TW, TC, USE, 1, 4, 1>(a, stream);
+    }
     if (TW == kFP8 || a.n <= 32) return launch_tile_k<TW, TC, USE, 4, 1, 2>(a, stream);
     // 128 x 128 fills the card more evenly; bf16 is bound by LDS there, and
     // takes 256 x 256 where there are enough of them
@@ -1966,31 +1973,33 @@ struct GradForm {
 static GradForm grad_form(int type, bool dw, int64_t r, int64_t k, int d) {
   GradForm f{256, 0, 0, 256};
   int wd = 2, most = 10, step = 2;    // waves along d, blocks of 16 columns a wave
-  if (type == kSplit) {
-    // 256 x 128: two steps of that fit LDS
-    const int columns = (d + 31) / 32;
-    f.tiles_d = (columns + 3) / 4;
-    f.nd = (columns + f.tiles_d - 1) / f.tiles_d <= 2 ? 2 : 4;
-    return f;
-  }
-  if (!dw && r <= 32) f.rows = 32, wd = 8, most = 3, step = 1, f.slots = 512;
+  if (type == kSplit) most = 4;       // two steps of 256 x 128 fit LDS
+  else if (!dw && r <= 32) f.rows = 32, wd = 8, most = 3, step = 1, f.slots = 512;
   else if (!dw && r <= 128) f.rows = 128, wd = 4, most = 5, step = 1, f.slots = 512;
   else if (dw && k <= 128) f.rows = 0, most = 4, f.slots = 768;
-  if (f.rows == 0 || (f.rows == 256 && type == kBF16)) {
+  if (f.rows == 0 || (f.rows == 256 && type != kF32)) {
     // bound by LDS or by what is written: the fewest tiles
     f.tiles_d = (d + 16 * wd * most - 1) / (16 * wd * most);
     f.nd = ((d + f.tiles_d - 1) / f.tiles_d + 63) / 64 * 2;
-    if (f.rows == 0 && f.nd > 2) f.nd = 4;
-    return f;
+    if ((f.rows == 0 || type == kSplit) && f.nd > 2) f.nd = 4;
+  } else {
+    // the fewest columns past d, and of those the most tiles, which fill the
+    // card more evenly; but no narrow ones where wide ones do
+    int least = INT32_MAX;
+    for (int n = most; n >= step; n -= step) {
+      const int t = (d + 16 * n * wd - 1) / (16 * n * wd);
+      if (t * n < least || (t * n == least && n > 2)) least = t * n, f.nd = n, f.tiles_d = t;
+    }
   }
-  // the fewest columns past d, and of those the most tiles, which fill the
-  // card more evenly; but no narrow ones where wide ones do
-  int least = INT32_MAX;
-  for (int n = most; n >= step; n -= step) {
-    const int t = (d + 16 * n * wd - 1) / (16 * n * wd);
-    if (t * n < least || (t * n == least && n > 2)) least = t * n, f.nd = n, f.tiles_d = t;
-  }
-  if (f.rows == 256 && f.nd <= 4) f.slots = 512;
+  if (f.rows != 256) return f;
+  // Little work: narrow tiles rather than many parts of the sums.  Times of both
+  // gradients, d = 300, with wide and with narrow tiles (us): bf16 1000 x 8000
+  // 121 and 75, 3000 x 2000 119 and 80, 8000 x 8000 241 and 298; float32 1000 x
+  // 2000 102 and 94, 8000 x 2000 262 and 278
+  if ((double)r * k * d <= (type == kBF16 ? 4e9 : 1e9))
+    while (f.nd > 2 && (r + 255) / 256 * f.tiles_d < 128)
+      f.nd -= 2, f.tiles_d = (d + 32 * f.nd - 1) / (32 * f.nd);
+  if (type == kF32 && f.nd <= 4) f.slots = 512;
   return f;
 }
 

@@ -101,7 +101,7 @@ _FLOAT, _BF16, _SPLIT = 0, 1, 3
 _BYTES = {_FLOAT: 4, _BF16: 2, _SPLIT: 6}
 # float32 goes in parts from so many samples and products on; see _kind
 _SPLIT_LOSS = 384, 1 << 31
-_SPLIT_GRAD = 192, 0
+_SPLIT_GRAD = 192, 1 << 30
 _SPLIT_COEF_BYTES = 256 << 20
 
 
@@ -115,10 +115,10 @@ def _kind(h: torch.Tensor, v: int, grad: bool) -> int:
     again.  Times in float32 and in parts (us):
       loss, d = 200: 512 x 30000 71 and 63, 4096 x 30000 438 and 300;
         256 x 200000 202 and 252, 1024 x 4000 28 and 37
-      gradient, d = 200: 256 x 4000 95 and 81, 1024 x 30000 460 and 292;
-        128 x 200000 402 and 484
-      gradient, d = 64: 1024 x 30000 166 and 153; 512 x 200000 438 and 556,
-        whose coefficients are past the cache"""
+      loss with its gradient, d = 300: 3000 x 3000 357 and 232, 8000 x 1000
+        305 and 215; 1000 x 1000 85 and 115, 300 x 3000 82 and 116
+      gradient, d = 64: 512 x 200000 438 and 556, whose coefficients are past
+        the cache"""
     if h.dtype == torch.bfloat16:
         return _BF16
     n, d = h.shape
