@@ -348,6 +348,8 @@ class GlintWord2VecModel:
         around every known word of ``sentences``, by the softmax over the
         whole vocabulary: how well the model predicts held-out text.  Needs
         to_gpu() and a model with syn1."""
+        if batch < 1:
+            raise ValueError(f"batch must be at least 1, got {batch}")
         if self._gpu is None:
             raise RuntimeError("call to_gpu() first")
         if self.syn1 is None:

@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pybind11
 from setuptools import setup, Extension
@@ -73,8 +74,8 @@ def build_hip_extension(name: str = "_hip_native",
 class BuildExt(build_ext):
     def run(self):
         super().run()
-        for name in HIP_EXTENSIONS:
-            build_hip_extension(name)
+        with ThreadPoolExecutor() as pool:      # minutes each
+            list(pool.map(build_hip_extension, HIP_EXTENSIONS))
 
 
 setup(

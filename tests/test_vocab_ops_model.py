@@ -220,6 +220,8 @@ def test_refusals(tmp_path):
         m.to_gpu(scores="int8")
     with pytest.raises(RuntimeError):
         m.softmax_loss([["w0001", "w0002"]])
+    with pytest.raises(ValueError, match="batch"):
+        m.softmax_loss([["w0001", "w0002"]], batch=0)
     m.save(str(tmp_path / "m"))
     with pytest.raises(ValueError):
         GlintWord2VecModel.load_sharded(str(tmp_path / "m"), device="cpu",
