@@ -8,12 +8,23 @@
 //   * rows in 8-bit floats (e4m3) with a power-of-two scale for each block of
 //     128 columns, and the product of such rows.
 //
-// All of them are matrix products whose one side is the table, so they share
-// one tile: 128 table rows x 128 sample rows per workgroup of four waves,
-// 64 x 64 per wave in 16x16 MFMA blocks, with the table's rows as the
-// instruction's M side.  A lane then holds four neighbouring table rows of
-// ONE sample, so the softmax's running maximum and sum stay in the lane until
-// the workgroup's last tile, and scores are stored 4 to an instruction.
+// The scores are a matrix product whose one side is the table.  Its rows are
+// the M side of the 16 x 16 matrix instructions: a lane then holds four
+// neighbouring table rows of ONE sample, so that the softmax's running maximum
+// and sum stay in the lane until the workgroup's last tile, coefficients are
+// written as the products with them read them, and scores are stored four to an
+// instruction.  Three kernels make them:
+//   resident_kernel  bf16 and 8-bit rows of up to 320 columns: the samples stay
+//                    in registers, and LDS is read for the table alone
+//   stream_kernel    up to 16 samples: the table goes from memory to registers
+//   tile_kernel      everything else: both sides by way of LDS
+// The gradient takes the vocabulary a piece at a time, its coefficients c in
+// memory between tile_kernel or resident_kernel and two products (grad_kernel).
+//
+// What bounds them, measured on one card: memory gives 4.8 TB/s in a copy; a
+// loop of bf16 instructions alone runs at 2.30 PFLOP/s, one of float32
+// instructions at 155 TFLOP/s; library products reach 1.35 PFLOP/s and 153
+// TFLOP/s at 8192^3.  Figures beside the kernels are for the sizes they name.
 
 #include <hip/hip_runtime.h>
 #include <pybind11/pybind11.h>
@@ -460,9 +471,10 @@ struct Sink {
       *reinterpret_cast<f32x4a4*>(o) = s;
   }
 
-  // An instruction that writes 16 rows of the output, 64 bytes each, is slow: half of the lanes swap one
-  // of two blocks with the other half, so that it writes 8 rows, 128 bytes
-  // each (4096 x 200k float32 scores: 1.08 ms without, 0.78 ms with).
+  // An instruction that writes 16 rows of the output, 64 bytes each, is slow:
+  // half of the lanes swap one of two blocks with the other half, so that it
+  // writes 8 rows, 128 bytes each (4096 x 200k float32 scores: 1.08 ms without,
+  // 0.78 ms with).
   template <int MR>
   __device__ __forceinline__ void take_store(const ScoreArgs& a, f32x4 (&acc)[MR][NS], int v1,
                                              int n1, bool cut) {
@@ -620,14 +632,22 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 
-// Rows of up to 32 KS columns of bf16 (or of 8 bits, on the table's side),
-// which on both sides start at multiples of 16 bytes.  A wave holds its 16 NS samples in
-// registers for the whole launch, so that LDS is read for the table alone:
+// Rows of up to 32 KS columns of bf16 (or of 8 bits, on the table's side), which
+// on both sides start at multiples of 16 bytes.  A wave holds its 16 NS samples
+// in registers for the whole launch, so that LDS is read for the table alone:
 // one fragment of 16 table rows feeds NS instructions.  Table tiles of kRows
-// rows are loaded straight into LDS, one ahead of the tile at work; two
-// workgroups fit a CU, and one's exponentials run beside the other's
-// products.  WN of the four waves have different samples, the others share
-// them and take different rows of the tile.
+// rows are loaded straight into LDS, up to three ahead of the tile at work; two
+// workgroups fit a CU, and one's exponentials run beside the other's products.
+// WN of the four waves have different samples, the others share them and take
+// different rows of the tile.
+// 8-bit rows are brought to bf16 with their scale: exact, while the instructions
+// on 8-bit operands lose bits inside (1.5e-5 to 2.8e-5 of the result).
+//   4096 samples, 1M x 300 bf16: 2.28 ms, 1.08 PFLOP/s (the matrix unit and
+//     the exponentials take turns); coefficients alone 3.1 ms
+//   1 sample: 107 us, 5.6 TB/s, bound by memory
+//   4096 queries, 200k x 300 in 8 bits, float32 scores: 0.77 ms
+//     (4.3 TB/s of stores, which bound it: a fill reaches 6.8)
+//   1 query of 1M x 300 in 8 bits: 57 us, 5.4 TB/s
 constexpr int resident_rows(int ks, int use, int wn, bool fp8) {
   // with stores, tiles of at most 20 KB: four of them fit, so that the stores
   // of several tiles, which are waited for in order with the loads, may be on
@@ -825,11 +845,19 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 
 // Rows of any width, both sides by way of LDS: 64 WV table rows x 16 NS WN
 // samples per workgroup, 64 x 16 NS per wave.  Steps of 64 bytes of a sample's
-// row go straight into LDS, three steps ahead of the one at work.  Both sides'
-// rows start at multiples of 16 bytes; 8-bit table rows are converted when
-// they are read from LDS, and their scales lie by block of columns, then row.
+// row (of each part) go straight into LDS, kAhead steps ahead of the one at
+// work.  Both sides' rows start at multiples of 16 bytes; 8-bit table rows are
+// converted when they are read from LDS, and their scales lie by block of
+// columns, then row.
+//   2047 samples, 100001 x 1024 bf16, coefficients: 0.54 ms, 0.78 PFLOP/s
+//     (LDS and barriers bound it)
+//   2047 samples, 30000 x 1024 float32 in parts, loss: 673 us, 187 TFLOP/s or
+//     1.12 PFLOP/s of bf16 (half of the matrix unit's time; all waves of a CU
+//     share one barrier a step)
+//   2000 samples, 3613 x 100 float32: 24 us, 60 TFLOP/s, one round of
+//     workgroups and its start
 template <int TW, int TC, int USE, int WV, int WN, int NS>
-__global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2) void tile_kernel(ScoreArgs a) {
+__global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   // float32 steps are long: two ahead do, and three workgroups fit a CU; the
   // small tile's are short
   constexpr int kWaves = WV * WN, MR = 4, P = Elem<TC>::parts;
@@ -1065,9 +1093,10 @@ __global__ __launch_bounds__(64 * WV * WN, TC == kSplit && WV * WN == 4 ? 1 : 2)
 }
 
 // Few samples: bound by the bytes of the table, which go from memory to the
-// registers of the one wave that needs them.  A wave takes 16 rows at a time,
-// eight loads of 16 bytes a lane ahead of the eight at work; the samples lie
-// in LDS as the instruction takes them.  Any type, size and alignment; VEC:
+// registers of the one wave that needs them (7 samples, 201905 x 860 float32:
+// 160 us, 4.3 TB/s).  A wave takes 16 rows at a time, eight loads of 16 bytes a
+// lane ahead of the eight at work; the samples lie in LDS as the instruction
+// takes them.  Any type, size and alignment; VEC:
 // table rows start at multiples of 16 bytes.
 template <int TW, int TC, int NS, int USE, bool VEC>
 __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
@@ -1176,8 +1205,9 @@ __global__ __launch_bounds__(256) void stream_kernel(ScoreArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Joins the parts of one sample's softmax and takes its target's score off:
-// one wave per sample, four to a workgroup.
+// Joins the parts of one sample's softmax and takes its target's score off: one
+// wave per sample, four to a workgroup.  Latency bounds it: two rows and some
+// hundred pairs a sample (4096 samples of 1M x 300: 7 us).
 // ---------------------------------------------------------------------------
 template <int T>
 __device__ __forceinline__ float elem(const char* p, int64_t i) {
@@ -1265,7 +1295,8 @@ struct GradArgs {
 };
 
 // Rows in parts of bf16: for each 32 columns 64 bytes of each part, and zeros
-// as in pack_kernel.  A thread takes 8 columns.
+// as in pack_kernel.  A thread takes 8 columns.  Bound by memory: 4 bytes read
+// and 6 written for each number.
 __global__ __launch_bounds__(256) void split_kernel(
     Rows h, const void* targets, int targets64, int64_t ignore, int64_t vocab, char* out,
     int64_t rows, int ldo) {
@@ -1315,13 +1346,16 @@ __global__ __launch_bounds__(256) void pack_kernel(
   }
 }
 
+// Bound by LDS and the matrix unit: 4096 samples, 1M x 300 bf16: 3.0 ms for
+// dh and 2.7 ms for dw, 0.83 and 0.91 PFLOP/s.
+//
 // Eight waves: WR times 16 J rows r, 8 / WR times 16 ND columns d.  With 256
 // rows and 32 ND columns narrow tables are read once and the coefficients, the
 // larger part, as often as there are tiles of d; fewer samples than that take
 // the forms with fewer rows.  Steps of 64 bytes of k (32 of bf16, 16 of
 // float32) go straight into LDS, kAhead steps ahead of the one at work: three,
-// two for float32, whose steps are long, or one where k is short: there several
-// workgroups a CU do more.
+// two for float32, whose steps are long, or one where k is short, as several
+// workgroups a CU do more there, and for kSplit, whose steps fill LDS.
 template <int T, bool DW, int ND, int WR, int J, int kAhead>
 __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
   constexpr int ES = Elem<T>::size, P = Elem<T>::parts, WD = 8 / WR;
@@ -1522,7 +1556,8 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
 }
 
 // A result from its parts: G lanes of a workgroup share a result, so that many
-// parts of few results are added at the same time, in a fixed order.
+// parts of few results are added at the same time, in a fixed order.  Bound by
+// memory, or by latency where there is little.
 template <int T, int G>
 __global__ __launch_bounds__(256) void sum_parts_kernel(
     const float* part, int splits, int64_t rows, int64_t ldp, int d, const float* scale0,
@@ -1560,7 +1595,8 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
 //
 // A workgroup takes 64 blocks of 128 columns that follow each other, four to
 // a group of lanes with all loads first; the position of the first one is the
-// only division by a length of 64 bits.
+// only division by a length of 64 bits.  Bound by memory: 1M x 300 bf16 in
+// 248 us, 3.7 TB/s (read and written).
 template <int T, bool TO_BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(
     Rows x, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
@@ -1634,7 +1670,8 @@ __global__ __launch_bounds__(256) void quantize_kernel(
 }
 
 // 8 columns to a lane, four times: rows of bf16 or f32 that follow each other
-// without a gap are written in one stream.
+// without a gap are written in one stream.  Bound by memory: 1M x 300 to
+// bfloat16 in 295 us, 3.1 TB/s, as lines of the output are shared by two rows.
 template <int TO>
 __global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char* out, int64_t ldo) {
   constexpr int kEach = 4;
@@ -2201,7 +2238,8 @@ static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int
   HIP_CHECK(hipGetLastError());
 }
 
-// The scales of 8-bit rows by block of columns, as the tile kernel takes them.
+// The scales of 8-bit rows by block of columns, as the tile kernel takes them: a
+// hundredth of the table's bytes.
 __global__ __launch_bounds__(256) void turn_scales_kernel(
     const uint8_t* scales, int64_t lds, int64_t rows, int blocks, uint8_t* out, int64_t ldo) {
   const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
