@@ -643,3 +643,57 @@ def test_gradients_are_not_captured(monkeypatch):
         out = S.softmax_loss(a, w, y)
     graph.replay()
     assert torch.equal(out, loss.detach())
+
+
+@gpu
+def test_two_threads_with_their_own_streams():
+    """Calls that run at the same time keep to their own workspaces."""
+    import threading
+    cases = [_inputs(300, 4000, 64, torch.bfloat16, seed=1),
+             _inputs(250, 50_000, 100, torch.float32, seed=2)]
+    one = torch.ones((), device="cuda")
+
+    def once(h, w, y):
+        loss, lse = S.softmax_loss_forward(h, w, y, gradient=True)
+        return (loss, *S.softmax_loss_backward(h, w, y, lse, one))
+    want = [once(*case) for case in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(case, ref):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                for a, b in zip(once(*case), ref):
+                    if not torch.equal(a, b):
+                        bad.append(len(case[0]))
+    threads = [threading.Thread(target=work, args=pair)
+               for pair in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d", [(300, 40_000, 100), (40, 300, 700)])
+def test_captured_float32(n, v, d):
+    """Parts of bfloat16 and small tiles, with new inputs on every replay."""
+    h, w, y = _inputs(n, v, d, torch.float32)
+    one = torch.ones((), device="cuda")
+
+    def once(a, b, t):
+        loss, lse = S.softmax_loss_forward(a, b, t, gradient=True)
+        return (loss, *S.softmax_loss_backward(a, b, t, lse, one))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once(h, w, y)
+    for k in range(4):
+        a, b, t = _inputs(n, v, d, torch.float32, seed=20 + k)
+        h.copy_(a), w.copy_(b), y.copy_(t)
+        graph.replay()
+        want = once(a, b, t)
+        torch.cuda.synchronize()
+        for x, z in zip(out, want):
+            assert torch.equal(x, z)
