@@ -869,6 +869,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   constexpr int kBytesS = TW == kFP8 ? kV : 0;
   constexpr int kInstr = (kBytesW + kBytesH) / 1024;          // loads of a whole wave
   constexpr int kEach = kInstr / kWaves, kMore = kInstr % kWaves;
+  constexpr bool kAmong = TC == kBF16 && NS >= 4;
   // the scales are one more load, of the last wave
   constexpr int kScaleWave = TW == kFP8 ? kWaves - 1 : -1;
   static_assert(kBytesW % 1024 == 0 && kBytesH % 1024 == 0 && kMore < kWaves, "");
@@ -1049,7 +1050,9 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
       wait_loads();
     }
     __syncthreads();
-    if (s + kAhead < all) fetch(at_buf == 0 ? kAhead : at_buf - 1);
+    const bool more = s + kAhead < all;
+    const int to = at_buf == 0 ? kAhead : at_buf - 1;
+    if (!kAmong && more) fetch(to);
     if (step == 0) {
 #pragma unroll
       for (int i = 0; i < MR; ++i)
@@ -1086,7 +1089,21 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
         for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
       }
     }
-    mma_all<TC>(fa, fb, acc);
+    if constexpr (kAmong) {
+      // loads among the products: in one block they would keep the matrix unit
+      // waiting
+      constexpr int kPerRow = (kFetches + MR - 1) / MR;
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        mma_row<TC>(fa[i], fb, acc[i]);
+        if (more)
+#pragma unroll
+          for (int k = i * kPerRow; k < (i + 1) * kPerRow && k < kFetches; ++k) fetch_one(to, k);
+      }
+      if (more) fetched();
+    } else {
+      mma_all<TC>(fa, fb, acc);
+    }
     if (++step == steps) finish_tile();
   }
   if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
