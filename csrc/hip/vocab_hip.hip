@@ -614,6 +614,9 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ void wait_all() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 // load_lds16 with 4 bytes a lane.
 __device__ __forceinline__ void load_lds4(const char* p, uint32_t offset, uint32_t lds) {
   const uint64_t at = (uint64_t)p;
@@ -869,7 +872,10 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   constexpr int kBytesS = TW == kFP8 ? kV : 0;
   constexpr int kInstr = (kBytesW + kBytesH) / 1024;          // loads of a whole wave
   constexpr int kEach = kInstr / kWaves, kMore = kInstr % kWaves;
-  constexpr bool kAmong = TC == kBF16 && NS >= 4;
+  // kMid: the barrier in the middle of a step; coefficients would spill more
+  // registers with it, and gain nothing.  kAmong: loads among the products.
+  constexpr bool kMid = TW == kBF16 && NS == 8 && USE != kCoef;
+  constexpr bool kAmong = TC == kBF16 && NS >= 4 && !kMid;
   // the scales are one more load, of the last wave
   constexpr int kScaleWave = TW == kFP8 ? kWaves - 1 : -1;
   static_assert(kBytesW % 1024 == 0 && kBytesH % 1024 == 0 && kMore < kWaves, "");
@@ -938,7 +944,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   sink.start(a, n);
   f32x4 acc[MR][NS];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i)
+  for (int i = 0; i < kAhead + kMid; ++i)
     if (i < all) fetch(i);
   int tile = t0, step = 0, at_buf = 0;
   auto finish_tile = [&]() INLINE {
@@ -1038,6 +1044,76 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
       if (++step == steps) finish_tile();
     }
     wait_loads();
+    if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
+    return;
+  }
+  if constexpr (kMid) {
+    // The same with one product a step: its second half runs beside the next
+    // step's first reads and the loads of four steps on (2047 samples, 100001 x
+    // 1024: loss 512 us, with the barrier at the step's start 527).
+    static_assert(kMore == 0 && kEach == MR, "");
+    u32x4 fa[MR], fb[NS], na[MR];
+    auto read_a = [&](int buf) INLINE {
+      const char* q = lds[buf] + wv * 64 * 64 + at;
+#pragma unroll
+      for (int i = 0; i < MR; ++i) na[i] = *reinterpret_cast<const u32x4*>(q + i * 16 * 64);
+    };
+    auto mma = [&](int j) INLINE {
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, fa[i]), __builtin_bit_cast(bf16x8, fb[j]), acc[i][j], 0, 0, 0);
+    };
+    if (kAhead < all) wait_loads_but<kAhead * kEach>();
+    else wait_loads();
+    __syncthreads();
+    if (all > 0) read_a(0);
+    for (int64_t s = 0; s < all; ++s) {
+      if (step == 0) {
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int j = 0; j < NS; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      const char* lh = lds[at_buf] + kBytesW + wn * (16 * NS) * kWideH + at;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) fb[j] = *reinterpret_cast<const u32x4*>(lh + j * 16 * 64);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) fa[i] = na[i];
+      if (step + 1 == steps && (a.h.kb & 63) != 0) {
+        // columns past the last one, whatever they hold
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int have = a.h.kb - (step * kWideH + g * 16 + q * 4);
+          const uint32_t keep = have >= 4 ? 0xffffffffu : have <= 0 ? 0u : (1u << (8 * have)) - 1;
+#pragma unroll
+          for (int i = 0; i < MR; ++i) fa[i][q] &= keep;
+#pragma unroll
+          for (int j = 0; j < NS; ++j) fb[j][q] &= keep;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NS / 2; ++j) mma(j);
+      __builtin_amdgcn_sched_barrier(0);
+      const int to = at_buf;
+      const bool more = s + kAhead + 1 < all;
+      at_buf = at_buf == kAhead ? 0 : at_buf + 1;
+      if (s + 1 < all) {
+        // step s + 1 has arrived, two more may be on their way
+        if (s + kAhead < all) wait_loads_but<(kAhead - 1) * kEach>();
+        else wait_loads();
+        wait_lds();
+        __syncthreads();
+        read_a(at_buf);
+      }
+#pragma unroll
+      for (int j = NS / 2; j < NS; ++j) {
+        mma(j);
+        if (more) fetch_one(to, j - NS / 2);
+      }
+      if (more) fetched();
+      if (++step == steps) finish_tile();
+    }
     if constexpr (USE == kLoss) sink.template finish_loss<WV, kWaves>(a, &lds[0][0], split, n0);
     return;
   }
