@@ -9,8 +9,10 @@ words ``y`` [N]
 
 The scores [N, V] are never kept: the loss is one pass over the table with a
 running maximum and sum, and the gradient takes the vocabulary in pieces.
-Products and sums are held in 32 bits; for bfloat16 tables the gradient's
-coefficients are rounded to bfloat16 before the products with the rows.
+Sums are held in 32 bits; for bfloat16 tables the gradient's coefficients are
+rounded to bfloat16 before the products with the rows.  float32 products of many
+samples are made of three bfloat16 parts of each number, which loses no more
+than float32's own rounding.
 
 Every function runs on the current stream of the tensors' device, allocates
 its workspace from torch's allocator for the one call, and does not
