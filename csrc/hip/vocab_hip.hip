@@ -600,11 +600,16 @@ __device__ __forceinline__ float col_scale_of(const ScoreArgs& a, int v) {
 
 // 16 bytes a lane from global memory straight into LDS, 1 KB from `lds` on.
 // The hardware counts it as a load; wait_loads() waits for it.
+// Two rules on wait states hold here that neither the hardware nor, in inline
+// assembly, the compiler sees to: one between a scalar write of M0 and the load,
+// and five between a vector instruction's write of a scalar register and a load
+// with that address (base may come from v_readfirstlane).  The write of M0 is
+// one of the five, s_nop 3 the other four.
 __device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint32_t lds) {
   const uint64_t at = (uint64_t)p;
   const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void wait_loads() {
@@ -622,7 +627,7 @@ __device__ __forceinline__ void load_lds4(const char* p, uint32_t offset, uint32
   const uint64_t at = (uint64_t)p;
   const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
                :: "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
 // Waits until only the last N loads and stores are outstanding: they end in
