@@ -1315,10 +1315,10 @@ __device__ __forceinline__ float elem(const char* p, int64_t i) {
 
 template <int T>
 __global__ __launch_bounds__(256) void loss_join_kernel(
-    Rows w, Rows h, const float2* part, int splits, int64_t ldp,
+    int64_t block0, Rows w, Rows h, const float2* part, int splits, int64_t ldp,
     const void* targets, int targets64, int64_t ignore, float* loss, float* lse) {
   const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t n = (block0 + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (n >= h.rows) return;
   float top = -INFINITY, sum = 0.f;
   for (int s = lane; s < splits; s += 64) {
@@ -1658,13 +1658,13 @@ __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs a) {
 // memory, or by latency where there is little.
 template <int T, int G>
 __global__ __launch_bounds__(256) void sum_parts_kernel(
-    const float* part, int splits, int64_t rows, int64_t ldp, int d, const float* scale0,
-    const float* scale1, char* out) {
+    int64_t block0, const float* part, int splits, int64_t rows, int64_t ldp, int d,
+    const float* scale0, const float* scale1, char* out) {
   constexpr int kEach = 256 / G;
   __shared__ float sums[G][kEach];
   const int at = threadIdx.x % kEach, group = threadIdx.x / kEach;
   const int64_t total = rows * d;
-  const int64_t i = (int64_t)blockIdx.x * kEach + at;
+  const int64_t i = (block0 + blockIdx.x) * kEach + at;
   float s = 0.f;
   if (i < total) {
     const int64_t r = i / d, c = i - r * d;
@@ -1697,10 +1697,10 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
 // 248 us, 3.7 TB/s (read and written).
 template <int T, bool TO_BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(
-    Rows x, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
+    int64_t block0, Rows x, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
   constexpr int kEach = 4;
   const int sub = threadIdx.x & 15;
-  const int64_t first = (int64_t)blockIdx.x * (16 * kEach);
+  const int64_t first = (block0 + blockIdx.x) * (16 * kEach);
   const int64_t row0 = first / blocks;
   const int in0 = (int)(first - row0 * blocks);
   int64_t row[kEach];
@@ -1771,10 +1771,11 @@ __global__ __launch_bounds__(256) void quantize_kernel(
 // without a gap are written in one stream.  Bound by memory: 1M x 300 to
 // bfloat16 in 295 us, 3.1 TB/s, as lines of the output are shared by two rows.
 template <int TO>
-__global__ __launch_bounds__(256) void dequantize_kernel(Rows x, int cols, char* out, int64_t ldo) {
+__global__ __launch_bounds__(256) void dequantize_kernel(int64_t block0, Rows x, int cols, char* out,
+                                                        int64_t ldo) {
   constexpr int kEach = 4;
   const int chunks = (cols + 7) / 8;
-  const int64_t first = (int64_t)blockIdx.x * (256 * kEach);
+  const int64_t first = (block0 + blockIdx.x) * (256 * kEach);
   const int64_t row0 = first / chunks;
   const int in0 = (int)(first - row0 * chunks);
   int64_t row[kEach];
@@ -1867,13 +1868,22 @@ static Rows make_rows(uintptr_t p, int64_t ld_elems, int64_t rows, int64_t cols,
   return r;
 }
 
-static int grid_of(int64_t blocks) {
-  if (blocks < 1 || blocks > 0x7fffffff) throw std::runtime_error("grid out of range");
+// Workgroups of a launch.  One of 2^32 threads or more would run with what is
+// left of their number in 32 bits, and report nothing.
+static int grid_of(int64_t blocks, int threads) {
+  if (blocks < 1 || blocks * threads > 0xffffffff) throw std::runtime_error("too large a launch");
   return (int)blocks;
 }
 
-static int score_grid(const ScoreArgs& a) {
-  return grid_of((int64_t)a.tiles_n * a.splits);
+// Launches of at most 2^31 threads, with the number of the first workgroup.
+template <typename K, typename... A>
+static void launch_all(K kernel, int64_t blocks, hipStream_t stream, const A&... args) {
+  for (int64_t b = 0; b < blocks; b += 1 << 23)
+    kernel<<<(int)std::min<int64_t>(1 << 23, blocks - b), 256, 0, stream>>>(b, args...);
+}
+
+static int score_grid(const ScoreArgs& a, int threads) {
+  return grid_of((int64_t)a.tiles_n * a.splits, threads);
 }
 
 // How many workgroups of a kernel the card holds at a time.
@@ -1918,9 +1928,9 @@ template <int KS, int NS, int WN, int USE, bool FP8>
 static void launch_resident_k(ScoreArgs& a, hipStream_t stream) {
   constexpr auto kernel = resident_kernel<KS, NS, WN, USE, FP8>;
   static const int slots = slots_of(kernel, 256, 0);
-  a.tiles_n = grid_of((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
+  a.tiles_n = (int)((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
   cut(a, resident_rows(KS, USE, WN, FP8), slots);
-  kernel<<<score_grid(a), 256, 0, stream>>>(a);
+  kernel<<<score_grid(a, 256), 256, 0, stream>>>(a);
 }
 
 template <int USE, bool FP8>
@@ -1943,9 +1953,9 @@ template <int TW, int TC, int USE, int WV, int WN, int NS>
 static void launch_tile_k(ScoreArgs& a, hipStream_t stream) {
   constexpr auto kernel = tile_kernel<TW, TC, USE, WV, WN, NS>;
   static const int slots = slots_of(kernel, 64 * WV * WN, 0);
-  a.tiles_n = grid_of((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
+  a.tiles_n = (int)((a.n + 16 * NS * WN - 1) / (16 * NS * WN));
   cut(a, 64 * WV, slots);
-  kernel<<<score_grid(a), 64 * WV * WN, 0, stream>>>(a);
+  kernel<<<score_grid(a, 64 * WV * WN), 64 * WV * WN, 0, stream>>>(a);
 }
 
 template <int TW, int TC, int USE>
@@ -1986,9 +1996,9 @@ static void launch_stream(ScoreArgs& a, hipStream_t stream) {
   const auto kernel = a.w.align == 16 ? stream_kernel<TW, TC, NS, USE, true>
                                       : stream_kernel<TW, TC, NS, USE, false>;
   const int lds = (int)stream_bytes(a, NS, TW == kFP8);
-  a.tiles_n = grid_of((a.n + 16 * NS - 1) / (16 * NS));
+  a.tiles_n = (int)((a.n + 16 * NS - 1) / (16 * NS));
   cut(a, 64, slots_of(kernel, 256, lds));
-  kernel<<<score_grid(a), 256, lds, stream>>>(a);
+  kernel<<<score_grid(a, 256), 256, lds, stream>>>(a);
 }
 
 // The kernel for scores of these samples and table rows.
@@ -2069,13 +2079,9 @@ static void softmax_loss(uintptr_t h, int64_t ldh, int64_t n, uintptr_t w, int64
       else launch_any<kF32, kF32, kLoss>(a, d, stream);
       parts += a.splits;
     }
-    const int joins = grid_of((n + 3) / 4);
-    if (type == kBF16)
-      loss_join_kernel<kBF16><<<joins, 256, 0, stream>>>(rw, rh, (const float2*)part, parts, n,
-          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
-    else
-      loss_join_kernel<kF32><<<joins, 256, 0, stream>>>(rw, rh, (const float2*)part, parts, n,
-          (const void*)targets, targets64, ignore, (float*)loss, (float*)lse);
+    launch_all(type == kBF16 ? loss_join_kernel<kBF16> : loss_join_kernel<kF32>, (n + 3) / 4,
+               stream, rw, rh, (const float2*)part, parts, n, (const void*)targets, targets64,
+               ignore, (float*)loss, (float*)lse);
   }
   if (reduce)      // 1: sum, 2: mean
     loss_reduce_kernel<<<1, 1024, 0, stream>>>((const float*)loss, (const void*)targets,
@@ -2088,8 +2094,8 @@ static void launch_sum_parts(const float* part, int splits, int64_t rows, int64_
                              const float* const (&scale)[2], int is_bf16, char* out,
                              hipStream_t stream) {
   auto go = [&](auto kernel, int each) {
-    kernel<<<grid_of((rows * d + each - 1) / each), 256, 0, stream>>>(part, splits, rows, ldp,
-                                                                     (int)d, scale[0], scale[1], out);
+    launch_all(kernel, (rows * d + each - 1) / each, stream, part, splits, rows, ldp, (int)d,
+               scale[0], scale[1], out);
   };
   if (splits >= 16)
     is_bf16 ? go(sum_parts_kernel<kBF16, 16>, 16) : go(sum_parts_kernel<kF32, 16>, 16);
@@ -2168,9 +2174,9 @@ static std::pair<int, int> softmax_plan(int64_t n, int64_t chunk, int64_t d, int
 
 template <int T, bool DW, int ND, int WR, int J, int kAhead>
 static void launch_grad_k(GradArgs& b, hipStream_t stream) {
-  b.tiles_r = grid_of((b.r + 16 * J * WR - 1) / (16 * J * WR));
+  b.tiles_r = (int)((b.r + 16 * J * WR - 1) / (16 * J * WR));
   const int64_t tiles = (int64_t)b.tiles_d * b.tiles_r;
-  const int blocks = grid_of(tiles * b.splits);
+  const int blocks = grid_of(tiles * b.splits, 512);
   grad_kernel<T, DW, ND, WR, J, kAhead><<<blocks, 512, 0, stream>>>(b);
 }
 
@@ -2304,10 +2310,9 @@ static void quantize_rows(uintptr_t x, int64_t ldx, int64_t rows, int64_t cols, 
     throw std::runtime_error("bad layout of the values");
   const Rows r = make_rows(x, ldx, rows, cols, is_bf16 ? 2 : 4);
   const int blocks = (int)((cols + 127) / 128);
-  const int grid = grid_of((rows * blocks + 63) / 64);
   auto go = [&](auto kernel) {
-    kernel<<<grid, 256, 0, stream>>>(r, blocks, (char*)values, ldv,
-                                     (uint8_t*)scales, lds);
+    launch_all(kernel, (rows * blocks + 63) / 64, stream, r, blocks, (char*)values, ldv,
+               (uint8_t*)scales, lds);
   };
   if (is_bf16) to_bf16 ? go(quantize_kernel<kBF16, true>) : go(quantize_kernel<kBF16, false>);
   else to_bf16 ? go(quantize_kernel<kF32, true>) : go(quantize_kernel<kF32, false>);
@@ -2330,9 +2335,8 @@ static void dequantize_rows(uintptr_t values, int64_t ldv, uintptr_t scales, int
   hipStream_t stream = (hipStream_t)stream_ptr;
   if (out % 16 != 0) throw std::runtime_error("bad layout of the output");
   const Rows r = make_fp8(values, ldv, scales, lds, rows, cols);
-  const int grid = grid_of((rows * ((cols + 7) / 8) + 1023) / 1024);
-  if (is_bf16) dequantize_kernel<kBF16><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
-  else dequantize_kernel<kF32><<<grid, 256, 0, stream>>>(r, (int)cols, (char*)out, ldo);
+  launch_all(is_bf16 ? dequantize_kernel<kBF16> : dequantize_kernel<kF32>,
+             (rows * ((cols + 7) / 8) + 1023) / 1024, stream, r, (int)cols, (char*)out, ldo);
   HIP_CHECK(hipGetLastError());
 }
 
@@ -2379,8 +2383,8 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
       part.p += v0 * part.ld;
       part.scales += v0 * part.lds;
       part.rows = rows;
-      dequantize_kernel<kBF16><<<grid_of((rows * ((k + 7) / 8) + 1023) / 1024), 256, 0, stream>>>(
-          part, (int)k, (char*)wide, dp);
+      launch_all(dequantize_kernel<kBF16>, (rows * ((k + 7) / 8) + 1023) / 1024, stream, part,
+                 (int)k, (char*)wide, dp);
       a.w = make_rows(wide, dp, rows, k, 2);
       a.v_end = (int)rows;
       a.splits = 1 << 20;
@@ -2390,7 +2394,7 @@ static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t value
     }
   } else if (turned) {
     const int64_t ldo = (n + 255) / 256 * 256;
-    turn_scales_kernel<<<grid_of(ldo / 256), 256, 0, stream>>>(
+    turn_scales_kernel<<<grid_of(ldo / 256, 256), 256, 0, stream>>>(
         a.w.scales, a.w.lds, n, (int)((k + 127) / 128), (uint8_t*)turned, ldo);
     a.w.scales = (const uint8_t*)turned;
     a.w.lds = ldo;
