@@ -293,7 +293,8 @@ template <int USE, int TC, int NS>
 struct Sink {
   float top[NS], sum[NS];                      // kLoss
   bool far;                                    // of the wave: past kFar
-  float lse2[NS], gg[NS];                      // kCoef; lse in powers of two
+  // kCoef; lse in powers of two, or itself where `far`
+  float lse2[NS], gg[NS];
   int yy[NS];                                  // -1: no loss
 
   __device__ __forceinline__ void start(const ScoreArgs& a, int64_t n) {
@@ -311,7 +312,7 @@ struct Sink {
           const int64_t y = target_of(a.targets, a.targets64, m);
           if (y != a.ignore && y >= 0 && y < a.vocab) {
             yy[j] = (int)y;
-            lse2[j] = a.lse[m] * kLog2e;
+            lse2[j] = a.lse[m];
             gg[j] = a.grad ? a.grad[m] : 1.f;
           }
         }
@@ -320,6 +321,9 @@ struct Sink {
 #pragma unroll
       for (int j = 0; j < NS; ++j) f |= fabsf(lse2[j]) > kFar;
       far = __any(f);
+      if (!far)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) lse2[j] *= kLog2e;
     }
   }
 
@@ -437,10 +441,11 @@ struct Sink {
       for (int i = 0; i < MR; ++i) {
         f32x4 c = acc[i][j];
         if (far) {
-          // the logarithm's own rounding may pass 0 here
+          // the difference first: it is exact for the scores that matter, while
+          // lse in powers of two would be off by whole powers; lse's own
+          // rounding may pass 0
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            c[e] = __builtin_amdgcn_exp2f(fminf(c[e] * kLog2e - lse2[j], 0.f));
+          for (int e = 0; e < 4; ++e) c[e] = exp_of(fminf(c[e] - lse2[j], 0.f));
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)

@@ -1,0 +1,87 @@
+"""Softmax cross entropy where numbers stop being ordinary: rows far from 0
+beside rows that are not finite, infinite table entries, batches without a
+target, and results of more than 2^30 numbers."""
+import math
+
+import pytest
+import torch
+
+from glint_word2vec_amd.ops import softmax as S
+from test_softmax_loss import _near, _reference
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+NEVER = 1 << 62, 1 << 62
+
+# (samples, columns, type, float32 in parts of bfloat16): the kernel with
+# resident samples, tiles of 256 x 32 and 128 x 128, float32 tiles of 64 x 64
+# and 128 x 128, and parts
+FORMS = [(40, 24, torch.bfloat16, False), (30, 400, torch.bfloat16, False),
+         (90, 400, torch.bfloat16, False), (40, 24, torch.float32, False),
+         (900, 24, torch.float32, False), (40, 24, torch.float32, True),
+         (200, 130, torch.float32, True)]
+forms = pytest.mark.parametrize("n,d,dtype,parts", FORMS)
+
+
+@pytest.fixture(autouse=True)
+def _as_asked(request, monkeypatch):
+    parts = getattr(request.node, "callspec", None) and \
+        request.node.callspec.params.get("parts")
+    if parts is not None:
+        for name in ("_SPLIT_LOSS", "_SPLIT_GRAD"):
+            monkeypatch.setattr(S, name, (0, 0) if parts else NEVER)
+
+
+def _far(n, d, dtype):
+    """300 words and n samples.  Column 0 of the words is k / 64, which
+    bfloat16 holds, and rows 3, 5, 7 and 8 are a power of two there and 0
+    elsewhere: scores are exact, 2^16 apart or more, and up to 7e20."""
+    g = torch.Generator().manual_seed(n + d)
+    h = torch.randn(n, d, generator=g) * 1.2 / d ** 0.25
+    w = torch.randn(300, d, generator=g) * 1.2 / d ** 0.25
+    w[:, 0] = torch.randperm(300, generator=g).sub(150) / 64
+    h, w = h.to(dtype), w.to(dtype)
+    y = torch.randint(0, 300, (n,), generator=g)
+    rows = [3, 5, 7, 8]
+    h[rows] = 0
+    h[rows, 0] = torch.tensor([2.0 ** 22, -2.0 ** 22, 2.0 ** 62, -2.0 ** 30],
+                              dtype=dtype)
+    y[3] = w[:, 0].argmax()                 # certain and right: no gradient
+    return h, w, y, rows
+
+
+def _far_reference(h, w, y, rows):
+    """As _reference with a gradient of 1 a row, but where a row's scores and
+    their distances are exact its probabilities are 1 and 0 and off by
+    nothing."""
+    out = list(_reference(h, w, y, grad=torch.ones(())))
+    bf16 = h.dtype == torch.bfloat16
+    normal = torch.ones(len(h), dtype=torch.bool)
+    normal[rows] = False
+    part = _reference(h[normal], w, y[normal], grad=torch.ones(()))
+    step = 2.0 ** -8 if bf16 else U
+    hh, ww = h.double(), w.double()
+    c = torch.softmax(hh[rows] @ ww.T, 1)
+    assert ((c == 0) | (c == 1)).all()
+    c[torch.arange(len(rows)), y[rows]] -= 1
+    # dh: two terms at most; dw: those of the other rows and one for each row
+    out[6][normal] = part[6]
+    out[6][rows] = 4 * U * (c.abs() @ ww.abs()) + step * (c @ ww).abs() + 1e-38
+    out[7] = part[7] + (2 * (len(h) + 2) * U + step) * (c.abs().T @ hh[rows].abs())
+    return out
+
+
+@gpu
+@forms
+def test_gradients_far_from_0(n, d, dtype, parts):
+    """|lse| above 1e6, where the exponent is taken another way."""
+    h, w, y, rows = _far(n, d, dtype)
+    want = _far_reference(h, w, y, rows)
+    a, b, t = h.cuda(), w.cuda(), y.cuda()
+    loss, lse = S.softmax_loss_forward(a, b, t, gradient=True)
+    assert torch.equal(lse[rows].double().cpu(), want[1][rows])
+    dh, dw = S.softmax_loss_backward(a, b, t, lse,
+                                     torch.ones((), device="cuda"))
+    _near(dh, want[4], want[6], "dh")
+    _near(dw, want[5], want[7], "dw")
+    assert (dh[3] == 0).all()
