@@ -443,9 +443,12 @@ struct Sink {
         if (far) {
           // the difference first: it is exact for the scores that matter, while
           // lse in powers of two would be off by whole powers; lse's own
-          // rounding may pass 0
+          // rounding may pass 0.  Not fminf(), which would drop a NaN
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = exp_of(fminf(c[e] - lse2[j], 0.f));
+          for (int e = 0; e < 4; ++e) {
+            const float below = c[e] - lse2[j];
+            c[e] = exp_of(below > 0.f ? 0.f : below);
+          }
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)

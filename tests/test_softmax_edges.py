@@ -85,3 +85,32 @@ def test_gradients_far_from_0(n, d, dtype, parts):
     _near(dh, want[4], want[6], "dh")
     _near(dw, want[5], want[7], "dw")
     assert (dh[3] == 0).all()
+
+
+@gpu
+@forms
+def test_rows_that_are_not_finite_beside_far_ones(n, d, dtype, parts):
+    """NaN, scores that overflow to -inf for every word, and scores that
+    overflow to both sides, in one wave with rows far from 0."""
+    h, w, y, rows = _far(n, d, dtype)
+    w[:, 1] = -2.0 ** 100
+    w[:, 2] = torch.where(torch.arange(300) % 2 == 0, 2.0 ** 100, -2.0 ** 100)
+    bad = [9, 11, 13]
+    h[:, 1:3] = 0
+    h[bad] = 0
+    h[9, 5] = math.nan
+    h[11, 1] = 2.0 ** 100
+    h[13, 2] = 2.0 ** 100
+    good = torch.ones(n, dtype=torch.bool)
+    good[bad] = False
+    kept = [i - sum(j < i for j in bad) for i in rows]
+    want = _far_reference(h[good], w, y[good], kept)
+    a, b, t = h.cuda(), w.cuda(), y.cuda()
+    loss, lse = S.softmax_loss_forward(a, b, t, gradient=True)
+    assert loss[bad].isnan().all() and lse[[9, 13]].isnan().all()
+    assert lse[11] == -math.inf
+    dh, dw = S.softmax_loss_backward(a, b, t, lse,
+                                     torch.ones((), device="cuda"))
+    assert dh[bad].isnan().all()
+    assert dw.isnan().all()
+    _near(dh[good], want[4], want[6], "dh")
