@@ -1357,6 +1357,8 @@ __global__ __launch_bounds__(256) void loss_join_kernel(
 
 // Sum or mean over the samples that count, in 64 bits and a fixed order.
 // factor = 1 / count for the mean, 1 for the sum; result = the sum times it.
+// The mean of none is NaN, and its factor 0: no gradient, where 0 times the
+// factor would be NaN too.
 __global__ __launch_bounds__(1024) void loss_reduce_kernel(
     const float* loss, const void* targets, int targets64, int64_t ignore,
     int64_t n, int mean, float* result, float* factor) {
@@ -1374,7 +1376,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(
     for (int i = 1; i < 16; ++i) s += sums[i], c += counts[i];
     const double f = mean ? 1.0 / (double)c : 1.0;
     *result = (float)(s * f);
-    *factor = (float)f;
+    *factor = c || !mean ? (float)f : 0.f;
   }
 }
 

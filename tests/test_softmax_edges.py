@@ -114,3 +114,20 @@ def test_rows_that_are_not_finite_beside_far_ones(n, d, dtype, parts):
     assert dh[bad].isnan().all()
     assert dw.isnan().all()
     _near(dh[good], want[4], want[6], "dh")
+
+
+@gpu
+@pytest.mark.parametrize("n,v,d,dtype,parts", [
+    (40, 300, 24, torch.bfloat16, False), (40, 300, 24, torch.float32, False),
+    (2000, 200, 64, torch.bfloat16, False), (600, 90, 40, torch.float32, True),
+    (2000, 200, 64, torch.float32, False), (5, 1000, 700, torch.bfloat16, False)])
+def test_mean_of_no_targets(n, v, d, dtype, parts):
+    """NaN, but ignored targets give no gradient."""
+    g = torch.Generator().manual_seed(n)
+    h = torch.randn(n, d, generator=g).to(dtype).cuda().requires_grad_()
+    w = torch.randn(v, d, generator=g).to(dtype).cuda().requires_grad_()
+    y = torch.full((n,), -1, device="cuda")
+    loss = S.softmax_loss(h, w, y)
+    assert math.isnan(loss.item())
+    loss.backward()
+    assert (h.grad == 0).all() and (w.grad == 0).all()
