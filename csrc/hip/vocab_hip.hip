@@ -120,18 +120,22 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-// The three parts of x.  What is not finite is all in the first.  Where bf16
-// would round x past the largest number, the parts are cut off instead of
-// rounded: all of x's sign, so that no sum of them passes x.
+// The three parts of x.  What is not finite is in the last, which meets the
+// other side's first part alone: infinity times that has the product's sign,
+// while the other parts may be 0 or of the other sign.  Its first part is 1 of
+// its sign, for what is infinite on the other side.  Where bf16 would round x
+// past the largest number, the parts are cut off instead of rounded: all of x's
+// sign, so that no sum of them passes x.
 __device__ __forceinline__ void split(float x, float& hi, float& mid, float& lo) {
   const uint32_t u = __float_as_uint(x);
   const bool finite = (u & 0x7f800000u) != 0x7f800000u;
   hi = (float)(__bf16)x;
   const bool cut = finite && __builtin_isinf(hi);
   if (cut) hi = __uint_as_float(u & 0xffff0000u);
+  if (!finite) hi = __builtin_copysignf(1.f, x);
   const float rest = finite ? x - hi : 0.f;
   mid = cut ? __uint_as_float(__float_as_uint(rest) & 0xffff0000u) : (float)(__bf16)rest;
-  lo = rest - mid;
+  lo = finite ? rest - mid : x;
 }
 __device__ __forceinline__ void split4(const f32x4& x, u32x2 (&to)[3]) {
   f32x4 t[3];

@@ -265,9 +265,10 @@ def softmax_loss(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
     the loss [N].  Losses are float32.  Targets equal to ``ignore_index``
     count nothing and give no gradient (the mean of none is NaN).  Any other
     target outside [0, V) cannot be refused without waiting for the GPU: its
-    loss is NaN, and it gives no gradient.  Rows whose scores are not finite
-    give NaN.  A call that needs gradients is refused while a graph is being
-    captured: softmax_loss_forward and softmax_loss_backward can be."""
+    loss is NaN, and it gives no gradient.  A score of NaN or +inf makes its row
+    NaN, and so does one of -inf for every word; otherwise a score of -inf is a
+    probability of 0.  A call that needs gradients is refused while a graph is
+    being captured: softmax_loss_forward and softmax_loss_backward can be."""
     if reduction not in _REDUCE:
         raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got "
                          f"{reduction!r}")

@@ -116,6 +116,59 @@ def test_rows_that_are_not_finite_beside_far_ones(n, d, dtype, parts):
     _near(dh[good], want[4], want[6], "dh")
 
 
+def _with_minus_infinity(n, d, dtype):
+    """Words 17 and 299 have -inf where every sample is positive; and what the
+    formula gives without them."""
+    g = torch.Generator().manual_seed(n)
+    h = (torch.randn(n, d, generator=g) * 1.2 / d ** 0.25).to(dtype)
+    w = (torch.randn(300, d, generator=g) * 1.2 / d ** 0.25).to(dtype)
+    y = torch.randint(0, 17, (n,), generator=g)
+    h[:, 6] = h[:, 6].abs() + 0.125
+    w[17, 6], w[299, 6] = -math.inf, -math.inf
+    others = [i for i in range(300) if i not in (17, 299)]
+    want = _reference(h, w[others], y, grad=torch.ones(()))
+    return h.cuda(), w.cuda(), y.cuda(), others, want
+
+
+@gpu
+@forms
+def test_table_entries_of_minus_infinity(n, d, dtype, parts):
+    """A score of -inf is a probability of 0, in every form: the loss is finite,
+    and the samples' gradients are NaN where 0 is multiplied by the entry, as
+    in the formula."""
+    h, w, y, _, want = _with_minus_infinity(n, d, dtype)
+    loss, lse = S.softmax_loss_forward(h, w, y, gradient=True)
+    _near(loss, want[0], want[2], "loss")
+    _near(lse, want[1], want[3], "lse")
+    dh, _ = S.softmax_loss_backward(h, w, y, lse,
+                                    torch.ones((), device="cuda"))
+    assert dh[:, 6].isnan().all()
+    rest = [k for k in range(d) if k != 6]
+    _near(dh[:, rest], want[4][:, rest], want[6][:, rest], "dh")
+    # a target that cannot be: its loss is infinite
+    y[2] = 17
+    assert S.softmax_loss_forward(h, w, y)[0][2] == math.inf
+
+
+@gpu
+@forms
+def test_infinite_on_both_sides(n, d, dtype, parts):
+    """Infinity times -infinity is a score of -inf; of one sign, or beside an
+    infinity of the other sign, the row is NaN."""
+    h, w, y, _, want = _with_minus_infinity(n, d, dtype)
+    h[4], h[5], h[8] = 0, 0, 0
+    w[:, 6] = -math.inf
+    w[:17, 6] = -2.0
+    h[4, 6], h[5, 6], h[8, 6] = math.inf, -math.inf, math.nan
+    loss, lse = S.softmax_loss_forward(h, w, y)
+    # row 4: -inf for every word; row 5: +inf
+    assert lse[4] == -math.inf and loss[[4, 5, 8]].isnan().all()
+    assert lse[[5, 8]].isnan().all()
+    rest = [i for i in range(n) if i not in (4, 5, 8)]
+    r = _reference(h[rest], w[:17], y[rest])
+    _near(loss[rest], r[0], r[2], "loss")
+
+
 @gpu
 @pytest.mark.parametrize("n,v,d,dtype,parts", [
     (40, 300, 24, torch.bfloat16, False), (40, 300, 24, torch.float32, False),
