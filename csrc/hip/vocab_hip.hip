@@ -300,6 +300,7 @@ struct Sink {
   // kCoef; lse in powers of two, or itself where `far`
   float lse2[NS], gg[NS];
   int yy[NS];                                  // -1: no loss
+  bool some;                                   // of the wave: without a loss
 
   __device__ __forceinline__ void start(const ScoreArgs& a, int64_t n) {
     if constexpr (USE == kLoss) {
@@ -321,10 +322,11 @@ struct Sink {
           }
         }
       }
-      bool f = false;
+      bool f = false, none = false;
 #pragma unroll
-      for (int j = 0; j < NS; ++j) f |= fabsf(lse2[j]) > kFar;
+      for (int j = 0; j < NS; ++j) f |= fabsf(lse2[j]) > kFar, none |= yy[j] < 0;
       far = __any(f);
+      some = __any(none);
       if (!far)
 #pragma unroll
         for (int j = 0; j < NS; ++j) lse2[j] *= kLog2e;
@@ -463,7 +465,11 @@ struct Sink {
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[e] -= first + e == yy[j] ? 1.f : 0.f;
         }
-        c *= gg[j];      // 0 without a loss: h is zeros there
+        c *= gg[j];      // 0 without a loss: h is zeros there,
+        if (some) {      // but 0 times a table's infinity is NaN
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = yy[j] >= 0 ? c[e] : 0.f;
+        }
         if (cut) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[e] = first + e < a.v_end ? c[e] : 0.f;

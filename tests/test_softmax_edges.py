@@ -152,6 +152,22 @@ def test_table_entries_of_minus_infinity(n, d, dtype, parts):
 
 @gpu
 @forms
+def test_words_of_minus_infinity_have_no_gradient(n, d, dtype, parts):
+    """Their probability is 0.  Neither samples without a target nor those that
+    fill the last tile change that."""
+    h, w, y, others, want = _with_minus_infinity(n, d, dtype)
+    for ignored in (0, 1):
+        loss, lse = S.softmax_loss_forward(h, w, y, gradient=True)
+        _, dw = S.softmax_loss_backward(h, w, y, lse,
+                                        torch.ones((), device="cuda"))
+        _near(dw[others], want[5], want[7], "dw")
+        assert (dw[[17, 299]] == 0).all()
+        y[::4] = -1
+        want = _reference(h, w[others], y, grad=torch.ones(()))
+
+
+@gpu
+@forms
 def test_infinite_on_both_sides(n, d, dtype, parts):
     """Infinity times -infinity is a score of -inf; of one sign, or beside an
     infinity of the other sign, the row is NaN."""
