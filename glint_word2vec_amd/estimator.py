@@ -347,7 +347,7 @@ class GlintWord2VecModel:
         """Mean -log probability of every context word within the window
         around every known word of ``sentences``, by the softmax over the
         whole vocabulary: how well the model predicts held-out text.  Needs
-        to_gpu() and a model with syn1."""
+        to_gpu() and a model with syn1, which the first call uploads."""
         if batch < 1:
             raise ValueError(f"batch must be at least 1, got {batch}")
         if self._gpu is None:
@@ -356,7 +356,10 @@ class GlintWord2VecModel:
             raise ValueError("the model has no syn1: it was saved without")
         import torch
         if not self._gpu_syn1:
-            self._gpu.load_host(self._f32(), self.syn1)
+            # syn1 alone: syn0 is what to_gpu() left, or what was made of it
+            self._gpu.syn1[:, :self.vector_size] = torch.from_numpy(
+                np.ascontiguousarray(self.syn1, dtype=np.float32)) \
+                .to(self._gpu.syn1.dtype)
             self._gpu_syn1 = True
         pairs = []
         for sent in sentences:
