@@ -346,8 +346,9 @@ class GlintWord2VecModel:
     def softmax_loss(self, sentences, batch: int = 8192) -> float:
         """Mean -log probability of every context word within the window
         around every known word of ``sentences``, by the softmax over the
-        whole vocabulary: how well the model predicts held-out text.  Needs
-        to_gpu() and a model with syn1, which the first call uploads."""
+        whole vocabulary: how well the model predicts held-out text.  The text
+        is read once, and scored ``batch`` pairs at a time as they are made.
+        Needs to_gpu() and a model with syn1, which the first call uploads."""
         if batch < 1:
             raise ValueError(f"batch must be at least 1, got {batch}")
         if self._gpu is None:
@@ -361,22 +362,38 @@ class GlintWord2VecModel:
                 np.ascontiguousarray(self.syn1, dtype=np.float32)) \
                 .to(self._gpu.syn1.dtype)
             self._gpu_syn1 = True
-        pairs = []
+        total = torch.zeros((), dtype=torch.float64, device=self._gpu.device)
+        count, held, parts = 0, 0, []
+        for pairs in self._context_pairs(sentences):
+            parts.append(pairs)
+            held += pairs.shape[1]
+            if held < batch:
+                continue
+            both = np.concatenate(parts, axis=1)
+            whole = held // batch * batch
+            for i in range(0, whole, batch):
+                total += self._pairs_loss(both[:, i:i + batch])
+            count += whole
+            held, parts = held - whole, [both[:, whole:]]
+        if held:
+            total += self._pairs_loss(np.concatenate(parts, axis=1))
+            count += held
+        return float(total) / count if count else float("nan")
+
+    def _context_pairs(self, sentences):
+        """(word, context word) pairs [2, n] of one sentence after the other,
+        both ways round."""
         for sent in sentences:
             ids = np.asarray([self.vocab[w] for w in sent if w in self.vocab],
                              dtype=np.int32)
             for o in range(1, min(self.config.window, len(ids) - 1) + 1):
-                pairs.append(np.stack([ids[:-o], ids[o:]]))
-                pairs.append(np.stack([ids[o:], ids[:-o]]))
-        if not pairs:
-            return float("nan")
-        both = torch.from_numpy(np.concatenate(pairs, axis=1)) \
-            .to(self._gpu.device)
-        total = torch.zeros((), dtype=torch.float64, device=both.device)
-        for i in range(0, both.shape[1], batch):
-            c, t = both[:, i:i + batch].unbind(0)
-            total += self._gpu.softmax_loss(c, t).double().sum()
-        return float(total) / both.shape[1]
+                yield np.stack([ids[:-o], ids[o:]])
+                yield np.stack([ids[o:], ids[:-o]])
+
+    def _pairs_loss(self, pairs):
+        import torch
+        both = torch.from_numpy(pairs).to(self._gpu.device)
+        return self._gpu.softmax_loss(both[0], both[1]).double().sum()
 
     def transform_sentences_gpu(self, sentences) -> np.ndarray:
         """Batched sentence-average transform on the GPU (ml:443-456)."""
