@@ -53,8 +53,10 @@ def build_hip_extension(name: str = "_hip_native",
     ext_suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     src = os.path.join(ROOT, "csrc", "hip", HIP_EXTENSIONS[name])
     out = os.path.join(PKG, name + ext_suffix)
+    # this file holds the compiler's switches
+    needs = (src, os.path.join(ROOT, "setup.py"))
     if not force and os.path.exists(out) and \
-            os.path.getmtime(out) > os.path.getmtime(src):
+            os.path.getmtime(out) > max(map(os.path.getmtime, needs)):
         return out
     cmd = [
         hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -75,7 +77,8 @@ class BuildExt(build_ext):
     def run(self):
         super().run()
         with ThreadPoolExecutor() as pool:      # minutes each
-            list(pool.map(build_hip_extension, HIP_EXTENSIONS))
+            list(pool.map(lambda name: build_hip_extension(
+                name, bool(self.force)), HIP_EXTENSIONS))
 
 
 setup(
