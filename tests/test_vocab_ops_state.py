@@ -10,6 +10,33 @@ U = 2.0 ** -24
 
 
 @gpu
+@pytest.mark.parametrize("count,alpha", [(40, 1e-3), (512, 5e-4)])
+def test_repeated_centers_add_up_in_bfloat16(count, alpha):
+    """Pairs of one center whose pushes are each under half a step of the row's
+    entries: the sum of them moves it."""
+    gs = _tables("bfloat16")
+    c = torch.full((count + 8,), 7)
+    c[:8] = torch.arange(20, 28)
+    t = torch.full((count + 8,), 11)
+    s0, s1 = gs.syn0[:, :52].double().cpu(), gs.syn1[:, :52].double().cpu()
+    gs.train_softmax(c, t, alpha)
+    p = torch.softmax(s0[c] @ s1.T, 1)
+    p[:, 11] -= 1
+    p = p * alpha
+    add = torch.zeros_like(s0).index_add_(0, c, p @ s1)
+    most = torch.zeros_like(s0).index_add_(0, c, p.abs() @ s1.abs())
+    # a coefficient and its pair's gradient are rounded once each, with room
+    # for the scores' error in float32; the row once, after the sum
+    off = 3 * 2.0 ** -8 * most + 2.0 ** -8 * (s0 - add).abs() * 1.01
+    got = gs.syn0[:, :52].double().cpu()
+    assert ((got - (s0 - add)).abs() <= off).all()
+    # (the row moves by far more than that)
+    assert (add[7].abs() > 4 * off[7]).sum() > 20
+    rest = [i for i in range(300) if i not in c.tolist()]
+    assert torch.equal(got[rest], s0[rest])
+
+
+@gpu
 def test_model_loss_leaves_the_table_as_it_is():
     """A table that was trained on after to_gpu() is the one that the loss is
     of, and stays."""
