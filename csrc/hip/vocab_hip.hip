@@ -24,7 +24,9 @@
 // What bounds them, measured on one card: memory gives 4.8 TB/s in a copy; a
 // loop of bf16 instructions alone runs at 2.30 PFLOP/s, one of float32
 // instructions at 155 TFLOP/s; library products reach 1.35 PFLOP/s and 153
-// TFLOP/s at 8192^3.  Figures beside the kernels are for the sizes they name.
+// TFLOP/s at 8192^3; a fill reaches 6.8 TB/s, and reads alone 5.6.  Figures
+// beside the kernels are for the sizes they name: of whole calls, or, where it
+// says so, averages of traced launches, which take up to a fifth longer.
 
 #include <hip/hip_runtime.h>
 #include <pybind11/pybind11.h>
@@ -425,8 +427,13 @@ struct Sink {
                                             int n1, bool cut, bool met) {
     const int lane = threadIdx.x & 63;
     // 16 samples x 16 table rows are 512 bytes (float32: 1 KB, or three times
-    // 512 bytes of its parts) in one piece, as a wave writes them and with every 16 bytes of one sample, as the products read
-    // them
+    // 512 bytes of its parts) in one piece, as a wave writes them and with
+    // every 16 bytes of one sample, as the products read them.
+    // bf16 rows take bf16 coefficients: the products' instructions have one type
+    // for both sides, and a second part of each coefficient would double two
+    // products.  Rounding them takes the gradient's error from 1.65e-3 of it
+    // (root mean square), which is its own rounding to bf16, to 1.72e-3 (256 x
+    // 10k x 128).  Who wants them in 32 bits calls with float32 rows.
     constexpr int es = TC == kF32 ? 4 : 2, parts = Elem<TC>::parts;
     const int in_block = (lane & 15) * (16 * es) + (lane >> 4) * (4 * es);
     auto put = [&](int i, int j, f32x4 c) {
@@ -625,7 +632,8 @@ __device__ __forceinline__ float col_scale_of(const ScoreArgs& a, int v) {
 // assembly, the compiler sees to: one between a scalar write of M0 and the load,
 // and five between a vector instruction's write of a scalar register and a load
 // with that address (base may come from v_readfirstlane).  The write of M0 is
-// one of the five, s_nop 3 the other four.
+// one of the five, s_nop 3 the other four (4096 samples, 1M x 300 bf16: 2 to 3 %
+// of the loss; the test of the built instructions' wait states looks for both).
 __device__ __forceinline__ void load_lds16(const char* p, uint32_t offset, uint32_t lds) {
   const uint64_t at = (uint64_t)p;
   const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
@@ -671,12 +679,12 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // different rows of the tile.
 // 8-bit rows are brought to bf16 with their scale: exact, while the instructions
 // on 8-bit operands lose bits inside (1.5e-5 to 2.8e-5 of the result).
-//   4096 samples, 1M x 300 bf16: 2.28 ms, 1.08 PFLOP/s (the matrix unit and
-//     the exponentials take turns); coefficients alone 3.1 ms
-//   1 sample: 107 us, 5.6 TB/s, bound by memory
+//   4096 samples, 1M x 300 bf16: 2.30 ms, 1.07 PFLOP/s (the matrix unit and
+//     the exponentials take turns); coefficients alone 3.3 ms traced
+//   1 sample: 116 us, 5.2 TB/s, bound by memory
 //   4096 queries, 200k x 300 in 8 bits, float32 scores: 0.77 ms
 //     (4.3 TB/s of stores, which bound it: a fill reaches 6.8)
-//   1 query of 1M x 300 in 8 bits: 57 us, 5.4 TB/s
+//   1 query of 1M x 300 in 8 bits: 58 us traced, 5.2 TB/s
 constexpr int resident_rows(int ks, int use, int wn, bool fp8) {
   // with stores, tiles of at most 20 KB: four of them fit, so that the stores
   // of several tiles, which are waited for in order with the loads, may be on
@@ -878,10 +886,10 @@ __global__ __launch_bounds__(256, 2) void resident_kernel(ScoreArgs a) {
 // work.  Both sides' rows start at multiples of 16 bytes; 8-bit table rows are
 // converted when they are read from LDS, and their scales lie by block of
 // columns, then row.
-//   2047 samples, 100001 x 1024 bf16, coefficients: 0.54 ms, 0.78 PFLOP/s
-//     (LDS and barriers bound it)
-//   2047 samples, 30000 x 1024 float32 in parts, loss: 673 us, 187 TFLOP/s or
-//     1.12 PFLOP/s of bf16 (half of the matrix unit's time; all waves of a CU
+//   2047 samples, 100001 x 1024 bf16, coefficients: 0.57 ms traced, 0.73
+//     PFLOP/s (LDS and barriers bound it)
+//   2047 samples, 30000 x 1024 float32 in parts, loss: 651 us, 193 TFLOP/s or
+//     1.16 PFLOP/s of bf16 (half of the matrix unit's time; all waves of a CU
 //     share one barrier a step)
 //   2000 samples, 3613 x 100 float32: 24 us, 60 TFLOP/s, one round of
 //     workgroups and its start
@@ -1076,7 +1084,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
   if constexpr (kMid) {
     // The same with one product a step: its second half runs beside the next
     // step's first reads and the loads of four steps on (2047 samples, 100001 x
-    // 1024: loss 512 us, with the barrier at the step's start 527).
+    // 1024: loss 512 us traced, with the barrier at the step's start 527).
     static_assert(kMore == 0 && kEach == MR, "");
     u32x4 fa[MR], fb[NS], na[MR];
     auto read_a = [&](int buf) INLINE {
@@ -1213,7 +1221,7 @@ __global__ __launch_bounds__(64 * WV * WN, 2) void tile_kernel(ScoreArgs a) {
 
 // Few samples: bound by the bytes of the table, which go from memory to the
 // registers of the one wave that needs them (7 samples, 201905 x 860 float32:
-// 160 us, 4.3 TB/s).  A wave takes 16 rows at a time, eight loads of 16 bytes a
+// 157 us, 4.4 TB/s).  A wave takes 16 rows at a time, eight loads of 16 bytes a
 // lane ahead of the eight at work; the samples lie in LDS as the instruction
 // takes them.  Any type, size and alignment; VEC:
 // table rows start at multiples of 16 bytes.
@@ -1468,7 +1476,7 @@ __global__ __launch_bounds__(256) void pack_kernel(
 }
 
 // Bound by LDS and the matrix unit: 4096 samples, 1M x 300 bf16: 3.0 ms for
-// dh and 2.7 ms for dw, 0.83 and 0.91 PFLOP/s.
+// dh and 2.8 ms for dw, both traced, 0.83 and 0.89 PFLOP/s.
 //
 // Eight waves: WR times 16 J rows r, 8 / WR times 16 ND columns d.  With 256
 // rows and 32 ND columns narrow tables are read once and the coefficients, the
@@ -1717,7 +1725,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(
 // A workgroup takes 64 blocks of 128 columns that follow each other, four to
 // a group of lanes with all loads first; the position of the first one is the
 // only division by a length of 64 bits.  Bound by memory: 1M x 300 bf16 in
-// 248 us, 3.7 TB/s (read and written).
+// 252 us traced, 3.6 TB/s (read and written).
 template <int T, bool TO_BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(
     int64_t block0, Rows x, int blocks, char* values, int64_t ldv, uint8_t* scales, int64_t lds) {
@@ -1791,8 +1799,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(
 }
 
 // 8 columns to a lane, four times: rows of bf16 or f32 that follow each other
-// without a gap are written in one stream.  Bound by memory: 1M x 300 to
-// bfloat16 in 295 us, 3.1 TB/s, as lines of the output are shared by two rows.
+// without a gap are written in one stream.  1M x 300 to bfloat16 in 299 us
+// traced, 3.0 TB/s: where the columns are no multiple of 8, as there, a lane
+// makes two stores of 8 bytes instead of one of 16.
 template <int TO>
 __global__ __launch_bounds__(256) void dequantize_kernel(int64_t block0, Rows x, int cols, char* out,
                                                         int64_t ldo) {
@@ -2377,7 +2386,7 @@ __global__ __launch_bounds__(256) void turn_scales_kernel(
 //   block of 128 columns and row, rows rounded up to 256
 //   m > 160: wide, bf16 [piece][k rounded up to 64].  Converting 8-bit rows in
 //   the product costs each workgroup registers that the product wants (1023 x
-//   150001 x 1024: 0.73 ms; converted first, a piece at a time, 0.50 ms)
+//   150001 x 1024: 0.73 ms; converted first, a piece at a time, 0.55 ms)
 static void matmul_rows(uintptr_t a_ptr, int64_t lda, int64_t m, uintptr_t values, int64_t ldv,
                         uintptr_t scales, int64_t lds, int64_t n, int64_t k, uintptr_t col_scale,
                         uintptr_t out, int out_bf16, uintptr_t turned, uintptr_t wide,

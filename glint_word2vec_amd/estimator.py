@@ -329,7 +329,9 @@ class GlintWord2VecModel:
         and sentence-average transform (pull_average kernel) then run
         device-side — the reference's server-side model ops.
         ``scores="fp8"``: findSynonyms scores an 8-bit copy of the table with
-        8-bit queries (ops/fp8.py; a value is off by 2^-4 at most)."""
+        8-bit queries (ops/fp8.py; a value is off by 2^-4 of it at most, small
+        ones by 2^-10 of their block's scale).  The copy is of the table as it
+        is then, and lies beside it: less to read, not less memory."""
         from .ops.gpu import GpuSgns
         if scores not in (None, "fp8"):
             raise ValueError(f"scores must be None or 'fp8', got {scores!r}")

@@ -4,8 +4,8 @@ matrix product, by hand-written kernels.
 A row's block of up to 128 columns is held as e4m3 values times one power of
 two, the smallest that keeps the block's largest value within 448.  Scaling by
 a power of two rounds nothing, so a value is off by at most half a step of
-e4m3: 2^-4 relative, or 2^-10 of the scale where it is that small.  A table
-takes half the memory and bandwidth of bfloat16.
+e4m3: 2^-4 relative, or 2^-10 of the scale where it is that small.  8-bit rows
+take half the memory and bandwidth of bfloat16.
 
 Every function runs on the current stream of the tensors' device, allocates
 from torch's allocator, and does not synchronise.
@@ -108,7 +108,8 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
 def dequantize_rows(q: Fp8Rows, dtype: torch.dtype = torch.float32
                     ) -> torch.Tensor:
     """The values that 8-bit rows stand for, exactly: bfloat16 holds them as
-    float32 does."""
+    float32 does for scales from 2^-124 on (quantize_rows makes none below
+    2^-120), and rounds what smaller ones leave below 2^-133."""
     q = _check_rows("q", q)
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"unsupported dtype {dtype}: float32 or bfloat16")
@@ -127,7 +128,8 @@ def matmul_rows(a: Union[torch.Tensor, Fp8Rows], b: Fp8Rows,
     """[M, K] rows times [N, K] rows, transposed: out[m, n] = <a_m, b_n>, times
     ``col_scale[n]`` (float32 [N]) where it is given, as [M, N] of ``out_dtype``
     (float32 or bfloat16).  ``a`` is held in 8 bits like ``b``; rows of floats
-    are brought to that first.  Products are exact and sums are in 32 bits."""
+    are brought to that first.  Products of what dequantize_rows gives as
+    bfloat16 are exact, and sums are in 32 bits."""
     b = _check_rows("b", b)
     if isinstance(a, Fp8Rows):
         a = _check_rows("a", a)

@@ -308,9 +308,14 @@ class GpuSgns:
                       alpha: float) -> torch.Tensor:
         """One SGD step on the sum of softmax_loss over the pairs, from the
         tables as they are before it; returns the losses [N].  Exact where
-        train_batch samples: every word's output row moves.  Repeated centers
-        add up, in a fixed order.  Pairs that are no words, as in
-        softmax_loss, move nothing."""
+        train_batch samples: every word's output row has its gradient.
+        Repeated centers add up, in a fixed order.  Pairs that are no words,
+        as in softmax_loss, move nothing.
+
+        A bfloat16 table is rounded to nearest after the step, as train_batch
+        rounds it: a change under half a step of an entry, 2^-9 to 2^-8 of it,
+        is lost.  With small rates that is most of what pushes away the words
+        that are no targets; float32 tables keep it."""
         from .softmax import softmax_loss_backward, softmax_loss_forward
         centers, targets = self._pairs(centers, targets)
         h = self.syn0[centers][:, :self.dim]

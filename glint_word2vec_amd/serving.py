@@ -117,7 +117,8 @@ class ShardedWord2VecModel:
         """Streaming sharded load (the PS-side load, mllib:717-722).
         Host RSS stays O(block_rows*dim) + the word index (~24 B/word).
         ``scores="fp8"``: findSynonyms scores an 8-bit copy of the shard with
-        8-bit queries (ops/fp8.py; GPU only)."""
+        8-bit queries (ops/fp8.py; GPU only).  The copy lies beside the shard:
+        less to read, not less memory."""
         if scores not in (None, "fp8"):
             raise ValueError(f"scores must be None or 'fp8', got {scores!r}")
         rank, world = comm.init_from_env()
