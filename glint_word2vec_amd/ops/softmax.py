@@ -269,8 +269,10 @@ def softmax_loss(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
     target outside [0, V) cannot be refused without waiting for the GPU: its
     loss is NaN, and it gives no gradient.  A score of NaN or +inf makes its row
     NaN, and so does one of -inf for every word; otherwise a score of -inf is a
-    probability of 0.  A call that needs gradients is refused while a graph is
-    being captured: softmax_loss_forward and softmax_loss_backward can be."""
+    probability of 0.  A score past float32's range counts as infinite, or, where
+    float32 goes in parts, as NaN.  A call that needs gradients is refused while
+    a graph is being captured: softmax_loss_forward and softmax_loss_backward
+    can be."""
     if reduction not in _REDUCE:
         raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got "
                          f"{reduction!r}")
